@@ -344,10 +344,8 @@ def work(case):
 def _e4m3_exact(r):
     """The e4m3 value nearest to r (ties to even), as float64: steps of 2^(e-3) for r in [2^e, 2^(e+1)), of 2^-9 below 2^-6."""
     a = r.double().abs()
-    e = torch.floor(torch.log2(a.clamp(min=2.0 ** -6))).clamp(min=-6)
-    e = torch.where(torch.ldexp(torch.ones_like(e), e + 1) <= a, e + 1, e)
-    e = torch.where(torch.ldexp(torch.ones_like(e), e).clamp(min=2.0 ** -6) > a.clamp(min=2.0 ** -6), e - 1, e)
-    step = torch.ldexp(torch.ones_like(e), e - 3)
+    e = torch.frexp(a.clamp(min=2.0 ** -6))[1].long() - 1
+    step = ((e - 3 + 1023) << 52).view(torch.float64)  # 2^(e - 3) by its bits
     return torch.copysign((torch.round(a / step) * step).clamp(max=F8_MAX), r.double())
 
 
