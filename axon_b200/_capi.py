@@ -38,6 +38,19 @@ BLOCK_BYTES = {QuantFormat.Q8_0: 34, QuantFormat.Q4_0: 18, QuantFormat.Q2_K: 84,
                QuantFormat.Q4_K: 144, QuantFormat.Q5_K: 176, QuantFormat.Q6_K: 210}
 
 
+class DType(enum.IntEnum):
+    """enum axq_dtype: element types of the 8-bit floating point and
+    mixture-of-experts entry points."""
+
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+    F8 = 3
+
+
+F8_BLOCK = 128  # columns (and, for weights, rows) that share one e4m3 scale
+
+
 class Status(enum.IntEnum):
     OK = 0
     ERR_INVALID = 1
@@ -98,6 +111,11 @@ SIGNATURES = {
     "axq_symm_wait_many": (ctypes.c_int, [_vp, ctypes.c_int, _vp]),
     "axq_symm_wait": (ctypes.c_int, [_vp, _vp]),
     "axq_matmul_f32": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "axq_quantize_f8": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _i64, _vp, _i64, _i64, ctypes.c_int, _vp]),
+    "axq_dequantize_f8": (ctypes.c_int, [_vp, _i64, _vp, ctypes.c_int, _vp, _i64, _i64, _vp]),
+    "axq_linear_f8_workspace_size": (_sz, [ctypes.c_int, _i64, _i64]),
+    "axq_linear_f8": (ctypes.c_int, [_vp, _i64, _vp, ctypes.c_int, _vp, _i64, _vp, _vp, ctypes.c_int, _vp, _i64, _i64,
+                                     _i64, _vp, _sz, _vp]),
     "axq_axon_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_uint32)]),
     "axq_axon_info": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp]),
     "axq_axon_read": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp, _sz, _vp]),

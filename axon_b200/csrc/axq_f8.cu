@@ -1,0 +1,226 @@
+// e4m3 packing: src[rows x cols] (fp32, fp16 or bf16) -> codes and one fp32
+// scale per block of R rows x 128 columns, R = 1 (activations) or 128
+// (weights):
+//   scale = RN(max|x| / 448),  code = e4m3(RN(x / scale)),
+// both roundings to nearest even, codes saturating; a block whose scale is 0
+// has codes 0.  NaN elements keep NaN codes and do not enter the maximum; an
+// infinity makes its block's scale infinite, so the block decodes to NaN.
+//
+// HBM-bound: every element is read once (the block stays in registers between
+// the maximum and the rounding) and one byte written.
+#include <algorithm>
+
+#include "axq_common.cuh"
+#include "axq_f8.cuh"
+#include "axq_internal.h"
+#include "axq_ptx.cuh"
+
+namespace axq {
+namespace {
+
+// Elements c0 .. c0+7 of a row (zero past `cols`).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int64_t c0, int64_t cols, float (&v)[8]) {
+    if (VEC && c0 + 8 <= cols) {
+        load8(row + c0, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? Elem<T>::get(row[c0 + i]) : 0.0f;
+    }
+}
+
+// 1 x 128 blocks: 16 lanes hold a block, 8 elements each; a half warp takes
+// kUnroll blocks at once so that their loads are in flight together.
+constexpr int kPackUnroll = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) f8_pack_rows_kernel(const T* __restrict__ src, uint8_t* __restrict__ codes,
+                                                           int64_t ld, float* __restrict__ scales, int64_t rows,
+                                                           int64_t cols, int nkb, int* __restrict__ err) {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // status word of the call this packing opens
+    // blocks number fewer than 2^31 (checked on the host), so 32-bit divisions serve
+    const uint32_t items = static_cast<uint32_t>(rows * nkb);
+    const uint32_t half = (blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+    const uint32_t halves = gridDim.x * blockDim.x >> 4;
+    const int l = threadIdx.x & 15;
+    for (uint32_t it0 = half; (it0 & ~1u) < items; it0 += halves * kPackUnroll) {
+        // both halves of a warp stay in the loop together (the shuffles are warp-wide)
+        float v[kPackUnroll][8];
+#pragma unroll
+        for (int u = 0; u < kPackUnroll; ++u) {
+            const uint32_t it = it0 + u * halves;
+            const uint32_t r = it / static_cast<uint32_t>(nkb);
+            const int64_t c0 = static_cast<int64_t>(it - r * nkb) * kF8Block + 8 * l;
+            if (it < items) {
+                load_row8<T, VEC>(src + static_cast<int64_t>(r) * cols, c0, cols, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kPackUnroll; ++u) {
+            const uint32_t it = it0 + u * halves;
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[u][i]));
+#pragma unroll
+            for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+            if (it >= items) continue;
+            const uint32_t r = it / static_cast<uint32_t>(nkb);
+            const uint32_t kb = it - r * nkb;
+            const float s = __fdiv_rn(m, kF8Max);
+            const F8Div div(s);
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[i] = cvt_e4m3x2(div(v[u][4 * i]), div(v[u][4 * i + 1])) |
+                       (cvt_e4m3x2(div(v[u][4 * i + 2]), div(v[u][4 * i + 3])) << 16);
+            const int64_t c0 = static_cast<int64_t>(kb) * kF8Block + 8 * l;
+            if (c0 < ld) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * ld + c0) = make_uint2(w[0], w[1]);
+            if (l == 0) scales[it] = s;
+        }
+    }
+}
+
+// 128 x 128 blocks: one CTA per block, 16 rows per warp, 4 elements per lane
+// and row, all 64 values of a thread in registers.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) f8_pack_blocks_kernel(const T* __restrict__ src, uint8_t* __restrict__ codes,
+                                                             int64_t ld, float* __restrict__ scales, int64_t rows,
+                                                             int64_t cols, int nkb) {
+    __shared__ float red[8];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t rb = blockIdx.x / static_cast<uint32_t>(nkb);
+    const int kb = static_cast<int>(blockIdx.x - static_cast<uint32_t>(rb) * nkb);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t r0 = rb * kF8Block + 16 * warp, c0 = static_cast<int64_t>(kb) * kF8Block + 4 * lane;
+    float v[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int64_t r = r0 + j;
+        const T* p = src + r * cols + c0;
+        if (VEC && r < rows && c0 + 4 <= cols) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 a = *reinterpret_cast<const float4*>(p);
+                v[j][0] = a.x; v[j][1] = a.y; v[j][2] = a.z; v[j][3] = a.w;
+            } else {
+                const uint2 a = *reinterpret_cast<const uint2*>(p);
+                T h[4];
+                memcpy(h, &a, 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[j][i] = Elem<T>::get(h[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][i] = (r < rows && c0 + i < cols) ? Elem<T>::get(p[i]) : 0.0f;
+        }
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(v[j][i]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+    const float s = __fdiv_rn(m, kF8Max);
+    const F8Div div(s);
+    if (threadIdx.x == 0) scales[blockIdx.x] = s;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int64_t r = r0 + j;
+        const uint32_t w = cvt_e4m3x2(div(v[j][0]), div(v[j][1])) | (cvt_e4m3x2(div(v[j][2]), div(v[j][3])) << 16);
+        if (r < rows && c0 < ld) *reinterpret_cast<uint32_t*>(codes + r * ld + c0) = w;
+    }
+}
+
+// dst = code * scale, one rounding; 4 elements per thread.
+__global__ void __launch_bounds__(256) f8_dequant_kernel(const uint8_t* __restrict__ codes, int64_t ld,
+                                                         const float* __restrict__ scales, int block_rows,
+                                                         float* __restrict__ dst, int64_t rows, int64_t cols, int nkb) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t quads = (cols + 3) / 4, n = rows * quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t r = i / quads, c = 4 * (i - r * quads);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + r * ld + c);
+        const float s = scales[r / block_rows * nkb + c / kF8Block];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (c + u >= cols) break;
+            __nv_fp8_e4m3 q;
+            q.__x = static_cast<__nv_fp8_storage_t>(w >> (8 * u));
+            dst[r * cols + c + u] = __fmul_rn(static_cast<float>(q), s);
+        }
+    }
+}
+
+// y = bias (or 0) on every row: a product over no columns.
+template <typename TY>
+__global__ void f8_fill_bias_kernel(TY* __restrict__ y, const float* __restrict__ bias, int64_t M, int64_t n,
+                                    int* __restrict__ err) {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+        y[i] = Elem<TY>::put(bias ? bias[i % M] : 0.0f);
+}
+
+}  // namespace
+
+cudaError_t f8_fill_bias_dispatch(int dtype, void* y, const float* bias, int64_t M, int64_t N, int* err, cudaStream_t s) {
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const int64_t grid = std::min<int64_t>((M * N + 255) / 256, int64_t(device_sm_count()) * 8);
+        cudaError_t e = launch_pdl(f8_fill_bias_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s,
+                                   static_cast<T*>(y), bias, M, M * N, err);
+        return e == cudaSuccess ? cudaGetLastError() : e;
+    });
+}
+
+cudaError_t f8_pack_dispatch(int dtype, const void* src, void* codes, int64_t ld, float* scales, int64_t rows,
+                             int64_t cols, int block_rows, int* err, cudaStream_t s) {
+    const int nkb = static_cast<int>((cols + kF8Block - 1) / kF8Block);
+    auto* out = static_cast<uint8_t*>(codes);
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const T* p = static_cast<const T*>(src);
+        // 16-byte loads (8 of a 16-bit type, 4 of fp32 in the block kernel's 8-byte ones) need every row aligned
+        const bool vec = reinterpret_cast<uintptr_t>(src) % 16 == 0 && (cols * sizeof(T)) % 16 == 0;
+        if (block_rows == 1) {
+            const int64_t halves = (rows * nkb + kPackUnroll - 1) / kPackUnroll;
+            const int64_t grid = std::min<int64_t>((halves + 15) / 16, int64_t(device_sm_count()) * 8);
+            auto k = vec ? f8_pack_rows_kernel<T, true> : f8_pack_rows_kernel<T, false>;
+            cudaError_t e = launch_pdl(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, p, out, ld, scales, rows,
+                                       cols, nkb, err);
+            return e == cudaSuccess ? cudaGetLastError() : e;
+        }
+        const int64_t grid = (rows + kF8Block - 1) / kF8Block * nkb;
+        auto k = vec ? f8_pack_blocks_kernel<T, true> : f8_pack_blocks_kernel<T, false>;
+        cudaError_t e = launch_pdl(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, p, out, ld, scales, rows, cols,
+                                   nkb);
+        return e == cudaSuccess ? cudaGetLastError() : e;
+    });
+}
+
+cudaError_t f8_dequant_dispatch(const void* codes, int64_t ld, const float* scales, int block_rows, float* dst,
+                                int64_t rows, int64_t cols, cudaStream_t s) {
+    const int nkb = static_cast<int>((cols + kF8Block - 1) / kF8Block);
+    const int64_t n = rows * ((cols + 3) / 4);
+    const int64_t grid = std::min<int64_t>((n + 255) / 256, int64_t(device_sm_count()) * 16);
+    cudaError_t e = launch_pdl(f8_dequant_kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s,
+                               static_cast<const uint8_t*>(codes), ld, scales, block_rows, dst, rows, cols, nkb);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+}  // namespace axq

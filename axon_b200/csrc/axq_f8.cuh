@@ -1,0 +1,95 @@
+// Element types of the float tensors the 8-bit floating point and
+// mixture-of-experts entry points take, and their conversions.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "../../include/axq.h"
+
+namespace axq {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    __device__ __forceinline__ static float get(float v) { return v; }
+    __device__ __forceinline__ static float put(float v) { return v; }
+};
+template <> struct Elem<__half> {
+    __device__ __forceinline__ static float get(__half v) { return __half2float(v); }
+    __device__ __forceinline__ static __half put(float v) { return __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+    __device__ __forceinline__ static float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+    __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+
+inline int host_dtype_size(int dtype) {
+    return dtype == AXQ_DT_F32 ? 4 : (dtype == AXQ_DT_F16 || dtype == AXQ_DT_BF16) ? 2 : 0;
+}
+
+// f.template operator()<T>() for the C type of `dtype` (already checked).
+template <class Fn>
+cudaError_t with_dtype(int dtype, Fn&& f) {
+    switch (dtype) {
+        case AXQ_DT_F32: return f(static_cast<float*>(nullptr));
+        case AXQ_DT_F16: return f(static_cast<__half*>(nullptr));
+        default: return f(static_cast<__nv_bfloat16*>(nullptr));
+    }
+}
+
+// Eight consecutive elements at p (16-byte aligned) as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        T h[8];
+        memcpy(h, w, 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::get(h[i]);
+    }
+}
+
+constexpr float kF8Max = 448.0f;  // largest e4m3 value
+constexpr int kF8Block = 128;     // columns (and, for weights, rows) that share one scale
+
+// Two e4m3 codes (RNE, saturating; NaN stays NaN): a in the low byte.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// x / s rounded to nearest for many x and one s.  With y = RN(1/s),
+// q = RN(x*y) and r = x - q*s (exact in one FMA), RN(q + r*y) is the
+// correctly rounded quotient unless s's significand is all ones (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990): two FMAs and a product instead of a division.  Where s
+// is outside 2^-90 .. 2^90 (r might not be exact) or all ones, the division
+// itself is used.  |x| < 2^-100 then gives a quotient below 2^-10, whose code
+// is 0 either way.
+struct F8Div {
+    float s, y;
+    bool fast;
+    __device__ __forceinline__ explicit F8Div(float scale) : s(scale) {
+        const uint32_t b = __float_as_uint(scale);
+        fast = scale > 8.0779357e-28f && scale < 1.2379400e27f && (b & 0x7FFFFFu) != 0x7FFFFFu;
+        y = __fdiv_rn(1.0f, scale);
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        if (fast) {
+            const float q = __fmul_rn(x, y);
+            return __fmaf_rn(-__fmaf_rn(q, s, -x), y, q);  // in this order -0 stays -0
+        }
+        if (s == 0.0f) return x != x ? x : 0.0f;
+        return __fdiv_rn(x, s);
+    }
+};
+
+}  // namespace axq

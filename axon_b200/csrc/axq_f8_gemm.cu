@@ -1,0 +1,560 @@
+// y[N x M] = X . W^T (+ bias) on e4m3 operands with one fp32 scale per 1 x 128
+// block of X and per 128 x 128 block of W:
+//   y[t][m] = sum_kb sx[t][kb] * sw[m/128][kb] * P_kb[t][m],
+//   P_kb[t][m] = sum over the 128 k of block kb of x[t][k] * w[m][k].
+//
+// P_kb is four tcgen05 MMAs of K = 32 into TMEM (fp32); the scales change
+// every 128 k, so each P_kb leaves TMEM and is added with its scale to fp32
+// registers while the tensor core works on the next block in another TMEM
+// buffer.  Tiles come by tensor-map copies in the 128-byte swizzle; copies
+// past the edges read zeros, so any M, N and K need no other masking than
+// that of the stores.
+//
+// Two forms:
+//  * f8_pair_kernel (many tokens): a CTA pair computes 256 tokens x BN
+//    weight rows with one cta_group::2 MMA; each CTA holds 128 tokens (TMEM
+//    lanes) and loads half of the weight rows, so the weights cross from L2
+//    once per pair.  A thread owns a token's row, so its scale is one product
+//    per 128 k.
+//  * f8_skinny_kernel (few tokens): 128 weight rows are the MMA's M side, NT
+//    >= N tokens its N side, and a cluster splits K; its CTAs' sums are joined
+//    through distributed shared memory in rank order.  HBM-bound on W.
+#include <algorithm>
+#include <cuda.h>
+
+#include "axq_common.cuh"
+#include "axq_f8.cuh"
+#include "axq_internal.h"
+#include "axq_ptx.cuh"
+#include "axq_tc.cuh"
+
+namespace axq {
+namespace {
+
+constexpr int kMaxF8Stages = 8;
+
+struct F8Args {
+    const float* sx;
+    const float* sw;
+    const float* bias;
+    void* y;
+    int64_t M, N;
+    int nkb;
+    int nbuf;    // TMEM buffers
+    int stages;
+    int tiles_n, tiles_m;  // pair kernel: token tiles, weight-row tiles
+    int* err;
+};
+
+struct F8Bars {
+    uint64_t full[kMaxF8Stages], empty[kMaxF8Stages];
+    uint64_t acc_full[4], acc_empty[4];
+    uint32_t tmem;
+    int abort;
+};
+
+// Bounded wait; on giving up sets the CTA's abort flag and the status word.
+__device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, F8Bars* b, int* err) {
+    if (mbar_wait_bounded(bar, parity, &b->abort)) return true;
+    *const_cast<volatile int*>(&b->abort) = 1;
+    if (err) atomicExch(err, 1);
+    return false;
+}
+
+// Eight values to y in its type (one or two 16-byte stores).
+template <typename TY>
+__device__ __forceinline__ void store8(TY* p, const float* v) {
+    if constexpr (sizeof(TY) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        TY h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = Elem<TY>::put(v[i]);
+        uint4 w;
+        memcpy(&w, h, 16);
+        *reinterpret_cast<uint4*>(p) = w;
+    }
+}
+
+constexpr int kPairThreads = 320;  // producer warp, MMA warp, eight epilogue warps
+
+template <int BN, typename TY>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    f8_pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, F8Args a) {
+    constexpr int kXBytes = 128 * 128;       // this CTA's 128 tokens x 128 k
+    constexpr int kWBytes = (BN / 2) * 128;  // this CTA's half of the weight rows
+    constexpr int kStage = kXBytes + kWBytes;
+    constexpr int kCols = BN / 2;            // accumulator columns of a thread
+    constexpr uint32_t kIdesc = idesc_e4m3_f32(BN, 256);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* stage0 = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    __shared__ F8Bars bars;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMaxF8Stages; ++i) {
+            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bars.acc_full[i], 1);
+            mbar_init(&bars.acc_empty[i], 16);  // eight epilogue warps of each CTA
+        }
+        bars.abort = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&mx);
+        prefetch_tensormap(&mw);
+    }
+    if (warp == 1) tmem_alloc_cg<2>(&bars.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem;
+    const int ntiles = a.tiles_n * a.tiles_m;
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            pdl_wait();
+            int s = 0;
+            uint32_t par = 0;
+            bool ok = true;
+            int64_t issued = 0;
+            for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+                // token tiles run fastest: the pairs at work share few weight tiles
+                const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
+                const int xr = tn * 256 + static_cast<int>(rank) * 128;
+                const int wr = tm * BN + static_cast<int>(rank) * (BN / 2);
+                for (int kb = 0; kb < a.nkb; ++kb) {
+                    ok = f8_wait(&bars.empty[s], par ^ 1, &bars, a.err);
+                    if (!ok) break;
+                    if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * kStage);
+                    const uint32_t fb = cluster_addr(&bars.full[s], 0);
+                    uint8_t* st = stage0 + s * kStage;
+                    tma_load_2d_pair(st, &mx, kb * 128, xr, fb);
+                    tma_load_2d_pair(st + kXBytes, &mw, kb * 128, wr, fb);
+                    ++issued;
+                    if (++s == a.stages) {
+                        s = 0;
+                        par ^= 1;
+                    }
+                }
+            }
+            if (!ok && rank == 0) {
+                // copies still in flight land before the pair's shared memory goes away
+                const int64_t from = issued > a.stages ? issued - a.stages : 0;
+                for (int64_t i = from; i < issued; ++i)
+                    mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int s = 0, b = 0;
+            uint32_t par = 0, bpar = 0;
+            bool ok = true;
+            for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+                for (int kb = 0; kb < a.nkb; ++kb) {
+                    ok = f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) &&
+                         f8_wait(&bars.full[s], par, &bars, a.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t xs = smem_u32(stage0 + s * kStage);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_e4m3<2>(tmem + b * BN, smem_desc_sw128(xs + 32 * k), smem_desc_sw128(xs + kXBytes + 32 * k),
+                                    kIdesc, k > 0);
+                    mma_commit_pair(&bars.empty[s]);
+                    mma_commit_pair(&bars.acc_full[b]);
+                    if (++s == a.stages) {
+                        s = 0;
+                        par ^= 1;
+                    }
+                    if (++b == a.nbuf) {
+                        b = 0;
+                        bpar ^= 1;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3, g = (warp - 2) >> 2;
+        pdl_wait();
+        int b = 0;
+        uint32_t bpar = 0;
+        bool ok = true;
+        TY* const y = static_cast<TY*>(a.y);
+        const bool vec = (a.M * sizeof(TY)) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+        for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+            const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
+            const int64_t t = static_cast<int64_t>(tn) * 256 + rank * 128 + 32 * q + lane;
+            const int64_t m0 = static_cast<int64_t>(tm) * BN + g * kCols;
+            const float* sx = a.sx + (t < a.N ? t : 0) * a.nkb;
+            const float* sw = a.sw + (m0 < a.M ? m0 / 128 : 0) * a.nkb;
+            float acc[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+            float nx = __ldg(sx), nw = __ldg(sw);
+            for (int kb = 0; kb < a.nkb; ++kb) {
+                const float sc = nx * nw;
+                if (kb + 1 < a.nkb) {
+                    nx = __ldg(sx + kb + 1);
+                    nw = __ldg(sw + kb + 1);
+                }
+                ok = f8_wait(&bars.acc_full[b], bpar, &bars, a.err);
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * BN + g * kCols;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    float v[32];
+                    tmem_ldw32(ta + c, v);
+                    if (c + 32 == kCols) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(cluster_addr(&bars.acc_empty[b], 0));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(v[i], sc, acc[c + i]);
+                }
+                if (++b == a.nbuf) {
+                    b = 0;
+                    bpar ^= 1;
+                }
+            }
+            if (!ok) break;
+            if (t < a.N) {
+                TY* yr = y + t * a.M + m0;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 8) {
+                    if (m0 + c >= a.M) break;
+                    if (a.bias) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (m0 + c + i < a.M) acc[c + i] += __ldg(a.bias + m0 + c + i);
+                    }
+                    if (vec && m0 + c + 8 <= a.M) {
+                        store8(yr + c, acc + c);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (m0 + c + i < a.M) yr[c + i] = Elem<TY>::put(acc[c + i]);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // neither CTA's barriers, shared memory or TMEM goes away under the other
+    pdl_launch_dependents();
+    if (warp == 1) tmem_dealloc_cg<2>(tmem, 512);
+}
+
+// ---- few tokens ---------------------------------------------------------------
+
+constexpr int skinny_warps(int nt) { return nt > 64 ? 8 : 4; }
+
+template <int NT, typename TY>
+__global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
+    f8_skinny_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, F8Args a, int splits) {
+    constexpr int kEpi = skinny_warps(NT);
+    constexpr int kCols = NT / (kEpi / 4);
+    constexpr int kWBytes = 128 * 128, kXBytes = NT * 128, kStage = kWBytes + kXBytes;
+    constexpr int kBuf = 2;
+    constexpr uint32_t kTmem = kBuf * NT <= 32 ? 32 : kBuf * NT;
+    constexpr uint32_t kIdesc = idesc_e4m3_f32(NT, 128);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* stage0 = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    float* sxs = reinterpret_cast<float*>(stage0 + a.stages * kStage);  // [kb][NT] scales of X
+    float* red = reinterpret_cast<float*>(stage0);                      // [NT][128] sums, after the last MMA
+    __shared__ F8Bars bars;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int mt = blockIdx.x / splits, rank = blockIdx.x - mt * splits;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(a.nkb) * rank / splits);
+    const int nk = static_cast<int>(static_cast<int64_t>(a.nkb) * (rank + 1) / splits) - kb0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMaxF8Stages; ++i) {
+            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+        }
+        for (int i = 0; i < kBuf; ++i) {
+            mbar_init(&bars.acc_full[i], 1);
+            mbar_init(&bars.acc_empty[i], kEpi);
+        }
+        bars.abort = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&mx);
+        prefetch_tensormap(&mw);
+    }
+    if (warp == 1) tmem_alloc(&bars.tmem, kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // The packing of X, launched before this kernel, let it start only
+            // after everything before the packing had finished, so W is there;
+            // X is waited for.
+            const int first = min(nk, a.stages);
+            for (int i = 0; i < first; ++i) {
+                mbar_arrive_expect_tx(&bars.full[i], kStage);
+                tma_load_2d(stage0 + i * kStage, &mw, (kb0 + i) * 128, mt * 128, &bars.full[i]);
+            }
+            pdl_wait();
+            for (int i = 0; i < first; ++i)
+                tma_load_2d(stage0 + i * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[i]);
+            int s = 0;
+            uint32_t par = 0;
+            bool ok = true;
+            int issued = first;
+            for (int i = first; i < nk; ++i) {
+                ok = f8_wait(&bars.empty[s], par, &bars, a.err);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&bars.full[s], kStage);
+                tma_load_2d(stage0 + s * kStage, &mw, (kb0 + i) * 128, mt * 128, &bars.full[s]);
+                tma_load_2d(stage0 + s * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[s]);
+                ++issued;
+                if (++s == a.stages) {
+                    s = 0;
+                    par ^= 1;
+                }
+            }
+            if (!ok)  // copies still in flight land before the shared memory goes away
+                for (int i = max(0, issued - a.stages); i < issued; ++i)
+                    mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0, b = 0;
+            uint32_t par = 0, bpar = 0;
+            for (int i = 0; i < nk; ++i) {
+                if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err))
+                    break;
+                tc_fence_after();
+                const uint32_t ws = smem_u32(stage0 + s * kStage);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mma_e4m3<1>(tmem + b * NT, smem_desc_sw128(ws + 32 * k), smem_desc_sw128(ws + kWBytes + 32 * k), kIdesc,
+                                k > 0);
+                mma_commit(&bars.empty[s]);
+                mma_commit(&bars.acc_full[b]);
+                if (++s == a.stages) {
+                    s = 0;
+                    par ^= 1;
+                }
+                if (++b == kBuf) {
+                    b = 0;
+                    bpar ^= 1;
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3, g = (warp - 2) >> 2;
+        const int et = threadIdx.x - 64;
+        pdl_wait();
+        for (int i = et; i < nk * NT; i += 32 * kEpi) {
+            const int n = i / nk, k = i - n * nk;
+            sxs[k * NT + n] = n < a.N ? __ldg(a.sx + static_cast<int64_t>(n) * a.nkb + kb0 + k) : 0.0f;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
+        float acc[kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+        const float* sw = a.sw + static_cast<int64_t>(mt) * a.nkb + kb0;
+        int b = 0;
+        uint32_t bpar = 0;
+        float nw = nk > 0 ? __ldg(sw) : 0.0f;
+        for (int i = 0; i < nk; ++i) {
+            const float wsc = nw;
+            if (i + 1 < nk) nw = __ldg(sw + i + 1);
+            const bool ok = f8_wait(&bars.acc_full[b], bpar, &bars, a.err);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            tc_fence_after();
+            const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * NT + g * kCols;
+            const float* sc = sxs + i * NT + g * kCols;
+#pragma unroll
+            for (int c = 0; c < kCols; c += 16) {
+                float v[16];
+                tmem_ldw16(ta + c, v);
+                if (c + 16 == kCols) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.acc_empty[b]);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(sc + c + j);
+                    acc[c + j] = fmaf(v[j], f.x * wsc, acc[c + j]);
+                    acc[c + j + 1] = fmaf(v[j + 1], f.y * wsc, acc[c + j + 1]);
+                    acc[c + j + 2] = fmaf(v[j + 2], f.z * wsc, acc[c + j + 2]);
+                    acc[c + j + 3] = fmaf(v[j + 3], f.w * wsc, acc[c + j + 3]);
+                }
+            }
+            if (++b == kBuf) {
+                b = 0;
+                bpar ^= 1;
+            }
+        }
+        // every MMA has read its stages (the last accumulator was waited for),
+        // so their memory holds the sums now: [token][weight row]
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) red[(g * kCols + i) * 128 + 32 * q + lane] = acc[i];
+    }
+    tc_fence_before();
+    __syncthreads();
+    pdl_launch_dependents();
+    if (warp == 1) tmem_dealloc(tmem, kTmem);
+    if (splits > 1) cluster_sync_all();
+    // the cluster's ranks each finish a share of the tokens
+    TY* const y = static_cast<TY*>(a.y);
+    const int n = static_cast<int>(a.N);
+    for (int i = threadIdx.x; i < ((n + splits - 1) / splits) * 128; i += blockDim.x) {
+        const int t = (i >> 7) * splits + rank, r = i & 127;
+        const int64_t m = static_cast<int64_t>(mt) * 128 + r;
+        if (t >= n || m >= a.M) continue;
+        float v = 0.0f;
+        if (splits == 1) {
+            v = red[t * 128 + r];
+        } else {
+            const float* p = red + t * 128 + r;
+            for (int k = 0; k < splits; ++k) v += ld_cluster_f32(cluster_addr(p, k));
+        }
+        if (a.bias) v += __ldg(a.bias + m);
+        y[static_cast<int64_t>(t) * a.M + m] = Elem<TY>::put(v);
+    }
+    if (splits > 1) cluster_sync_all();  // a rank's sums stay until every rank has read them
+}
+
+// ---- host ---------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// Map of a [rows x cols] matrix of bytes with row stride ld, in boxes of
+// box_rows x 128 bytes.
+cudaError_t byte_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    EncodeFn fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t steps[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), int grid, int threads, int cluster, size_t smem, cudaStream_t s,
+                           Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;  // 0: the kernel's own __cluster_dims__
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+template <int BN, typename TY>
+cudaError_t launch_pair(const F8Linear& l, F8Args a, cudaStream_t s) {
+    constexpr int kStage = 128 * 128 + (BN / 2) * 128;
+    CUtensorMap mx, mw;
+    if (cudaError_t e = byte_map(&mx, l.x, l.N, l.K, l.x_ld, 128); e != cudaSuccess) return e;
+    if (cudaError_t e = byte_map(&mw, l.w, l.M, l.K, l.w_ld, BN / 2); e != cudaSuccess) return e;
+    a.tiles_n = static_cast<int>((l.N + 255) / 256);
+    a.tiles_m = static_cast<int>((l.M + BN - 1) / BN);
+    a.nbuf = 512 / BN;
+    a.stages = std::min(kMaxF8Stages, 196 * 1024 / kStage);
+    const int smem = a.stages * kStage + 1024;
+    static std::atomic<int> cfg[64];
+    if (cudaError_t e = ensure_dyn_smem(f8_pair_kernel<BN, TY>, smem, cfg); e != cudaSuccess) return e;
+    const int64_t tiles = int64_t(a.tiles_n) * a.tiles_m;
+    if (tiles >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
+    const int pairs = static_cast<int>(std::min<int64_t>(tiles, device_sm_count() / 2));
+    return launch_cluster(f8_pair_kernel<BN, TY>, 2 * pairs, kPairThreads, 0, smem, s, mx, mw, a);
+}
+
+template <int NT, typename TY>
+cudaError_t launch_skinny(const F8Linear& l, F8Args a, cudaStream_t s) {
+    constexpr int kStage = 128 * 128 + NT * 128;
+    CUtensorMap mx, mw;
+    if (cudaError_t e = byte_map(&mx, l.x, l.N, l.K, l.x_ld, NT); e != cudaSuccess) return e;
+    if (cudaError_t e = byte_map(&mw, l.w, l.M, l.K, l.w_ld, 128); e != cudaSuccess) return e;
+    const int tiles = static_cast<int>((l.M + 127) / 128);
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count() && splits * 4 <= a.nkb) splits *= 2;
+    const int per = (a.nkb + splits - 1) / splits;  // blocks of K of one CTA
+    // two CTAs per SM, unless the scales of X take the room
+    const int scales = (per * NT * 4 + 127) / 128 * 128;
+    int budget = 110 * 1024 - 1024 - scales;
+    if (budget < 3 * kStage) budget = 224 * 1024 - 1024 - scales;
+    a.stages = std::min({kMaxF8Stages, std::max(per, NT * 512 / kStage + 1), budget / kStage});
+    if (a.stages < 2) return launch_pair<128, TY>(l, a, s);  // K so long that the scales of X fill shared memory
+    a.stages = std::max(a.stages, (NT * 512 + kStage - 1) / kStage);  // the sums need NT x 128 floats
+    const int smem = a.stages * kStage + scales + 1024;
+    static std::atomic<int> cfg[64];
+    if (cudaError_t e = ensure_dyn_smem(f8_skinny_kernel<NT, TY>, smem, cfg); e != cudaSuccess) return e;
+    return launch_cluster(f8_skinny_kernel<NT, TY>, tiles * splits, 64 + 32 * skinny_warps(NT), splits, smem, s, mx, mw, a,
+                          splits);
+}
+
+}  // namespace
+
+cudaError_t f8_gemm_dispatch(const F8Linear& l, cudaStream_t s) {
+    F8Args a{};
+    a.sx = l.x_scales;
+    a.sw = l.w_scales;
+    a.bias = l.bias;
+    a.y = l.y;
+    a.M = l.M;
+    a.N = l.N;
+    a.nkb = static_cast<int>((l.K + kF8Block - 1) / kF8Block);
+    a.err = l.err;
+    return with_dtype(l.y_dtype, [&](auto* tag) {
+        using TY = std::remove_pointer_t<decltype(tag)>;
+        if (l.N <= 16) return launch_skinny<16, TY>(l, a, s);
+        if (l.N <= 32) return launch_skinny<32, TY>(l, a, s);
+        if (l.N <= 64) return launch_skinny<64, TY>(l, a, s);
+        if (l.N <= 128) return launch_skinny<128, TY>(l, a, s);
+        const int64_t wide = (l.N + 255) / 256 * ((l.M + 255) / 256);
+        return wide * 2 >= device_sm_count() ? launch_pair<256, TY>(l, a, s) : launch_pair<128, TY>(l, a, s);
+    });
+}
+
+}  // namespace axq

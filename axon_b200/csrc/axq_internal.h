@@ -63,6 +63,32 @@ size_t gemm_workspace_bytes(int fmt, int64_t M, int64_t K, int64_t N);
 cudaError_t gemm_dispatch(int fmt, const void* w, const float* x, float* out, int64_t M, int64_t K, int64_t N, int flags,
                           void* ws, size_t ws_bytes, int* err, cudaStream_t s);
 
+// e4m3 packing and its decode (axq_f8.cu); err, if given, is set to 0.
+cudaError_t f8_pack_dispatch(int dtype, const void* src, void* codes, int64_t ld, float* scales, int64_t rows,
+                             int64_t cols, int block_rows, int* err, cudaStream_t s);
+cudaError_t f8_dequant_dispatch(const void* codes, int64_t ld, const float* scales, int block_rows, float* dst,
+                                int64_t rows, int64_t cols, cudaStream_t s);
+
+cudaError_t f8_fill_bias_dispatch(int dtype, void* y, const float* bias, int64_t M, int64_t N, int* err, cudaStream_t s);
+
+// y[N x M] = X . W^T on e4m3 operands (axq_f8_gemm.cu): w [M x K] codes with
+// row stride w_ld and 128 x 128 scales; x [N x K] codes with row stride x_ld
+// and 1 x 128 scales.
+struct F8Linear {
+    const void* w;
+    const float* w_scales;
+    int64_t w_ld;
+    const void* x;
+    const float* x_scales;
+    int64_t x_ld;
+    const float* bias;
+    void* y;
+    int y_dtype;
+    int64_t M, K, N;
+    int* err;
+};
+cudaError_t f8_gemm_dispatch(const F8Linear& a, cudaStream_t s);
+
 // Raises `kernel`'s dynamic shared-memory limit on the current device to at
 // least `smem`.  `cfg` (one per kernel instantiation, zero-initialised
 // static storage) records the largest limit set per device; the limit only

@@ -255,6 +255,41 @@ int axq_matmul_sharded(void* comm, int fmt, const void* a_q_local, const float* 
  * multiply-adds (no TF32): this library's own tiled kernel. */
 int axq_matmul_f32(const float* a, const float* b, float* out, int64_t M, int64_t K, int64_t N, axq_stream_t stream);
 
+/* ---- 8-bit floating point blocks --------------------------------------------
+ * A matrix in e4m3 codes (one byte per element, row stride ld bytes, a
+ * multiple of 16 that is at least cols; the base 16-byte aligned) with one fp32
+ * scale per block of block_rows x 128 elements, block_rows = 128 (weights) or 1
+ * (activations): scales [ceil(rows / block_rows) x ceil(cols / 128)], row-major;
+ * value = code * scale.  The reference has no floating-point blocks; the entry
+ * points stand beside axq_quantize, axq_dequantize and axq_linear. */
+enum axq_dtype { AXQ_DT_F32 = 0, AXQ_DT_F16 = 1, AXQ_DT_BF16 = 2, AXQ_DT_F8 = 3 };
+
+/* Pack src [rows x cols] (dtype F32, F16 or BF16; row-major): per block
+ * scale = max|x| / 448 and code = e4m3(x / scale), all three rounded to nearest
+ * even in that order, codes saturating at 448.  A block whose scale is 0 has
+ * codes 0; NaN elements get the NaN code and do not enter the maximum; an
+ * infinity makes the block's scale infinite (it decodes to NaN).  Bytes between
+ * cols and ld that lie in the last block of 128 columns are set to 0. */
+int axq_quantize_f8(int dtype, const void* src, void* codes, int64_t ld, float* scales, int64_t rows, int64_t cols,
+                    int block_rows, axq_stream_t stream);
+
+/* dst [rows x cols] (fp32, row-major) = code * scale. */
+int axq_dequantize_f8(const void* codes, int64_t ld, const float* scales, int block_rows, float* dst, int64_t rows,
+                      int64_t cols, axq_stream_t stream);
+
+/* y [tokens x out_features] (y_dtype F32, F16 or BF16) = x . W^T (+ bias
+ * [out_features], fp32, or NULL), W [out_features x in_features] packed in
+ * 128 x 128 blocks.  x is [tokens x in_features] in x_dtype: F32, F16 or BF16
+ * (row-major, x_ld = in_features, x_scales NULL; packed into 1 x 128 blocks by
+ * the call, as axq_quantize_f8 does), or F8 (already packed so, x_ld its row
+ * stride).  Sums are fp32; the result is rounded once.  The workspace holds the
+ * status word and the packed x (256-byte aligned); a bounded wait that gave up
+ * is reported by axq_workspace_status. */
+size_t axq_linear_f8_workspace_size(int x_dtype, int64_t in_features, int64_t tokens);
+int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int x_dtype, const void* x, int64_t x_ld,
+                  const float* x_scales, const float* bias, int y_dtype, void* y, int64_t out_features,
+                  int64_t in_features, int64_t tokens, void* workspace, size_t workspace_bytes, axq_stream_t stream);
+
 /* ---- .axon tensor files ---------------------------------------------------
  * Replace save_tensor / load_tensor / save_checkpoint / load_checkpoint
  * (src/core/serialize.cpp:84-203) for device buffers.  The byte format is
