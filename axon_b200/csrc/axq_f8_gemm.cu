@@ -46,19 +46,29 @@ struct F8Args {
     int* err;
 };
 
+// One commit per K block serves both who waits for it: done[s] says that the
+// MMAs on stage s have finished, so the stage may be filled again and the
+// accumulator of that block be read.
 struct F8Bars {
-    uint64_t full[kMaxF8Stages], empty[kMaxF8Stages];
-    uint64_t acc_full[4], acc_empty[4];
+    uint64_t full[kMaxF8Stages], done[kMaxF8Stages];
+    uint64_t acc_empty[4];
     uint32_t tmem;
     int abort;
 };
 
-// Bounded wait; on giving up sets the CTA's abort flag and the status word.
+// Bounded wait of a whole warp; on giving up sets the CTA's abort flag and the
+// status word.
 __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, F8Bars* b, int* err) {
-    if (mbar_wait_bounded(bar, parity, &b->abort)) return true;
-    *const_cast<volatile int*>(&b->abort) = 1;
-    if (err) atomicExch(err, 1);
-    return false;
+    bool ok = mbar_try_wait(bar, parity);
+#pragma unroll 1
+    for (int i = 0; i < 16 && !ok; ++i) ok = mbar_try_wait(bar, parity);  // before the slower timer is read
+    if (__builtin_expect(!ok, 0)) ok = mbar_wait_bounded(bar, parity, &b->abort);
+    ok = __all_sync(0xFFFFFFFFu, ok);
+    if (__builtin_expect(!ok, 0)) {
+        *const_cast<volatile int*>(&b->abort) = 1;
+        if (err) atomicExch(err, 1);
+    }
+    return ok;
 }
 
 // Eight values to y in its type (one or two 16-byte stores).
@@ -77,7 +87,12 @@ __device__ __forceinline__ void store8(TY* p, const float* v) {
     }
 }
 
-constexpr int kPairThreads = 320;  // producer warp, MMA warp, eight epilogue warps
+// Warps 0 and 1 copy and issue MMAs (2 and 3 only pad their warpgroup), 4 to
+// 11 are the epilogue.  Registers move from the first warpgroup to the two of
+// the epilogue: 128 * (56 + 2 * 224) is what 384 threads are launched with (168
+// each).
+constexpr int kPairThreads = 384;
+constexpr int kPairRegsLow = 56, kPairRegsHigh = 224;
 
 template <int BN, typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
@@ -95,12 +110,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxF8Stages; ++i) {
             mbar_init(&bars.full[i], 1);
-            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.done[i], 1);
         }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&bars.acc_full[i], 1);
-            mbar_init(&bars.acc_empty[i], 16);  // eight epilogue warps of each CTA
-        }
+        for (int i = 0; i < 4; ++i) mbar_init(&bars.acc_empty[i], 16);  // eight epilogue warps of each CTA
         bars.abort = 0;
         fence_mbar_init();
         prefetch_tensormap(&mx);
@@ -115,79 +127,85 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int ntiles = a.tiles_n * a.tiles_m;
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
+    if (warp < 4) regs_dec<kPairRegsLow>();
     if (warp == 0) {
-        if (lane == 0) {
-            pdl_wait();
-            int s = 0;
-            uint32_t par = 0;
-            bool ok = true;
-            int64_t issued = 0;
-            for (int tile = pair; tile < ntiles && ok; tile += npairs) {
-                // token tiles run fastest: the pairs at work share few weight tiles
-                const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
-                const int xr = tn * 256 + static_cast<int>(rank) * 128;
-                const int wr = tm * BN + static_cast<int>(rank) * (BN / 2);
-                for (int kb = 0; kb < a.nkb; ++kb) {
-                    ok = f8_wait(&bars.empty[s], par ^ 1, &bars, a.err);
-                    if (!ok) break;
+        pdl_wait();
+        int s = 0;
+        uint32_t par = 0;
+        bool ok = true;
+        int64_t issued = 0;
+        for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+            // token tiles run fastest: the pairs at work share few weight tiles
+            const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
+            const int xr = tn * 256 + static_cast<int>(rank) * 128;
+            const int wr = tm * BN + static_cast<int>(rank) * (BN / 2);
+            for (int kb = 0; kb < a.nkb; ++kb) {
+                ok = f8_wait(&bars.done[s], par ^ 1, &bars, a.err);
+                if (!ok) break;
+                if (elect_one()) {
                     if (rank == 0) mbar_arrive_expect_tx(&bars.full[s], 2 * kStage);
                     const uint32_t fb = cluster_addr(&bars.full[s], 0);
                     uint8_t* st = stage0 + s * kStage;
                     tma_load_2d_pair(st, &mx, kb * 128, xr, fb);
                     tma_load_2d_pair(st + kXBytes, &mw, kb * 128, wr, fb);
-                    ++issued;
-                    if (++s == a.stages) {
-                        s = 0;
-                        par ^= 1;
-                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == a.stages) {
+                    s = 0;
+                    par ^= 1;
                 }
             }
-            if (!ok && rank == 0) {
-                // copies still in flight land before the pair's shared memory goes away
-                const int64_t from = issued > a.stages ? issued - a.stages : 0;
-                for (int64_t i = from; i < issued; ++i)
-                    mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
-            }
+        }
+        if (!ok && rank == 0) {
+            // copies still in flight land before the pair's shared memory goes away
+            const int64_t from = issued > a.stages ? issued - a.stages : 0;
+            for (int64_t i = from; i < issued; ++i)
+                mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
         }
         __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            int s = 0, b = 0;
+    } else if (warp == 1 || warp == 2) {
+        if (rank == 0) {
+            // Two issuing warps take K blocks in turn, each block in its own
+            // accumulator, so that the waits and the commit of one run beside
+            // the MMAs of the other.
+            const int mytiles = (ntiles - pair + npairs - 1) / npairs;
+            const int64_t blocks = static_cast<int64_t>(mytiles) * a.nkb;
+            int s = (warp - 1) % a.stages, b = warp - 1;
             uint32_t par = 0, bpar = 0;
-            bool ok = true;
-            for (int tile = pair; tile < ntiles && ok; tile += npairs) {
-                for (int kb = 0; kb < a.nkb; ++kb) {
-                    ok = f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) &&
-                         f8_wait(&bars.full[s], par, &bars, a.err);
-                    if (!ok) break;
-                    tc_fence_after();
+            for (int64_t it = warp - 1; it < blocks; it += 2) {
+                if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err))
+                    break;
+                tc_fence_after();
+                if (elect_one()) {
                     const uint32_t xs = smem_u32(stage0 + s * kStage);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         mma_e4m3<2>(tmem + b * BN, smem_desc_sw128(xs + 32 * k), smem_desc_sw128(xs + kXBytes + 32 * k),
                                     kIdesc, k > 0);
-                    mma_commit_pair(&bars.empty[s]);
-                    mma_commit_pair(&bars.acc_full[b]);
-                    if (++s == a.stages) {
-                        s = 0;
-                        par ^= 1;
-                    }
-                    if (++b == a.nbuf) {
-                        b = 0;
-                        bpar ^= 1;
-                    }
+                    mma_commit_pair(&bars.done[s]);
+                }
+                __syncwarp();
+                if ((s += 2) >= a.stages) {
+                    s -= a.stages;
+                    par ^= 1;
+                }
+                if ((b += 2) >= a.nbuf) {
+                    b -= a.nbuf;
+                    bpar ^= 1;
                 }
             }
         }
-        __syncwarp();
-    } else {
-        const int q = warp & 3, g = (warp - 2) >> 2;
+    } else if (warp >= 4) {
+        regs_inc<kPairRegsHigh>();
+        const int q = warp & 3, g = (warp - 4) >> 2;
         pdl_wait();
-        int b = 0;
-        uint32_t bpar = 0;
+        int b = 0, s = 0;
+        uint32_t par = 0;
         bool ok = true;
         TY* const y = static_cast<TY*>(a.y);
         const bool vec = (a.M * sizeof(TY)) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+        const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + g * kCols;
         for (int tile = pair; tile < ntiles && ok; tile += npairs) {
             const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
             const int64_t t = static_cast<int64_t>(tn) * 256 + rank * 128 + 32 * q + lane;
@@ -198,34 +216,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
             float nx = __ldg(sx), nw = __ldg(sw);
-            for (int kb = 0; kb < a.nkb; ++kb) {
+            // Two chunks of 32 columns in turn: the load of one runs under the
+            // FMAs of the other, across K blocks too.
+            float v[2][32];
+            ok = f8_wait(&bars.done[s], par, &bars, a.err);
+            if (ok) {
+                tc_fence_after();
+                tmem_ld32_issue(ta + b * BN, v[0]);
+            }
+            for (int kb = 0; kb < a.nkb && ok; ++kb) {
                 const float sc = nx * nw;
                 if (kb + 1 < a.nkb) {
                     nx = __ldg(sx + kb + 1);
                     nw = __ldg(sw + kb + 1);
                 }
-                ok = f8_wait(&bars.acc_full[b], bpar, &bars, a.err);
-                if (!__all_sync(0xFFFFFFFFu, ok)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * BN + g * kCols;
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    float v[32];
-                    tmem_ldw32(ta + c, v);
-                    if (c + 32 == kCols) {
+                for (int c = 0; c < kCols / 32; ++c) {
+                    tmem_ld_wait(v[c & 1]);
+                    if (c + 1 < kCols / 32) {
+                        tmem_ld32_issue(ta + b * BN + 32 * (c + 1), v[(c + 1) & 1]);
+                    } else {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(cluster_addr(&bars.acc_empty[b], 0));
+                        if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(&bars.acc_empty[b], 0));
+                        if (++b == a.nbuf) b = 0;
+                        if (++s == a.stages) {
+                            s = 0;
+                            par ^= 1;
+                        }
+                        if (kb + 1 < a.nkb) {
+                            ok = f8_wait(&bars.done[s], par, &bars, a.err);
+                            tc_fence_after();
+                            if (ok) tmem_ld32_issue(ta + b * BN, v[0]);
+                        }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(v[i], sc, acc[c + i]);
-                }
-                if (++b == a.nbuf) {
-                    b = 0;
-                    bpar ^= 1;
+                    for (int i = 0; i < 32; i += 2)
+                        fma2(acc[32 * c + i], acc[32 * c + i + 1], v[c & 1][i], v[c & 1][i + 1], sc, sc);
                 }
             }
             if (!ok) break;
@@ -282,12 +309,9 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxF8Stages; ++i) {
             mbar_init(&bars.full[i], 1);
-            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.done[i], 1);
         }
-        for (int i = 0; i < kBuf; ++i) {
-            mbar_init(&bars.acc_full[i], 1);
-            mbar_init(&bars.acc_empty[i], kEpi);
-        }
+        for (int i = 0; i < kBuf; ++i) mbar_init(&bars.acc_empty[i], kEpi);
         bars.abort = 0;
         fence_mbar_init();
         prefetch_tensormap(&mx);
@@ -300,65 +324,70 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
     const uint32_t tmem = bars.tmem;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // The packing of X, launched before this kernel, let it start only
-            // after everything before the packing had finished, so W is there;
-            // X is waited for.
-            const int first = min(nk, a.stages);
+        // The packing of X, launched before this kernel, let it start only
+        // after everything before the packing had finished, so W is there; X
+        // is waited for.
+        const int first = min(nk, a.stages);
+        if (elect_one()) {
             for (int i = 0; i < first; ++i) {
                 mbar_arrive_expect_tx(&bars.full[i], kStage);
                 tma_load_2d(stage0 + i * kStage, &mw, (kb0 + i) * 128, mt * 128, &bars.full[i]);
             }
-            pdl_wait();
+        }
+        __syncwarp();
+        pdl_wait();
+        if (elect_one()) {
             for (int i = 0; i < first; ++i)
                 tma_load_2d(stage0 + i * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[i]);
-            int s = 0;
-            uint32_t par = 0;
-            bool ok = true;
-            int issued = first;
-            for (int i = first; i < nk; ++i) {
-                ok = f8_wait(&bars.empty[s], par, &bars, a.err);
-                if (!ok) break;
+        }
+        __syncwarp();
+        int s = 0;
+        uint32_t par = 0;
+        bool ok = true;
+        int issued = first;
+        for (int i = first; i < nk; ++i) {
+            ok = f8_wait(&bars.done[s], par, &bars, a.err);
+            if (!ok) break;
+            if (elect_one()) {
                 mbar_arrive_expect_tx(&bars.full[s], kStage);
                 tma_load_2d(stage0 + s * kStage, &mw, (kb0 + i) * 128, mt * 128, &bars.full[s]);
                 tma_load_2d(stage0 + s * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[s]);
-                ++issued;
-                if (++s == a.stages) {
-                    s = 0;
-                    par ^= 1;
-                }
             }
-            if (!ok)  // copies still in flight land before the shared memory goes away
-                for (int i = max(0, issued - a.stages); i < issued; ++i)
-                    mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
+            __syncwarp();
+            ++issued;
+            if (++s == a.stages) {
+                s = 0;
+                par ^= 1;
+            }
         }
+        if (!ok)  // copies still in flight land before the shared memory goes away
+            for (int i = max(0, issued - a.stages); i < issued; ++i)
+                mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0, b = 0;
-            uint32_t par = 0, bpar = 0;
-            for (int i = 0; i < nk; ++i) {
-                if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err))
-                    break;
-                tc_fence_after();
+        int s = 0, b = 0;
+        uint32_t par = 0, bpar = 0;
+        for (int i = 0; i < nk; ++i) {
+            if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err)) break;
+            tc_fence_after();
+            if (elect_one()) {
                 const uint32_t ws = smem_u32(stage0 + s * kStage);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     mma_e4m3<1>(tmem + b * NT, smem_desc_sw128(ws + 32 * k), smem_desc_sw128(ws + kWBytes + 32 * k), kIdesc,
                                 k > 0);
-                mma_commit(&bars.empty[s]);
-                mma_commit(&bars.acc_full[b]);
-                if (++s == a.stages) {
-                    s = 0;
-                    par ^= 1;
-                }
-                if (++b == kBuf) {
-                    b = 0;
-                    bpar ^= 1;
-                }
+                mma_commit(&bars.done[s]);
+            }
+            __syncwarp();
+            if (++s == a.stages) {
+                s = 0;
+                par ^= 1;
+            }
+            if (++b == kBuf) {
+                b = 0;
+                bpar ^= 1;
             }
         }
-        __syncwarp();
     } else {
         const int q = warp & 3, g = (warp - 2) >> 2;
         const int et = threadIdx.x - 64;
@@ -372,14 +401,13 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
 #pragma unroll
         for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
         const float* sw = a.sw + static_cast<int64_t>(mt) * a.nkb + kb0;
-        int b = 0;
-        uint32_t bpar = 0;
+        int b = 0, s = 0;
+        uint32_t par = 0;
         float nw = nk > 0 ? __ldg(sw) : 0.0f;
         for (int i = 0; i < nk; ++i) {
             const float wsc = nw;
             if (i + 1 < nk) nw = __ldg(sw + i + 1);
-            const bool ok = f8_wait(&bars.acc_full[b], bpar, &bars, a.err);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (!f8_wait(&bars.done[s], par, &bars, a.err)) break;
             tc_fence_after();
             const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * NT + g * kCols;
             const float* sc = sxs + i * NT + g * kCols;
@@ -401,9 +429,10 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
                     acc[c + j + 3] = fmaf(v[j + 3], f.w * wsc, acc[c + j + 3]);
                 }
             }
-            if (++b == kBuf) {
-                b = 0;
-                bpar ^= 1;
+            if (++b == kBuf) b = 0;
+            if (++s == a.stages) {
+                s = 0;
+                par ^= 1;
             }
         }
         // every MMA has read its stages (the last accumulator was waited for),
@@ -524,7 +553,7 @@ cudaError_t launch_skinny(const F8Linear& l, F8Args a, cudaStream_t s) {
     const int scales = (per * NT * 4 + 127) / 128 * 128;
     int budget = 110 * 1024 - 1024 - scales;
     if (budget < 3 * kStage) budget = 224 * 1024 - 1024 - scales;
-    a.stages = std::min({kMaxF8Stages, std::max(per, NT * 512 / kStage + 1), budget / kStage});
+    a.stages = std::min({kMaxF8Stages, std::max(std::max(per, 2), NT * 512 / kStage + 1), budget / kStage});
     if (a.stages < 2) return launch_pair<128, TY>(l, a, s);  // K so long that the scales of X fill shared memory
     a.stages = std::max(a.stages, (NT * 512 + kStage - 1) / kStage);  // the sums need NT x 128 floats
     const int smem = a.stages * kStage + scales + 1024;

@@ -115,6 +115,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 
 // ---- 8-bit floating point operands, tensor-map copies, CTA pairs ------------
 
+// True in one lane of a converged warp.  Copies and MMAs are issued under it
+// inside loops that the whole warp runs: the compiler then knows that one
+// thread issues and keeps descriptors and addresses in uniform registers (a
+// loop under `lane == 0` took 985 clocks for a block of K where this takes 565).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 // Shared-memory descriptor of a K-major tile whose rows are 128 bytes in the
 // 128-byte swizzle (what a tensor-map copy with SWIZZLE_128B writes): groups
 // of 8 rows are 1024 bytes apart; the tile starts on a 1024-byte boundary and
@@ -212,6 +226,46 @@ __device__ __forceinline__ void tmem_ldw32(uint32_t taddr, float (&v)[32]) {
         : "memory");
 }
 
+// The same load without the wait, and the wait that v may be read after: the
+// wait lists v as changed, so no use of v moves before it.
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                   "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+
+// d = a * s + d on two floats at once (one instruction for the pair).
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float s0, float s1) {
+    asm("{\n\t.reg .b64 d, a, s;\n\t"
+        "mov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\t"
+        "fma.rn.f32x2 d, a, s, d;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(a0), "f"(a1), "f"(s0), "f"(s1));
+}
+
+// Moves this warpgroup's register limit (all its four warps call it).
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Copy of one box of a two-dimensional tensor map (x: element of the row,
 // y: row) into shared memory, counted on `bar` in bytes.  x times the
 // element size must be a multiple of 16.
@@ -249,8 +303,12 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+// Arrival on another CTA's barrier that orders nothing but TMEM reads already
+// waited for (tcgen05.wait::ld and the fence before it): relaxed, since a
+// release at cluster scope drains every outstanding load of the warp first
+// (it took 4 of 11 warp-cycles per instruction in the pair kernel).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
