@@ -94,6 +94,9 @@ __device__ __forceinline__ void store8(TY* p, const float* v) {
 constexpr int kPairThreads = 384;
 constexpr int kPairRegsLow = 56, kPairRegsHigh = 224;
 
+// Output staging of an epilogue warp: 32 rows of 128 bytes, 16 bytes apart.
+constexpr int kOutRow = 144, kOutWarpBytes = 32 * kOutRow;
+
 template <int BN, typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     f8_pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, F8Args a) {
@@ -104,6 +107,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     constexpr uint32_t kIdesc = idesc_e4m3_f32(BN, 256);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* stage0 = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint8_t* out_stage = stage0 + a.stages * kStage;
     __shared__ F8Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -256,24 +260,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
             }
             if (!ok) break;
-            if (t < a.N) {
-                TY* yr = y + t * a.M + m0;
+            // Through shared memory, so that a store covers 128 bytes of four
+            // rows and not 16 bytes of 32 (the MMAs wait meanwhile: 5.5 us a
+            // tile before): kOutCols columns of the warp's 32 rows at a time.
+            constexpr int kOutCols = 128 / static_cast<int>(sizeof(TY));
+            uint8_t* const own = out_stage + (warp - 4) * kOutWarpBytes;
+            const int64_t t0 = t - lane;
+            const int rows = static_cast<int>(min64(32, a.N - t0));
 #pragma unroll
-                for (int c = 0; c < kCols; c += 8) {
-                    if (m0 + c >= a.M) break;
-                    if (a.bias) {
+            for (int c0 = 0; c0 < kCols; c0 += kOutCols) {
+                if (m0 + c0 >= a.M) break;
+                if (a.bias) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (m0 + c + i < a.M) acc[c + i] += __ldg(a.bias + m0 + c + i);
-                    }
-                    if (vec && m0 + c + 8 <= a.M) {
-                        store8(yr + c, acc + c);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (m0 + c + i < a.M) yr[c + i] = Elem<TY>::put(acc[c + i]);
-                    }
+                    for (int i = 0; i < kOutCols; ++i)
+                        if (m0 + c0 + i < a.M) acc[c0 + i] += __ldg(a.bias + m0 + c0 + i);
                 }
+#pragma unroll
+                for (int i = 0; i < kOutCols; i += 8)
+                    store8(reinterpret_cast<TY*>(own + lane * kOutRow) + i, acc + c0 + i);
+                __syncwarp();
+                if (vec && m0 + c0 + kOutCols <= a.M) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = 4 * j + (lane >> 3);
+                        if (r < rows)
+                            *reinterpret_cast<uint4*>(y + (t0 + r) * a.M + m0 + c0 + (lane & 7) * (kOutCols / 8)) =
+                                *reinterpret_cast<const uint4*>(own + r * kOutRow + (lane & 7) * 16);
+                    }
+                } else {
+                    for (int r = 0; r < rows; ++r)
+                        for (int c = lane; c < kOutCols && m0 + c0 + c < a.M; c += 32)
+                            y[(t0 + r) * a.M + m0 + c0 + c] = reinterpret_cast<const TY*>(own + r * kOutRow)[c];
+                }
+                __syncwarp();
             }
         }
     }
@@ -529,8 +548,10 @@ cudaError_t launch_pair(const F8Linear& l, F8Args a, cudaStream_t s) {
     a.tiles_n = static_cast<int>((l.N + 255) / 256);
     a.tiles_m = static_cast<int>((l.M + BN - 1) / BN);
     a.nbuf = 512 / BN;
-    a.stages = std::min(kMaxF8Stages, 196 * 1024 / kStage);
-    const int smem = a.stages * kStage + 1024;
+    constexpr int kOut = 8 * kOutWarpBytes;
+    a.stages = std::min(kMaxF8Stages, (224 * 1024 - 1024 - kOut) / kStage);
+    static_assert(512 / BN <= (224 * 1024 - 1024 - kOut) / kStage, "an accumulator buffer needs a stage of its own");
+    const int smem = a.stages * kStage + kOut + 1024;
     static std::atomic<int> cfg[64];
     if (cudaError_t e = ensure_dyn_smem(f8_pair_kernel<BN, TY>, smem, cfg); e != cudaSuccess) return e;
     const int64_t tiles = int64_t(a.tiles_n) * a.tiles_m;
