@@ -178,7 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             int s = (warp - 1) % a.stages, b = warp - 1;
             uint32_t par = 0, bpar = 0;
             for (int64_t it = warp - 1; it < blocks; it += 2) {
-                if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err))
+                if (!f8_wait(&bars.full[s], par, &bars, a.err) || !f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err))
                     break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -210,6 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         TY* const y = static_cast<TY*>(a.y);
         const bool vec = (a.M * sizeof(TY)) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
         const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + g * kCols;
+        const uint32_t empty0 = cluster_addr(&bars.acc_empty[0], 0);
         for (int tile = pair; tile < ntiles && ok; tile += npairs) {
             const int tn = tile % a.tiles_n, tm = tile / a.tiles_n;
             const int64_t t = static_cast<int64_t>(tn) * 256 + rank * 128 + 32 * q + lane;
@@ -242,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     } else {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(cluster_addr(&bars.acc_empty[b], 0));
+                        if (elect_one()) mbar_arrive_cluster_relaxed(empty0 + 8 * b);
                         if (++b == a.nbuf) b = 0;
                         if (++s == a.stages) {
                             s = 0;
