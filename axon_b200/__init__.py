@@ -54,6 +54,11 @@ from .f8 import (  # noqa: F401
     linear_f8,
     quantize_f8,
 )
+from .moe import (  # noqa: F401
+    moe_mlp_q,
+    moe_q,
+    moe_route,
+)
 from .axon_file import (  # noqa: F401
     AxonRecord,
     axon_records,
@@ -77,6 +82,7 @@ from .shard import (  # noqa: F401
 __all__ = [
     "AxqError", "QuantFormat", "QTensor", "Status", "Workspace", "quantize", "dequantize", "matmul_q",
     "matmul_q8_0", "matmul_q4", "matmul_q2_K", "matmul_q3_K", "matmul_q4_K", "matmul_q5_K", "matmul_q6_K",
-    "linear_q", "gate_up_silu", "mlp_q", "F8Tensor", "quantize_f8", "dequantize_f8", "linear_f8", "quantized_size", "quantized_size_2d", "matmul_workspace_size", "lib", "lib_path",
+    "linear_q", "gate_up_silu", "mlp_q", "F8Tensor", "quantize_f8", "dequantize_f8", "linear_f8",
+    "moe_route", "moe_mlp_q", "moe_q", "quantized_size", "quantized_size_2d", "matmul_workspace_size", "lib", "lib_path",
     "Communicator", "SymmetricBuffer", "matmul_sharded_p2p", "wait_all", "allgather_", "matmul_sharded", "row_bytes", "shard_bounds", "shard_rows",
 ]

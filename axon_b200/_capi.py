@@ -48,6 +48,7 @@ class DType(enum.IntEnum):
     F8 = 3
 
 
+F8_E4M3 = 64  # AXQ_F8_E4M3
 F8_BLOCK = 128  # columns (and, for weights, rows) that share one e4m3 scale
 
 
@@ -116,6 +117,10 @@ SIGNATURES = {
     "axq_linear_f8_workspace_size": (_sz, [ctypes.c_int, _i64, _i64]),
     "axq_linear_f8": (ctypes.c_int, [_vp, _i64, _vp, ctypes.c_int, _vp, _i64, _vp, _vp, ctypes.c_int, _vp, _i64, _i64,
                                      _i64, _vp, _sz, _vp]),
+    "axq_moe_route": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int, _vp]),
+    "axq_moe_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "axq_moe_mlp": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp, _vp,
+                                   _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "axq_axon_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_uint32)]),
     "axq_axon_info": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp]),
     "axq_axon_read": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp, _sz, _vp]),

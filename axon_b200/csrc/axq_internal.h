@@ -89,6 +89,25 @@ struct F8Linear {
 };
 cudaError_t f8_gemm_dispatch(const F8Linear& a, cudaStream_t s);
 
+// Mixture-of-experts layer (axq_moe.cu).
+struct MoeMlp {
+    int fmt, fmt_down;  // AXQ_* format ids or AXQ_F8_E4M3
+    const void *w_gate, *w_up, *w_down;
+    const float *s_gate, *s_up, *s_down;
+    int64_t gate_bytes, down_bytes;  // of all experts' packed rows
+    int dtype;
+    const void* x;
+    const int* ids;
+    const float* weights;
+    void* y;
+    int64_t tokens, hidden, ffn;
+    int experts, top_k;
+};
+size_t moe_workspace_bytes(int64_t tokens, int top_k, int64_t hidden, int64_t ffn);
+cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens,
+                               int experts, int top_k, int64_t hidden, int normalize, cudaStream_t s);
+cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s);
+
 // Raises `kernel`'s dynamic shared-memory limit on the current device to at
 // least `smem`.  `cfg` (one per kernel instantiation, zero-initialised
 // static storage) records the largest limit set per device; the limit only

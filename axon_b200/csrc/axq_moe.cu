@@ -1,0 +1,781 @@
+// Mixture-of-experts layer for a few tokens on packed expert weights:
+//   ids, p = top_k of softmax(x . W_router^T)
+//   y[t]   = sum_j p[t][j] * W_down[e] . (silu(W_gate[e] . x) * (W_up[e] . x)),
+//            e = ids[t][j].
+//
+// HBM-bound on the packed bytes of the experts that some token chose; each is
+// read once per group of up to 4 NB of its tokens.
+//
+//  * moe_route_kernel: a cluster of 8 CTAs per 4 tokens splits the experts, its
+//    first CTA picks the top_k.
+//  * moe_prep_kernel: the plan (tokens' choices sorted by expert, in groups), and
+//    records of x: per 256 elements two fp16 terms (x 2^-e ~ hi + lo, 22 bits) in
+//    the order of the weights' MMA fragments, and sums for the minimums.
+//  * moe_expert_kernel: a producer warp streams packed rows through a ring of
+//    shared-memory stages (bulk copies); eight consumer warps decode them into
+//    exact fp16 fragments (axq_moe_decode.cuh) and multiply with mma.sync
+//    m16n8k16, whose 8 columns are the two terms of four tokens.  Runs twice: gate
+//    and up (tile 0 and 1 of a unit are 16 rows of each, joined by silu), and
+//    down (32 rows).  mma.sync and not tcgen05: the weights are decoded in
+//    registers, and with at most 8 columns the tensor pipe is idle most of the
+//    time either way.
+//  * moe_combine_kernel: y from the experts' products, in the order of the
+//    token's choices (no atomics on values: results do not depend on timing).
+#include <algorithm>
+
+#include "axq_common.cuh"
+#include "axq_f8.cuh"
+#include "axq_internal.h"
+#include "axq_moe.cuh"
+#include "axq_moe_decode.cuh"
+#include "axq_ptx.cuh"
+#include "axq_tc.cuh"
+
+namespace axq {
+namespace {
+
+// ---- router ---------------------------------------------------------------------
+
+constexpr int kRouteCtas = 8, kRouteWarps = 8, kRouteTokens = 4;
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Logits in fp32 (FMAs over lanes of 128 columns, then a tree over the lanes);
+// ties go to the lowest index, NaN logits are chosen last.
+template <typename T>
+__global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRouteWarps)
+    moe_route_kernel(const T* __restrict__ x, const float* __restrict__ w, int* __restrict__ ids, float* __restrict__ wt,
+                     int64_t tokens, int experts, int top_k, int64_t hidden, int normalize, bool vec) {
+    extern __shared__ float logits[];  // [kRouteTokens][experts], of the cluster's first CTA
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouteCtas) * kRouteTokens;
+    const int nt = static_cast<int>(min64(kRouteTokens, tokens - t0));
+    cluster_sync_all();  // the first CTA's shared memory is there
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int e = static_cast<int>(rank) * kRouteWarps + warp; e < experts; e += kRouteCtas * kRouteWarps) {
+        float acc[kRouteTokens] = {};
+        const float* we = w + static_cast<int64_t>(e) * hidden;
+        if (vec) {
+            for (int64_t k = 4 * lane; k < hidden; k += 128) {
+                const float4 a = *reinterpret_cast<const float4*>(we + k);
+#pragma unroll
+                for (int t = 0; t < kRouteTokens; ++t) {
+                    if (t >= nt) break;
+                    const T* xp = x + (t0 + t) * hidden + k;
+                    float v[4];
+                    if constexpr (sizeof(T) == 4) {
+                        const float4 b = *reinterpret_cast<const float4*>(xp);
+                        v[0] = b.x; v[1] = b.y; v[2] = b.z; v[3] = b.w;
+                    } else {
+                        const uint2 b = *reinterpret_cast<const uint2*>(xp);
+                        T h[4];
+                        memcpy(h, &b, 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = Elem<T>::get(h[i]);
+                    }
+                    acc[t] = fmaf(a.x, v[0], fmaf(a.y, v[1], fmaf(a.z, v[2], fmaf(a.w, v[3], acc[t]))));
+                }
+            }
+        } else {
+            for (int64_t k = lane; k < hidden; k += 32)
+#pragma unroll
+                for (int t = 0; t < kRouteTokens; ++t)
+                    if (t < nt) acc[t] = fmaf(we[k], Elem<T>::get(x[(t0 + t) * hidden + k]), acc[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < kRouteTokens; ++t) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(0xFFFFFFFFu, acc[t], d);
+            if (lane == 0 && t < nt) st_cluster_f32(cluster_addr(logits + t * experts + e, 0), acc[t]);
+        }
+    }
+    cluster_sync_all();
+    if (rank != 0 || warp >= nt) return;
+    float* l = logits + warp * experts;
+    float mx = -INFINITY;
+    for (int e = lane; e < experts; e += 32) mx = fmaxf(mx, l[e]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
+    float all = 0.0f;
+    for (int e = lane; e < experts; e += 32) all += expf(l[e] - mx);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, d);
+    float mine = 0.0f, sum = 0.0f;
+    int my_id = 0;
+    for (int j = 0; j < top_k; ++j) {
+        // best of the experts not yet chosen (chosen ones are marked by a bit of `taken`)
+        float bv = 0.0f;
+        int bi = INT32_MAX;
+        for (int e = lane; e < experts; e += 32) {
+            const float v = l[e];
+            const bool first = bi == INT32_MAX;
+            // order: greater value first, NaN after everything, then the lower index
+            const bool better = first || (isnan(bv) ? !isnan(v) : v > bv);
+            if (__float_as_uint(v) != 0xFFFFDEADu && better) {
+                bv = v;
+                bi = e;
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            const float ov = __shfl_xor_sync(0xFFFFFFFFu, bv, d);
+            const int oi = __shfl_xor_sync(0xFFFFFFFFu, bi, d);
+            bool take;
+            if (oi == INT32_MAX) take = false;
+            else if (bi == INT32_MAX) take = true;
+            else if (isnan(ov) || isnan(bv)) take = isnan(ov) == isnan(bv) ? oi < bi : isnan(bv);
+            else take = ov > bv || (ov == bv && oi < bi);
+            if (take) {
+                bv = ov;
+                bi = oi;
+            }
+        }
+        const float p = expf(bv - mx);
+        sum += p;
+        if (lane == j % 32) {
+            mine = p;
+            my_id = bi;
+        }
+        __syncwarp();
+        if (lane == 0) l[bi] = __uint_as_float(0xFFFFDEADu);  // a NaN no product gives
+        __syncwarp();
+    }
+    if (lane < top_k) {
+        ids[(t0 + warp) * top_k + lane] = my_id;
+        wt[(t0 + warp) * top_k + lane] = mine / (normalize ? sum : all);
+    }
+}
+
+// ---- plan and activation records ---------------------------------------------------
+
+// Record of one row and CG: eight 128-byte lines (one for each pair of MMAs:
+// [term][lane part][16 bytes]), the sums [term][lane part][8 bytes], the scale.
+constexpr int kRec = 1152;
+constexpr int kRecSums = 1024, kRecScale = 1088;
+
+// Two fp16 terms of v (already scaled): v = hi + lo within 2^-22 of it.
+__device__ __forceinline__ void split2(float v, __half& hi, __half& lo) {
+    hi = __float2half_rn(v);
+    const float r = v - __half2float(hi);
+    lo = __float2half_rn(isfinite(r) ? r : 0.0f);
+}
+
+// One warp: the record of 256 elements in s (shared memory, zero past the end).
+template <int F>
+__device__ __forceinline__ void write_record(const float* s, uint8_t* rec, int lane) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(s[32 * j + lane]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    // A power of two brings the largest element to [2^8, 2^9): fp16 then holds
+    // sums of 32 elements, and terms down to 2^-33 of the largest.
+    const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127 - 8, -118), 118);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const int mp = lane >> 2, i = lane & 3;
+    __half hi[8], lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int el = Order<F>::elem(2 * mp + (k >> 2), i, k & 3);
+        split2(s[el] * up, hi[k], lo[k]);
+    }
+    uint4 a, b;
+    memcpy(&a, hi, 16);
+    memcpy(&b, lo, 16);
+    *reinterpret_cast<uint4*>(rec + mp * 128 + i * 16) = a;
+    *reinterpret_cast<uint4*>(rec + mp * 128 + 64 + i * 16) = b;
+    if constexpr (Order<F>::SUMS > 0) {
+        if (lane < 16) {  // lane part lane / 4, slot lane % 4
+            constexpr int N = 256 / Order<F>::SUMS;
+            const int sb = Order<F>::sum(lane >> 2, lane & 3);
+            float v = 0.0f;
+            if (sb >= 0)
+                for (int k = 0; k < N; ++k) v += s[sb * N + ((k + lane) & (N - 1))];
+            __half h, l;
+            split2(v * up, h, l);
+            reinterpret_cast<__half*>(rec + kRecSums)[lane] = h;
+            reinterpret_cast<__half*>(rec + kRecSums + 32)[lane] = l;
+        }
+    }
+    if (lane == 0) *reinterpret_cast<float*>(rec + kRecScale) = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+constexpr int kPrepWarps = 8;
+
+// Rows of x (or h) -> records; block 0 also makes the plan when ids are given.
+// need (may be null): rows whose expert id is out of range are skipped.
+template <int F, typename T>
+__global__ void __launch_bounds__(32 * kPrepWarps)
+    moe_prep_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int ncg, uint8_t* __restrict__ rec,
+                    const int* __restrict__ need, int experts, MoePlan plan) {
+    __shared__ float buf[kPrepWarps][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (plan.ids && blockIdx.x == 0) {
+        moe_make_plan(plan);
+        return;
+    }
+    const int64_t b = blockIdx.x - (plan.ids ? 1 : 0);
+    const int64_t it = b * kPrepWarps + warp;
+    if (it >= rows * ncg) return;
+    const int64_t r = it / ncg;
+    const int cg = static_cast<int>(it - r * ncg);
+    if (need && static_cast<unsigned>(need[r]) >= static_cast<unsigned>(experts)) return;
+    const int64_t k0 = static_cast<int64_t>(cg) * 256;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int64_t k = k0 + 32 * j + lane;
+        buf[warp][32 * j + lane] = k < cols ? Elem<T>::get(x[r * cols + k]) : 0.0f;
+    }
+    __syncwarp();
+    write_record<F>(buf[warp], rec + it * kRec, lane);
+}
+
+// ---- experts -------------------------------------------------------------------------
+
+constexpr int kConsumers = 8;
+constexpr int kMoeThreads = (kConsumers + 1) * 32;
+constexpr int kMoeStages = 8;  // most
+constexpr int kTileRows = 32;  // rows of a unit: two tiles of 16
+
+struct MoeBars {
+    uint64_t full[kMoeStages], empty[kMoeStages];
+    int abort;
+};
+
+struct ExpertArgs {
+    const uint8_t* w[2];   // tile 0's and tile 1's matrix
+    const float* sc[2];    // e4m3: their scales
+    int64_t w_bytes;       // bytes of each (all experts)
+    int64_t rb;            // bytes from row to row
+    int64_t rows;          // rows of an expert
+    int64_t row_bytes;     // packed bytes of a row
+    int ncg, nblk;         // CGs and (32- or 128-element) blocks of a row
+    int gate_up;           // tile 1 is `up` and the result silu(tile 0) * tile 1; else tile 1 follows tile 0
+    int tiles;             // units of an expert
+    int slots, wps;        // units a stage holds, warps (and CGs of a stage) per unit: slots * wps = 8
+    int rs, stage_bytes, stages;
+    const uint8_t* rec;    // activation records
+    int64_t rec_row;       // bytes of a record row
+    int rec_div;           // record row of pair p: p / rec_div
+    float* out;            // [pair][rows]
+    MoePlan plan;
+    int* err;
+};
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Compile-time loop over MMA pairs 0..7.
+template <class Fn, int... Js>
+__device__ __forceinline__ void each_pair_impl(Fn&& f, std::integer_sequence<int, Js...>) {
+    (f(std::integral_constant<int, Js>{}), ...);
+}
+template <class Fn>
+__device__ __forceinline__ void each_pair(Fn&& f) {
+    each_pair_impl(f, std::make_integer_sequence<int, 8>{});
+}
+
+// One CG of one tile (rows g and g + 8 of it at p0, p1) times NB blocks of four
+// tokens: tot[n][r] += row r's product with token 4 n + i.
+template <int F, int NB>
+__device__ __forceinline__ void moe_cg(const uint8_t* p0, const uint8_t* p1, int i, const uint8_t* const (&rec)[NB],
+                                       const float (&xs)[NB], int blocks, const float* wsc, float (&tot)[NB][2]) {
+    MoeRow<F> r0, r1;
+    r0.load(p0, i);
+    r1.load(p1, i);
+    float acc[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
+    each_pair([&](auto MPc) {
+        constexpr int MP = decltype(MPc)::value;
+        uint4 b[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) b[n] = __ldg(reinterpret_cast<const uint4*>(rec[n] + MP * 128));
+        uint32_t x[4], y[4];
+        if constexpr (F == F_Q6_K) {
+            uint32_t xh[4], yh[4];
+            r0.template pair<MP>(x, xh);
+            r1.template pair<MP>(y, yh);
+            const uint32_t h0[4] = {xh[0], yh[0], xh[1], yh[1]}, h1[4] = {xh[2], yh[2], xh[3], yh[3]};
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                mma16816(acc[n], h0, b[n].x, b[n].y);
+                mma16816(acc[n], h1, b[n].z, b[n].w);
+            }
+        } else {
+            r0.template pair<MP>(x);
+            r1.template pair<MP>(y);
+        }
+        const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            mma16816(acc[n], a0, b[n].x, b[n].y);
+            mma16816(acc[n], a1, b[n].z, b[n].w);
+        }
+        if constexpr (F == F_Q8_0 || F == F_Q4_0) {
+            // block MP is done: its fp16 scales in fp32 (blocks past the row's end hold other rows' bytes)
+            const float d0 = r0.d(), d1 = r1.d();
+            const bool in = MP < blocks;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if (in) {
+                    tot[n][0] = fmaf(xs[n] * d0, acc[n][0] + acc[n][1], tot[n][0]);
+                    tot[n][1] = fmaf(xs[n] * d1, acc[n][2] + acc[n][3], tot[n][1]);
+                }
+                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+            }
+        }
+        if constexpr (F == F_F8 && MP % 4 == 3) {
+            const bool in = MP / 4 < blocks;
+            const float d = in ? __ldg(wsc + MP / 4) : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if (in) {
+                    tot[n][0] = fmaf(xs[n] * d, acc[n][0] + acc[n][1], tot[n][0]);
+                    tot[n][1] = fmaf(xs[n] * d, acc[n][2] + acc[n][3], tot[n][1]);
+                }
+                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+            }
+        }
+    });
+    if constexpr (Order<F>::SUMS > 0) {
+        uint32_t m0[2], m1[2];
+        r0.mins(m0);
+        r1.mins(m1);
+        const uint32_t a[4] = {m0[0], m1[0], m0[1], m1[1]};
+        const float d0 = r0.d(), d1 = r1.d(), q0 = r0.dm(), q1 = r1.dm();
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            // the line of this lane's column and part: sums are 8 bytes where codes are 16
+            const uint8_t* line = rec[n];
+            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(line)) & 127u;  // term * 64 + i * 16
+            const uint2 b = __ldg(reinterpret_cast<const uint2*>(line - off + kRecSums + off / 2));
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma16816(c, a, b.x, b.y);
+            tot[n][0] = fmaf(xs[n], fmaf(d0, acc[n][0] + acc[n][1], -q0 * (c[0] + c[1])), tot[n][0]);
+            tot[n][1] = fmaf(xs[n], fmaf(d1, acc[n][2] + acc[n][3], -q1 * (c[2] + c[3])), tot[n][1]);
+        }
+    }
+}
+
+// Bounded wait of a whole warp (see MoeBars::abort).
+__device__ __forceinline__ bool moe_wait(uint64_t* bar, uint32_t parity, MoeBars* b, int* err) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (__builtin_expect(!ok, 0)) ok = mbar_wait_bounded(bar, parity, &b->abort);
+    ok = __all_sync(0xFFFFFFFFu, ok);
+    if (__builtin_expect(!ok, 0)) {
+        *const_cast<volatile int*>(&b->abort) = 1;
+        atomicExch(err, 1);
+    }
+    return ok;
+}
+
+template <int F, int NB>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const ExpertArgs a) {
+    constexpr int CGB = moe_cg_bytes<F>();
+    constexpr int kTok = 4 * NB;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127);
+    float* red = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [2][warp][tile][token][16]
+    __shared__ MoeBars bars;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMoeStages; ++s) {
+            mbar_init(&bars.full[s], 1);
+            mbar_init(&bars.empty[s], kConsumers);
+        }
+        bars.abort = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_dependents();
+    const int ngroups = *a.plan.ngroups;
+    const int64_t per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group
+    const int64_t rounds = ngroups * per;
+    const int64_t lo = rounds * blockIdx.x / gridDim.x, hi = rounds * (blockIdx.x + 1) / gridDim.x;
+    const int ksteps = (a.ncg + a.wps - 1) / a.wps;
+
+    if (warp == kConsumers) {
+        const uint64_t policy = l2_evict_first_policy();
+        int s = 0;
+        uint32_t par = 0;
+        bool ok = true;
+        int64_t issued = 0;
+        for (int64_t rd = lo; rd < hi && ok; ++rd) {
+            const int grp = static_cast<int>(rd / per);
+            const int t0 = static_cast<int>(rd - grp * per) * a.slots;
+            const int64_t expert = a.plan.groups[grp].x;
+            for (int k = 0; k < ksteps; ++k) {
+                ok = moe_wait(&bars.empty[s], par ^ 1, &bars, a.err);
+                if (!ok) break;
+                uint8_t* st = ring + s * a.stage_bytes;
+                const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
+                const int64_t seg = min64(static_cast<int64_t>(a.wps) * CGB, a.row_bytes - off);
+                // lane: stage row `lane` of every slot; the bytes come from the 16-byte rounded range around the segment
+                uint32_t tx = 0;
+                for (int u = 0; u < a.slots; ++u) {
+                    const int64_t row = a.gate_up ? static_cast<int64_t>(t0 + u) * 16 + (lane & 15)
+                                                  : static_cast<int64_t>(t0 + u) * 32 + lane;
+                    if (t0 + u >= a.tiles || row >= a.rows) continue;
+                    const int64_t at = (expert * a.rows + row) * a.rb + off;
+                    const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
+                    if (to <= a.w_bytes) {
+                        tx += static_cast<uint32_t>(to - from);
+                    } else {  // the rounded end would leave the buffer: bytes one by one
+                        const uint8_t* src = a.w[lane >> 4] + at;
+                        uint8_t* dst = st + (u * kTileRows + lane) * a.rs + (at & 15);
+                        for (int64_t c = 0; c < seg; ++c) dst[c] = src[c];
+                    }
+                }
+                tx = __reduce_add_sync(0xFFFFFFFFu, tx);
+                __syncwarp();  // bytes copied by lanes come before the arrival
+                if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], tx);
+                __syncwarp();
+                for (int u = 0; u < a.slots; ++u) {
+                    const int64_t row = a.gate_up ? static_cast<int64_t>(t0 + u) * 16 + (lane & 15)
+                                                  : static_cast<int64_t>(t0 + u) * 32 + lane;
+                    if (t0 + u >= a.tiles || row >= a.rows) continue;
+                    const int64_t at = (expert * a.rows + row) * a.rb + off;
+                    const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
+                    if (to <= a.w_bytes)
+                        bulk_g2s_hint(st + (u * kTileRows + lane) * a.rs, a.w[lane >> 4] + from,
+                                      static_cast<uint32_t>(to - from), &bars.full[s], policy);
+                }
+                ++issued;
+                if (++s == a.stages) {
+                    s = 0;
+                    par ^= 1;
+                }
+            }
+        }
+        if (!ok)  // copies still in flight land before the shared memory goes away
+            for (int64_t i = max(int64_t(0), issued - a.stages); i < issued; ++i)
+                mbar_wait_bounded(&bars.full[i % a.stages], static_cast<uint32_t>((i / a.stages) & 1));
+        return;
+    }
+
+    const int g = lane >> 2, i = lane & 3;
+    const int u = warp / a.wps, col = warp - u * a.wps;
+    int s = 0;
+    uint32_t par = 0;
+    bool ok = true;
+    for (int64_t rd = lo; rd < hi; ++rd) {
+        const int grp = static_cast<int>(rd / per);
+        const int tile = static_cast<int>(rd - grp * per) * a.slots + u;
+        const int4 gd = a.plan.groups[grp];  // expert, first entry of pairs, number of them
+        // this lane's B column: term g & 1 of token 4 n + g / 2 (past the group's end: its first)
+        const uint8_t* rec0[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int t = 4 * n + (g >> 1);
+            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)];
+            rec0[n] = a.rec + p / a.rec_div * a.rec_row + (g & 1) * 64 + i * 16;
+        }
+        // the scale of this lane's accumulator columns: token 4 n + i
+        const uint8_t* scale0[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int t = 4 * n + i;
+            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)];
+            scale0[n] = a.rec + p / a.rec_div * a.rec_row + kRecScale;
+        }
+        float tot[2][NB][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) tot[t][n][0] = tot[t][n][1] = 0.0f;
+        for (int k = 0; k < ksteps; ++k) {
+            if (ok) ok = moe_wait(&bars.full[s], par, &bars, a.err);
+            const int cg = k * a.wps + col;
+            if (ok && cg < a.ncg && tile < a.tiles) {
+                const uint8_t* rec[NB];
+                float xs[NB];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    rec[n] = rec0[n] + static_cast<int64_t>(cg) * kRec;
+                    xs[n] = __ldg(reinterpret_cast<const float*>(scale0[n] + static_cast<int64_t>(cg) * kRec));
+                }
+                const uint8_t* st = ring + s * a.stage_bytes + u * kTileRows * a.rs + col * CGB;
+                const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int64_t row = a.gate_up ? static_cast<int64_t>(tile) * 16 : static_cast<int64_t>(tile) * 32 + 16 * t;
+                    const int64_t at = (gd.x * a.rows + row + g) * a.rb + off;
+                    const uint8_t* p0 = st + (16 * t + g) * a.rs + (at & 15);
+                    const uint8_t* p1 = st + (16 * t + g + 8) * a.rs + ((at + 8 * a.rb) & 15);
+                    constexpr int kPerCg = F == F_F8 ? 2 : 8;
+                    const float* wsc = nullptr;
+                    if constexpr (F == F_F8) wsc = a.sc[t] + ((gd.x * a.rows + min64(row, a.rows - 1)) / 128) * a.nblk + 2 * cg;
+                    moe_cg<F, NB>(p0, p1, i, rec, xs, a.nblk - kPerCg * cg, wsc, tot[t]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.empty[s]);
+            if (++s == a.stages) {
+                s = 0;
+                par ^= 1;
+            }
+        }
+        // join the warps of each unit (two buffers: the next round's sums may be written while slow warps still read)
+        float* rb = red + ((rd - lo) & 1) * (kConsumers * 2 * kTok * 16);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float* q = rb + ((warp * 2 + t) * kTok + 4 * n + i) * 16;
+                q[g] = tot[t][n][0];
+                q[g + 8] = tot[t][n][1];
+            }
+        asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+        const int per_unit = a.gate_up ? kTok * 16 : kTok * 32;
+        for (int o = threadIdx.x; o < a.slots * per_unit; o += kConsumers * 32) {
+            const int un = o / per_unit, r = o - un * per_unit;
+            const int tl = static_cast<int>(rd - grp * per) * a.slots + un;
+            // outputs of a unit: [token][row]
+            const int t = a.gate_up ? r >> 4 : r >> 5, rr = a.gate_up ? r & 15 : r & 31;
+            const int64_t row = static_cast<int64_t>(tl) * (a.gate_up ? 16 : 32) + rr;
+            if (tl >= a.tiles || row >= a.rows || t >= gd.z) continue;
+            float v[2] = {0.0f, 0.0f};
+            for (int w = un * a.wps; w < (un + 1) * a.wps; ++w) {
+                if (a.gate_up) {
+                    v[0] += rb[((w * 2) * kTok + t) * 16 + rr];
+                    v[1] += rb[((w * 2 + 1) * kTok + t) * 16 + rr];
+                } else {
+                    v[0] += rb[((w * 2 + (rr >> 4)) * kTok + t) * 16 + (rr & 15)];
+                }
+            }
+            const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
+            a.out[static_cast<int64_t>(a.plan.pairs[gd.y + t]) * a.rows + row] = z;
+        }
+    }
+}
+
+// y[t][c] = sum_j p[t][j] z[t top_k + j][c], j in order; ids out of range add nothing.
+template <typename T>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const float* __restrict__ z, const int* __restrict__ ids,
+                                                          const float* __restrict__ wt, T* __restrict__ y, int64_t tokens,
+                                                          int64_t hidden, int top_k, int experts) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t n = tokens * hidden;
+    for (int64_t o = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; o < n;
+         o += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t t = o / hidden, c = o - t * hidden;
+        float v = 0.0f;
+        for (int j = 0; j < top_k; ++j) {
+            const int64_t p = t * top_k + j;
+            if (static_cast<unsigned>(ids[p]) < static_cast<unsigned>(experts)) v = fmaf(wt[p], z[p * hidden + c], v);
+        }
+        y[o] = Elem<T>::put(v);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+template <class Fn>
+cudaError_t with_moe_fmt(int fmt, Fn&& f) {
+    switch (fmt) {
+        case F_Q8_0: return f(std::integral_constant<int, F_Q8_0>{});
+        case F_Q4_0: return f(std::integral_constant<int, F_Q4_0>{});
+        case F_Q2_K: return f(std::integral_constant<int, F_Q2_K>{});
+        case F_Q3_K: return f(std::integral_constant<int, F_Q3_K>{});
+        case F_Q4_K: return f(std::integral_constant<int, F_Q4_K>{});
+        case F_Q5_K: return f(std::integral_constant<int, F_Q5_K>{});
+        case F_Q6_K: return f(std::integral_constant<int, F_Q6_K>{});
+        case F_F8: return f(std::integral_constant<int, F_F8>{});
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+template <int F, int NB>
+cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
+    constexpr int CGB = moe_cg_bytes<F>();
+    a.ncg = static_cast<int>((cols + 255) / 256);
+    if constexpr (F == F_F8) {
+        a.nblk = static_cast<int>((cols + 127) / 128);
+        a.row_bytes = cols;
+    } else {
+        constexpr int BE = Traits<F>::BE;
+        const int64_t blocks = (cols + BE - 1) / BE;
+        a.nblk = static_cast<int>(blocks) * (BE == 256 ? 8 : 1);
+        a.row_bytes = a.rb = blocks * Traits<F>::BB;
+    }
+    // short rows: several units share a stage, so that every warp has a CG
+    a.slots = a.ncg <= 2 ? 4 : a.ncg <= 4 ? 2 : 1;
+    a.wps = kConsumers / a.slots;
+    a.tiles = static_cast<int>((a.rows + (a.gate_up ? 15 : 31)) / (a.gate_up ? 16 : 32));
+    // row stride of a stage: the segment, its phase of up to 15 bytes, the 4 that word loads read past it, rounded
+    // to an odd multiple of 16 so that eight rows start in different banks
+    const int cgs = std::min(a.wps, a.ncg);
+    a.rs = (cgs * CGB + 15 + 4 + 15) / 16 * 16;
+    while (a.rs % 128 != 16) a.rs += 16;
+    a.stage_bytes = a.slots * kTileRows * a.rs;
+    const int red = 2 * kConsumers * 2 * 4 * NB * 16 * 4;
+    const int budget = 112 * 1024 - 512 - red;  // two CTAs per SM
+    a.stages = std::min(kMoeStages, budget / a.stage_bytes);
+    int per_sm = 2;
+    if (a.stages < 2) {
+        a.stages = std::min(kMoeStages, (224 * 1024 - 512 - red) / a.stage_bytes);
+        per_sm = 1;
+    }
+    if (a.stages < 2) return cudaErrorInvalidConfiguration;
+    const int smem = a.stages * a.stage_bytes + red + 128;
+    static std::atomic<int> cfg[64];
+    if (cudaError_t e = ensure_dyn_smem(moe_expert_kernel<F, NB>, smem, cfg); e != cudaSuccess) return e;
+    cudaError_t e = launch_pdl(moe_expert_kernel<F, NB>, dim3(static_cast<unsigned>(device_sm_count() * per_sm)),
+                               dim3(kMoeThreads), smem, s, a);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int nb, cudaStream_t s) {
+    return with_moe_fmt(fmt, [&](auto f) {
+        constexpr int F = decltype(f)::value;
+        return nb == 1 ? launch_expert<F, 1>(a, cols, s) : launch_expert<F, 2>(a, cols, s);
+    });
+}
+
+template <typename T>
+cudaError_t launch_prep(int fmt, const T* x, int64_t rows, int64_t cols, uint8_t* rec, const int* need, int experts,
+                        const MoePlan& plan, cudaStream_t s) {
+    const int ncg = static_cast<int>((cols + 255) / 256);
+    const int64_t grid = (rows * ncg + kPrepWarps - 1) / kPrepWarps + (plan.ids ? 1 : 0);
+    return with_moe_fmt(fmt, [&](auto f) {
+        constexpr int F = decltype(f)::value;
+        cudaError_t e = launch_pdl(moe_prep_kernel<F, T>, dim3(static_cast<unsigned>(grid)), dim3(32 * kPrepWarps), 0, s, x,
+                                   rows, cols, ncg, rec, need, experts, plan);
+        return e == cudaSuccess ? cudaGetLastError() : e;
+    });
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Tokens of one pass: their choices fit the plan.
+int64_t pass_tokens(int top_k) { return std::max<int64_t>(1, kMoePairs / top_k); }
+
+struct MoeSpace {
+    size_t plan, rec_x, rec_h, h, z, total;
+};
+
+MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
+    const int64_t t = std::min(tokens, pass_tokens(top_k)), p = t * top_k;
+    MoeSpace w{};
+    size_t at = 256;  // status word
+    auto take = [&](size_t n) {
+        const size_t r = at;
+        at += up256(n);
+        return r;
+    };
+    w.plan = take(kMoePlanBytes);
+    w.rec_x = take(static_cast<size_t>(t) * ((hidden + 255) / 256) * kRec);
+    w.rec_h = take(static_cast<size_t>(p) * ((ffn + 255) / 256) * kRec);
+    w.h = take(static_cast<size_t>(p) * ffn * 4);
+    w.z = take(static_cast<size_t>(p) * hidden * 4);
+    w.total = at;
+    return w;
+}
+
+}  // namespace
+
+size_t moe_workspace_bytes(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
+    return moe_space(tokens, top_k, hidden, ffn).total;
+}
+
+cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens,
+                               int experts, int top_k, int64_t hidden, int normalize, cudaStream_t s) {
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const bool vec = hidden % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                         reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
+        const int64_t clusters = (tokens + kRouteTokens - 1) / kRouteTokens;
+        const size_t smem = static_cast<size_t>(kRouteTokens) * experts * 4;
+        cudaError_t e = launch_pdl(moe_route_kernel<T>, dim3(static_cast<unsigned>(clusters * kRouteCtas)),
+                                   dim3(32 * kRouteWarps), smem, s, static_cast<const T*>(x), w, ids, weights, tokens,
+                                   experts, top_k, hidden, normalize, vec);
+        return e == cudaSuccess ? cudaGetLastError() : e;
+    });
+}
+
+cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s) {
+    const MoeSpace w = moe_space(m.tokens, m.top_k, m.hidden, m.ffn);
+    auto* base = static_cast<uint8_t*>(ws);
+    const int64_t step = pass_tokens(m.top_k);
+    const int size = host_dtype_size(m.dtype);
+    for (int64_t t0 = 0; t0 < m.tokens; t0 += step) {
+        const int64_t t = std::min(step, m.tokens - t0), p = t * m.top_k;
+        // groups of 4 tokens unless the experts have more on average: the second block of columns costs registers
+        const int nb = p > 4 * m.experts ? 2 : 1;
+        MoePlan plan = moe_plan_at(base + w.plan);
+        plan.ids = m.ids + t0 * m.top_k;
+        plan.npairs = static_cast<int>(p);
+        plan.experts = m.experts;
+        plan.group = 4 * nb;
+        plan.err = t0 == 0 ? err : nullptr;
+        const MoePlan made = [&] {
+            MoePlan q = plan;
+            q.ids = nullptr;
+            return q;
+        }();
+        const void* x = static_cast<const uint8_t*>(m.x) + t0 * m.hidden * size;
+        void* y = static_cast<uint8_t*>(m.y) + t0 * m.hidden * size;
+        float* h = reinterpret_cast<float*>(base + w.h);
+        float* z = reinterpret_cast<float*>(base + w.z);
+        cudaError_t e = with_dtype(m.dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            return launch_prep<T>(m.fmt, static_cast<const T*>(x), t, m.hidden, base + w.rec_x, nullptr, m.experts, plan, s);
+        });
+        if (e != cudaSuccess) return e;
+        ExpertArgs a{};
+        a.w[0] = static_cast<const uint8_t*>(m.w_gate);
+        a.w[1] = static_cast<const uint8_t*>(m.w_up);
+        a.sc[0] = m.s_gate;
+        a.sc[1] = m.s_up;
+        a.rb = m.hidden;  // e4m3; the packed formats set their own
+        a.w_bytes = m.gate_bytes;
+        a.rows = m.ffn;
+        a.gate_up = 1;
+        a.rec = base + w.rec_x;
+        a.rec_row = (m.hidden + 255) / 256 * kRec;
+        a.rec_div = m.top_k;
+        a.out = h;
+        a.plan = made;
+        a.err = err;
+        if (e = launch_experts(m.fmt, a, m.hidden, nb, s); e != cudaSuccess) return e;
+        e = launch_prep<float>(m.fmt_down, h, p, m.ffn, base + w.rec_h, plan.ids, m.experts, made, s);
+        if (e != cudaSuccess) return e;
+        a.w[0] = a.w[1] = static_cast<const uint8_t*>(m.w_down);
+        a.sc[0] = a.sc[1] = m.s_down;
+        a.rb = m.ffn;
+        a.w_bytes = m.down_bytes;
+        a.rows = m.hidden;
+        a.gate_up = 0;
+        a.rec = base + w.rec_h;
+        a.rec_row = (m.ffn + 255) / 256 * kRec;
+        a.rec_div = 1;
+        a.out = z;
+        if (e = launch_experts(m.fmt_down, a, m.ffn, nb, s); e != cudaSuccess) return e;
+        e = with_dtype(m.dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            const int64_t grid = std::min<int64_t>((t * m.hidden + 255) / 256, int64_t(device_sm_count()) * 8);
+            cudaError_t r = launch_pdl(moe_combine_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s,
+                                       static_cast<const float*>(z), plan.ids, m.weights + t0 * m.top_k, static_cast<T*>(y),
+                                       t, m.hidden, m.top_k, m.experts);
+            return r == cudaSuccess ? cudaGetLastError() : r;
+        });
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+}  // namespace axq

@@ -1,0 +1,94 @@
+// The plan of a mixture-of-experts pass: the tokens' choices ("pairs", p = token
+// * top_k + j) sorted by expert, cut into groups of tokens that share a read of
+// the expert's weights.
+#pragma once
+
+#include <cstdint>
+
+namespace axq {
+
+constexpr int kMoePairs = 512;     // choices of one pass, at most
+constexpr int kMoeExperts = 1024;  // experts, at most
+
+struct MoePlan {
+    const int* ids;  // null once the plan is made
+    int npairs, experts, group;
+    int* ngroups;
+    int4* groups;    // expert, first entry of pairs, entries
+    int* pairs;
+    int* err;        // status word to clear, or null
+};
+
+constexpr size_t kMoePlanBytes = 256 + kMoePairs * 16 + kMoePairs * 4;
+
+inline MoePlan moe_plan_at(uint8_t* p) {
+    MoePlan m{};
+    m.ngroups = reinterpret_cast<int*>(p);
+    m.groups = reinterpret_cast<int4*>(p + 256);
+    m.pairs = reinterpret_cast<int*>(p + 256 + kMoePairs * 16);
+    return m;
+}
+
+// Makes the plan with one block of 256 threads.  Ids out of range (a padded
+// token, an expert held elsewhere) appear in no group.
+__device__ __forceinline__ void moe_make_plan(const MoePlan& m) {
+    __shared__ int ids[kMoePairs];
+    __shared__ int first[kMoeExperts];
+    __shared__ int warp_sum[2][8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0 && m.err) *m.err = 0;
+    for (int p = tid; p < m.npairs; p += 256) ids[p] = m.ids[p];
+    __syncthreads();
+    // counts of experts 4 tid .. 4 tid + 3, then sums over the experts before
+    int cnt[4] = {0, 0, 0, 0};
+    for (int p = 0; p < m.npairs; ++p) {
+        const int d = ids[p] - 4 * tid;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cnt[j] += (d == j && ids[p] < m.experts) ? 1 : 0;
+    }
+    int c = 0, g = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        c += cnt[j];
+        g += (cnt[j] + m.group - 1) / m.group;
+    }
+    int ci = c, gi = g;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int a = __shfl_up_sync(0xFFFFFFFFu, ci, d), b = __shfl_up_sync(0xFFFFFFFFu, gi, d);
+        if (lane >= d) {
+            ci += a;
+            gi += b;
+        }
+    }
+    if (lane == 31) {
+        warp_sum[0][warp] = ci;
+        warp_sum[1][warp] = gi;
+    }
+    __syncthreads();
+    int cb = ci - c, gb = gi - g;
+    for (int w = 0; w < warp; ++w) {
+        cb += warp_sum[0][w];
+        gb += warp_sum[1][w];
+    }
+    if (tid == 255) *m.ngroups = gb + g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        first[4 * tid + j] = cb;
+        for (int k = 0; k * m.group < cnt[j]; ++k)
+            m.groups[gb + k] = make_int4(4 * tid + j, cb + k * m.group, min(m.group, cnt[j] - k * m.group), 0);
+        cb += cnt[j];
+        gb += (cnt[j] + m.group - 1) / m.group;
+    }
+    __syncthreads();
+    // a pair's place: after the earlier pairs of its expert
+    for (int p = tid; p < m.npairs; p += 256) {
+        const int e = ids[p];
+        if (static_cast<unsigned>(e) >= static_cast<unsigned>(m.experts)) continue;
+        int r = first[e];
+        for (int q = 0; q < p; ++q) r += ids[q] == e ? 1 : 0;
+        m.pairs[r] = p;
+    }
+}
+
+}  // namespace axq

@@ -1,0 +1,392 @@
+// Decoders of packed weight rows into mma.sync m16n8k16 A fragments (fp16,
+// exact) for the mixture-of-experts kernels.
+//
+// A column group (CG) is 256 elements of a row.  Lane (g, i) = (lane / 4,
+// lane % 4) of a warp holds, of each of its rows, 64 of a CG's elements: which
+// ones is each format's choice, as long as the activation records hold x in the
+// same order (Order<F>::elem).  In the formats with integer sub-block scales a
+// lane owns whole sub-blocks, so that it decodes only their scales.
+//
+// fp16 holds integers up to 2048 exactly, and 0x6400 | c is 1024 + c.  So
+// (1024 + c * 2^s) * (sc / 2^s) - 1024 * sc / 2^s, one FMA on two codes, is
+// sc * c exactly wherever |sc * c| <= 2048 (or has at most 11 significant
+// bits): code extraction, conversion and sub-block scale cost a mask and an FMA
+// for two elements, and the MMAs add a whole CG without touching the sums.  The
+// block's fp16 d and dmin are applied in fp32 once per CG.
+#pragma once
+
+#include "axq_common.cuh"
+#include "axq_f8.cuh"
+#include "axq_ptx.cuh"
+
+namespace axq {
+
+constexpr int F_F8 = 64;  // AXQ_F8_E4M3: e4m3 codes with 128 x 128 scales
+
+// Element (0..255) of the CG at slot 0..3 of MMA m (0..15) of lane part i.
+// Slots 0, 1 are the low and high half of the first fragment register, 2, 3 of
+// the second.  SUMS: sub-blocks whose sums of x weigh the minimums (0: none);
+// sum(i, j) is the sub-block at slot j of lane part i, -1 where there is none.
+template <int F> struct Order {
+    static constexpr bool K4 = F == F_Q4_K || F == F_Q5_K;
+    static constexpr bool K16 = F == F_Q2_K || F == F_Q3_K || F == F_Q6_K;
+    static constexpr int SUMS = K4 ? 8 : K16 ? 16 : 0;
+    __host__ __device__ static constexpr int elem(int m, int i, int slot) {
+        const int bo = slot == 1 ? 2 : slot == 2 ? 1 : slot;  // bytes 0, 2 of a word, then 1, 3
+        if (K4) return 64 * i + 32 * (m & 1) + 4 * (m >> 1) + bo;
+        if (K16) {
+            // Q2_K: lane part i starts at word i of its four (conflict-free loads)
+            const int v = F == F_Q2_K ? ((m >> 2) + i) & 3 : m >> 2;
+            return 128 * (i >> 1) + 32 * (m & 3) + 16 * (i & 1) + 4 * v + bo;
+        }
+        if (F == F_Q8_0) return 32 * (m >> 1) + 8 * i + 4 * (m & 1) + slot;
+        if (F == F_Q4_0) return 32 * (m >> 1) + 2 * (4 * i + bo) + (m & 1);
+        return 128 * (m >> 3) + 32 * i + 4 * (m & 7) + slot;  // e4m3
+    }
+    __host__ __device__ static constexpr int sum(int i, int j) {
+        if (K4) return j < 2 ? 2 * i + j : -1;
+        if (K16) return 8 * (i >> 1) + 2 * j + (i & 1);
+        return -1;
+    }
+};
+
+template <int F> constexpr int moe_cg_bytes() {
+    return F == F_F8 ? 256 : F == F_Q8_0 ? 8 * 34 : F == F_Q4_0 ? 8 * 18 : Traits<F == F_F8 ? F_Q4_K : F>::BB;
+}
+
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t h2_const(float v) {
+    const __half2 h = __float2half2_rn(v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// A small integer as an fp16 pair (v, v).
+__device__ __forceinline__ uint32_t h2_of(int v) {
+    const __half2 h = __half2half2(__int2half_rn(v));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t h2_of2(int lo, int hi) {
+    const __half2 h = __halves2half2(__int2half_rn(lo), __int2half_rn(hi));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (w & MASK) | OR in one LOP3.
+template <uint32_t MASK, uint32_t OR>
+__device__ __forceinline__ uint32_t and_or(uint32_t w) { return (w & MASK) | OR; }
+
+constexpr uint32_t kMagic = 0x64006400u;  // 1024 in both halves
+
+// Words at a 2-byte aligned shared address: the two aligned words around each.
+template <int N>
+__device__ __forceinline__ void ld_words2(const uint8_t* p, uint32_t (&out)[N]) {
+    const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
+    const uint32_t* b = reinterpret_cast<const uint32_t*>(p - mis);
+    uint32_t w[N + 1];
+#pragma unroll
+    for (int k = 0; k <= N; ++k) w[k] = b[k];
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = __funnelshift_r(w[k], w[k + 1], mis * 8);
+}
+
+__device__ __forceinline__ uint32_t ld_half2b(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
+
+// Row<F>: one row's part of one CG.  load(p, i) reads the header; pair<MP>(a)
+// gives the fragments of MMAs 2 MP (a[0], a[1]) and 2 MP + 1 (a[2], a[3]);
+// mins(a) those of the minimums' MMA (sub-block sums of x against them); d() and
+// dm() scale the sums of codes and of minimums.
+template <int F> struct MoeRow;
+
+// Q4_K {d, dmin, scales[12], qs[128]}: lane part i owns qs[32i ..], the
+// sub-blocks 2i (low nibbles) and 2i + 1 (high nibbles): 63 * 15 <= 2048.
+// Q5_K {d, dmin, scales[12], qh[32], qs[128]}: the fifth bit of sub-block s is
+// bit s of qh[l]: 63 * 31 <= 2048.
+template <int F> struct MoeRowK45 {
+    const uint8_t* q;
+    uint32_t hd, w[4], h[4];
+    uint32_t scl, cl, sch, ch, mn;
+    int sh;
+    const uint8_t* qh;
+    __device__ __forceinline__ void load(const uint8_t* p, int i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        hd = v.x;
+        // 6-bit scales and minimums j = 2i, 2i + 1 (get_scale_min_k4): bytes 0-3 hold scales 0-3, 4-7 minimums 0-3,
+        // 8-11 the low halves of both for 4-7, whose high two bits are the top bits of the first eight bytes
+        const int by = 16 * (i & 1);  // bit offset of bytes 2i & 3 ..
+        const uint32_t s0 = v.y >> by, m0 = v.z >> by, t0 = v.w >> by;
+        int sa, sb, ma, mb;
+        if (i < 2) {
+            sa = s0 & 63; sb = (s0 >> 8) & 63;
+            ma = m0 & 63; mb = (m0 >> 8) & 63;
+        } else {
+            sa = (t0 & 15) | ((s0 >> 2) & 0x30); sb = ((t0 >> 8) & 15) | ((s0 >> 10) & 0x30);
+            ma = ((t0 >> 4) & 15) | ((m0 >> 2) & 0x30); mb = ((t0 >> 12) & 15) | ((m0 >> 10) & 0x30);
+        }
+        scl = h2_of(sa);
+        cl = hmul2(scl, h2_const(-1024.0f));
+        const uint32_t s1 = h2_of(sb);
+        sch = hmul2(s1, h2_const(0.0625f));
+        ch = hmul2(s1, h2_const(-64.0f));
+        mn = h2_of2(ma, mb);
+        q = p + (F == F_Q4_K ? 16 : 48) + 32 * i;
+        qh = p + 16;
+        sh = 2 * i;
+    }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        if constexpr (MP % 4 == 0) {
+            const uint4 v = *reinterpret_cast<const uint4*>(q + 4 * MP);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            if constexpr (F == F_Q5_K) {
+                const uint4 u = *reinterpret_cast<const uint4*>(qh + 4 * MP);
+                h[0] = u.x >> sh; h[1] = u.y >> sh; h[2] = u.z >> sh; h[3] = u.w >> sh;
+            }
+        }
+        const uint32_t x = w[MP % 4], y = x >> 8;
+        uint32_t t0 = and_or<0x000F000Fu, kMagic>(x), t1 = and_or<0x000F000Fu, kMagic>(y);
+        uint32_t t2 = and_or<0x00F000F0u, kMagic>(x), t3 = and_or<0x00F000F0u, kMagic>(y);
+        if constexpr (F == F_Q5_K) {
+            const uint32_t b = h[MP % 4];
+            t0 |= (b << 4) & 0x00100010u;
+            t1 |= (b >> 4) & 0x00100010u;
+            t2 |= (b << 7) & 0x01000100u;
+            t3 |= (b >> 1) & 0x01000100u;
+        }
+        a[0] = hfma2(t0, scl, cl);
+        a[1] = hfma2(t1, scl, cl);
+        a[2] = hfma2(t2, sch, ch);
+        a[3] = hfma2(t3, sch, ch);
+    }
+    __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn; a[1] = 0; }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd & 0xFFFFu); }
+    __device__ __forceinline__ float dm() const { return h2f_flush(hd >> 16); }
+};
+template <> struct MoeRow<F_Q4_K> : MoeRowK45<F_Q4_K> {};
+template <> struct MoeRow<F_Q5_K> : MoeRowK45<F_Q5_K> {};
+
+// Q2_K {d, dmin, scales[16], qs[64]}: lane part i owns qs[16i .. 16i + 15],
+// whose four 2-bit fields are sub-blocks 8(i/2) + 2j + (i%2), j = 0..3: 15 * 3.
+template <> struct MoeRow<F_Q2_K> {
+    const uint8_t* q;
+    uint32_t hd, sc[4], c[4], mn[2], w;
+    int rot;
+    __device__ __forceinline__ void load(const uint8_t* p, int i) {
+        hd = *reinterpret_cast<const uint32_t*>(p);
+        const uint32_t* s = reinterpret_cast<const uint32_t*>(p + 4 + 8 * (i >> 1));
+        const int by = 8 * (i & 1);
+        const uint32_t a = s[0] >> by, b = s[1] >> by;  // bytes 2j + (i & 1) at bits 0, 16
+        const int v[4] = {static_cast<int>(a & 255), static_cast<int>((a >> 16) & 255), static_cast<int>(b & 255),
+                          static_cast<int>((b >> 16) & 255)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t x = h2_of(v[j] & 15);
+            sc[j] = j ? hmul2(x, h2_const(1.0f / static_cast<float>(1 << (2 * j)))) : x;
+            c[j] = hmul2(x, h2_const(-1024.0f / static_cast<float>(1 << (2 * j))));
+        }
+        mn[0] = h2_of2(v[0] >> 4, v[1] >> 4);
+        mn[1] = h2_of2(v[2] >> 4, v[3] >> 4);
+        q = p + 20 + 16 * i;
+        rot = i;
+    }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        if constexpr (MP % 2 == 0) w = reinterpret_cast<const uint32_t*>(q)[(MP / 2 + rot) & 3];
+        constexpr int j = 2 * (MP % 2);  // MMA 2 MP: field j, MMA 2 MP + 1: field j + 1
+        constexpr uint32_t m0 = 0x00030003u << (2 * j), m1 = 0x00030003u << (2 * j + 2);
+        const uint32_t y = w >> 8;
+        a[0] = hfma2(and_or<m0, kMagic>(w), sc[j], c[j]);
+        a[1] = hfma2(and_or<m0, kMagic>(y), sc[j], c[j]);
+        a[2] = hfma2(and_or<m1, kMagic>(w), sc[j + 1], c[j + 1]);
+        a[3] = hfma2(and_or<m1, kMagic>(y), sc[j + 1], c[j + 1]);
+    }
+    __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd & 0xFFFFu); }
+    __device__ __forceinline__ float dm() const { return h2f_flush(hd >> 16); }
+};
+
+// Q3_K {hmask[32], qs[64], scales[12], d}: the fields of Q2_K with a third bit,
+// bit 4(i/2) + j of hmask[16(i%2) + l]; value = d * sc * (code - 4), sc = 6 bits
+// - 32.  The codes (0..7) go through the MMAs, 4 sc through the minimums'.
+template <> struct MoeRow<F_Q3_K> {
+    uint32_t hd, sc[4], c[4], mn[2], w[4], h[4];
+    __device__ __forceinline__ void load(const uint8_t* p, int i) {
+        hd = ld_half2b(p + 108);
+        uint32_t s[3];
+        ld_words2(p + 96, s);
+        // scale is = 8n + 2j + lh: low 4 bits in nibble n of byte 2j + lh of the first eight, high 2 bits at
+        // 2 (is >> 2) of byte 8 + (is & 3)
+        const int n = i >> 1, lh = i & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int by = 2 * j + lh;  // 0..7
+            const uint32_t lo = (s[j >> 1] >> (8 * (2 * (j & 1) + lh) + 4 * n)) & 15u;
+            const uint32_t hi = (s[2] >> (8 * (by & 3) + 2 * (2 * n + (j >> 1)))) & 3u;
+            const int v = static_cast<int>(lo | (hi << 4)) - 32;
+            const uint32_t x = h2_of(v);
+            sc[j] = j ? hmul2(x, h2_const(1.0f / static_cast<float>(1 << (2 * j)))) : x;
+            c[j] = hmul2(x, h2_const(-1024.0f / static_cast<float>(1 << (2 * j))));
+        }
+        const uint32_t lo16 = 0x5410u;
+        mn[0] = hmul2(__byte_perm(sc[0], sc[1], lo16), 0x4C004400u);  // 4 sc of fields 0 and 1 (field 1 is kept / 4)
+        mn[1] = hmul2(__byte_perm(sc[2], sc[3], lo16), 0x5C005400u);  // fields 2 and 3 (/ 16, / 64): x 64, x 256
+        ld_words2(p + 32 + 32 * n + 16 * lh, w);
+        ld_words2(p + 16 * lh, h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] >>= 4 * n;
+    }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        constexpr int j = 2 * (MP % 2);
+        constexpr uint32_t m0 = 0x00030003u << (2 * j), m1 = 0x00030003u << (2 * j + 2);
+        constexpr uint32_t b0 = 0x00040004u << (2 * j), b1 = 0x00040004u << (2 * j + 2);
+        const uint32_t x = w[MP / 2], y = x >> 8, b = h[MP / 2];
+        a[0] = hfma2(and_or<m0, kMagic>(x) | ((b << (j + 2)) & b0), sc[j], c[j]);
+        a[1] = hfma2(and_or<m0, kMagic>(y) | ((b >> (6 - j)) & b0), sc[j], c[j]);
+        a[2] = hfma2(and_or<m1, kMagic>(x) | ((b << (j + 3)) & b1), sc[j + 1], c[j + 1]);
+        a[3] = hfma2(and_or<m1, kMagic>(y) | ((b >> (5 - j)) & b1), sc[j + 1], c[j + 1]);
+    }
+    __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
+    __device__ __forceinline__ float dm() const { return h2f_flush(hd); }
+};
+
+// Q6_K {ql[128], qh[64], scales[16], d}: field t of lane part i is sub-block
+// 8(i/2) + 2t + (i%2); code = 4 bits of ql + 16 * 2 bits of qh, value = d * sc *
+// (code - 32) with sc of 8 bits.  sc * code does not fit fp16, its two parts do:
+// |sc| * 15 <= 1920 and |sc| * 16 * {0..3}, so each MMA is issued twice, on the
+// low and on the high bits; 32 sc goes through the minimums'.  Scales are kept /
+// 4, so that 1024 * sc / 4 is finite.
+template <> struct MoeRow<F_Q6_K> {
+    uint32_t hd, sc[4], mn[2], lo[8], hi[4];
+    __device__ __forceinline__ void load(const uint8_t* p, int i) {
+        const int n = i >> 1, lh = i & 1;
+        hd = ld_half2b(p + 208);
+        uint32_t s[2];
+        ld_words2(p + 192 + 8 * n, s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int v = static_cast<int8_t>(s[t >> 1] >> (8 * (2 * (t & 1) + lh)));
+            sc[t] = hmul2(h2_of(v), h2_const(0.25f));
+        }
+        mn[0] = __byte_perm(sc[0], sc[1], 0x5410u);
+        mn[1] = __byte_perm(sc[2], sc[3], 0x5410u);
+        uint32_t a[4], b[4];
+        ld_words2(p + 64 * n + 16 * lh, a);
+        ld_words2(p + 64 * n + 32 + 16 * lh, b);
+        ld_words2(p + 128 + 32 * n + 16 * lh, hi);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            lo[k] = a[k];      // fields 0 (low nibbles) and 2 (high)
+            lo[4 + k] = b[k];  // fields 1 and 3
+        }
+    }
+    // low bits (a) and high bits (b) of MMAs 2 MP, 2 MP + 1: fields t, t + 1 of word MP / 2
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4], uint32_t (&b)[4]) {
+        constexpr int t = 2 * (MP % 2), v = MP / 2;
+        const uint32_t m256 = h2_const(-1024.0f), m64 = h2_const(-64.0f), s16 = h2_const(0.0625f);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {  // fields t, t + 1: the nibble at bit 0 (t = 0) or 4 (t = 2) of lo[4f + v]
+            const uint32_t x = lo[4 * f + v], y = x >> 8;
+            const uint32_t s = sc[t + f];
+            if constexpr (t == 0) {
+                const uint32_t c = hmul2(s, m256);
+                a[2 * f] = hfma2(and_or<0x000F000Fu, kMagic>(x), s, c);
+                a[2 * f + 1] = hfma2(and_or<0x000F000Fu, kMagic>(y), s, c);
+            } else {
+                const uint32_t c = hmul2(s, m64), r = hmul2(s, s16);
+                a[2 * f] = hfma2(and_or<0x00F000F0u, kMagic>(x), r, c);
+                a[2 * f + 1] = hfma2(and_or<0x00F000F0u, kMagic>(y), r, c);
+            }
+            // 2 bits at 2 (t + f) of hi[v]: 16 * s * field; in place the field is x 4^(t + f)
+            const uint32_t z = hi[v], u = z >> 8;
+            constexpr float k0 = 16.0f / static_cast<float>(1 << (2 * t)), k1 = 4.0f / static_cast<float>(1 << (2 * t));
+            const uint32_t r = hmul2(s, f ? h2_const(k1) : h2_const(k0));
+            // (1024 + field * 4^n) * r - 1024 * r: 1024 * r <= 16 * 32 * 1024 would overflow for n = 0, so subtract first
+            const uint32_t one = h2_const(-1024.0f), unit = h2_const(1.0f);
+            const uint32_t mk = f ? 0x00030003u << (2 * t + 2) : 0x00030003u << (2 * t);
+            b[2 * f] = hmul2(hfma2((z & mk) | kMagic, unit, one), r);
+            b[2 * f + 1] = hmul2(hfma2((u & mk) | kMagic, unit, one), r);
+        }
+    }
+    __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd) * 4.0f; }
+    __device__ __forceinline__ float dm() const { return h2f_flush(hd) * 128.0f; }
+};
+
+// Q8_0 {d, qs[32]} x 8 and Q4_0 {d, qs[16]} x 8: a block's d is fp16, so its
+// two MMAs (2 MP and 2 MP + 1 are block MP) are scaled in fp32; lane part i
+// holds 8 elements of every block.
+template <> struct MoeRow<F_Q8_0> {
+    const uint8_t* p;
+    int i;
+    uint32_t hd;
+    __device__ __forceinline__ void load(const uint8_t* q, int part) { p = q; i = part; }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        hd = ld_half2b(p + 34 * MP);
+        uint32_t w[2];
+        ld_words2(p + 34 * MP + 2 + 8 * i, w);
+        const uint32_t off = h2_const(-1152.0f), unit = h2_const(1.0f);  // 1024 + 128
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t u = w[k] ^ 0x80808080u;
+            a[2 * k] = hfma2(__byte_perm(u, 0x64646464u, 0x4140u), unit, off);
+            a[2 * k + 1] = hfma2(__byte_perm(u, 0x64646464u, 0x4342u), unit, off);
+        }
+    }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
+};
+template <> struct MoeRow<F_Q4_0> {
+    const uint8_t* p;
+    int i;
+    uint32_t hd;
+    __device__ __forceinline__ void load(const uint8_t* q, int part) { p = q; i = part; }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        hd = ld_half2b(p + 18 * MP);
+        uint32_t w[1];
+        ld_words2(p + 18 * MP + 2 + 4 * i, w);
+        const uint32_t x = w[0], y = x >> 8;
+        const uint32_t unit = h2_const(1.0f), o0 = h2_const(-1032.0f), s = h2_const(0.0625f), o1 = h2_const(-72.0f);
+        a[0] = hfma2(and_or<0x000F000Fu, kMagic>(x), unit, o0);
+        a[1] = hfma2(and_or<0x000F000Fu, kMagic>(y), unit, o0);
+        a[2] = hfma2(and_or<0x00F000F0u, kMagic>(x), s, o1);
+        a[3] = hfma2(and_or<0x00F000F0u, kMagic>(y), s, o1);
+    }
+    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
+};
+
+// e4m3: MMAs 0-7 are the first 128 columns, 8-15 the second; each half has one
+// fp32 scale for the whole tile of rows.
+template <> struct MoeRow<F_F8> {
+    const uint8_t* p;
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const uint8_t* q, int i) { p = q + 32 * i; }
+    __device__ __forceinline__ static uint32_t cvt(uint32_t two) {
+        uint32_t r;
+        asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(two));
+        return r;
+    }
+    template <int MP>
+    __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
+        if constexpr (MP % 2 == 0) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + 128 * (MP / 4) + 8 * (MP % 4));
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t x = w[2 * (MP % 2) + k];
+            a[2 * k] = cvt(x);
+            a[2 * k + 1] = cvt(x >> 16);
+        }
+    }
+};
+
+}  // namespace axq

@@ -1,0 +1,104 @@
+"""Mixture-of-experts layer for a few tokens on packed experts.
+
+Beside :func:`gate_up_silu` and :func:`mlp_q`: the same gated block, with each
+token's experts chosen by a router.  Expert weights are one tensor per matrix,
+the experts' rows after one another: a :class:`QTensor` in any packed format or
+an :class:`F8Tensor` in 128 x 128 blocks.  The reference (ruwwww/Axon) has no
+router and no gated block.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from ._capi import BLOCK_BYTES, F8_BLOCK, F8_E4M3, check, lib
+from .f8 import F8Tensor, _float_type, _invalid, _on, _same_device, _scratch
+from .ops import QTensor, _packed_bytes, _req_cuda, _stream_handle
+
+
+def _weights(w, rows: int, cols: int, name: str):
+    """(format id, codes, scales or None) of experts' weights [rows x cols]."""
+    if tuple(w.shape) != (rows, cols):
+        raise _invalid(f"{name} must be [{rows} x {cols}] (got {tuple(w.shape)})")
+    if isinstance(w, F8Tensor):
+        w._check(name)
+        if w.block_rows != F8_BLOCK or w.data.shape[1] != cols:
+            raise _invalid(f"{name}: e4m3 experts are packed in 128 x 128 blocks, their rows without padding")
+        return F8_E4M3, w.data, w.scales
+    if not isinstance(w, QTensor) or w.fmt not in BLOCK_BYTES:
+        raise _invalid(f"{name} must be a QTensor or an F8Tensor")
+    _req_cuda(w.data, name, torch.uint8)
+    if w.data.numel() < _packed_bytes(rows, cols, w.fmt):
+        raise _invalid(f"{name} is smaller than its shape")
+    return int(w.fmt), w.data, None
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bool = True,
+              stream: Optional[torch.cuda.Stream] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(ids int32 [N, top_k], weights fp32 [N, top_k]) of the top_k largest of
+    softmax(x . w_router^T), largest first, ties to the lowest index.
+
+    x is fp32, fp16 or bf16 [N, hidden], w_router fp32 [experts, hidden];
+    ``normalize``: a token's weights add up to 1."""
+    dtype = _float_type(x, "x")
+    _req_cuda(w_router, "w_router", torch.float32)
+    if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
+        raise _invalid("moe_route: x must be [N x hidden] and w_router [experts x hidden]")
+    _same_device(x.device, w_router=w_router)
+    n = x.shape[0]
+    with _on(x.device, stream):
+        ids = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
+        weights = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
+        check(lib().axq_moe_route(int(dtype), x.data_ptr(), w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), n,
+                                  w_router.shape[0], top_k, x.shape[1], int(normalize), _stream_handle(stream, x.device)))
+    return ids, weights
+
+
+def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate, w_up, w_down, experts: int,
+              out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """y[t] = sum_j weights[t, j] * W_down[e] . (silu(W_gate[e] . x[t]) * (W_up[e] . x[t])), e = ids[t, j].
+
+    x [N, hidden] in fp32, fp16 or bf16; ids int32 [N, top_k] (an id outside
+    0 .. experts - 1 adds nothing); w_gate and w_up [experts * ffn, hidden] in one
+    format, w_down [experts * hidden, ffn].  Products and sums are fp32, y has x's
+    type."""
+    dtype = _float_type(x, "x")
+    _req_cuda(ids, "ids", torch.int32)
+    _req_cuda(weights, "weights", torch.float32)
+    if x.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != weights.shape:
+        raise _invalid("moe_mlp_q: x must be [N x hidden], ids and weights [N x top_k]")
+    (n, hidden), top_k = x.shape, ids.shape[1]
+    if experts < 1 or w_gate.shape[0] % experts:
+        raise _invalid("moe_mlp_q: w_gate must have experts * ffn rows")
+    ffn = w_gate.shape[0] // experts
+    fmt, gate, gate_s = _weights(w_gate, experts * ffn, hidden, "w_gate")
+    fmt_up, up, up_s = _weights(w_up, experts * ffn, hidden, "w_up")
+    fmt_down, down, down_s = _weights(w_down, experts * hidden, ffn, "w_down")
+    if fmt != fmt_up:
+        raise _invalid("moe_mlp_q: w_gate and w_up must have the same format")
+    _same_device(x.device, ids=ids, weights=weights, w_gate=gate, w_up=up, w_down=down, out=out)
+    with _on(x.device, stream):
+        if out is None:
+            out = torch.empty_like(x)
+        if _float_type(out, "out") != dtype or out.shape != x.shape:
+            raise _invalid("moe_mlp_q: out must have x's shape and type")
+        buf, wp, wbytes = _scratch(int(lib().axq_moe_workspace_size(n, top_k, hidden, ffn)), x.device)
+        check(lib().axq_moe_mlp(fmt, gate.data_ptr(), _ptr(gate_s), up.data_ptr(), _ptr(up_s), fmt_down, down.data_ptr(),
+                                _ptr(down_s), int(dtype), x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(),
+                                n, experts, top_k, hidden, ffn, wp, wbytes, _stream_handle(stream, x.device)))
+        del buf
+    return out
+
+
+def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: int, normalize: bool = True,
+          out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None
+          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The whole layer: :func:`moe_route`, then :func:`moe_mlp_q`.  Returns (y, ids, weights)."""
+    ids, weights = moe_route(x, w_router, top_k, normalize, stream)
+    y = moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, w_router.shape[0], out=out, stream=stream)
+    return y, ids, weights

@@ -290,6 +290,39 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
                   const float* x_scales, const float* bias, int y_dtype, void* y, int64_t out_features,
                   int64_t in_features, int64_t tokens, void* workspace, size_t workspace_bytes, axq_stream_t stream);
 
+/* ---- mixture of experts -------------------------------------------------------
+ * A layer for a few tokens on packed experts; it generalises axq_gate_up_silu and
+ * the down projection behind it to experts that each token chooses (the reference
+ * has neither). */
+#define AXQ_F8_E4M3 64 /* as a weight format: e4m3 codes with 128 x 128 scales */
+#define AXQ_MOE_MAX_EXPERTS 1024
+#define AXQ_MOE_MAX_TOP_K 32
+
+/* ids [tokens x top_k] and weights [tokens x top_k] of the top_k largest of
+ * softmax(x . W_router^T), largest first, ties to the lowest index (NaN logits
+ * last): x [tokens x hidden] in dtype F32, F16 or BF16, w_router [experts x hidden]
+ * fp32, both row-major.  normalize != 0: a token's weights are divided by their
+ * sum.  Logits and softmax are fp32. */
+int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids, float* weights, int64_t tokens,
+                  int64_t experts, int64_t top_k, int64_t hidden, int normalize, axq_stream_t stream);
+
+/* y[t] = sum_j weights[t][j] * W_down[e] . (silu(W_gate[e] . x[t]) * (W_up[e] .
+ * x[t])), e = ids[t][j], added in the order of j; an id outside 0 .. experts - 1
+ * adds nothing, and an expert may be named more than once.
+ * w_gate and w_up hold experts x ffn packed rows of hidden elements, w_down
+ * experts x hidden rows of ffn elements, each expert's after the one before, in
+ * the formats fmt (gate and up) and fmt_down, 16-byte aligned.  For AXQ_F8_E4M3
+ * the rows are codes without padding and *_scales their 128 x 128 scales (hidden
+ * and ffn multiples of 128); otherwise *_scales are NULL.  x and y are [tokens x
+ * hidden] in dtype F32, F16 or BF16.  Products and sums are fp32 (x and the hidden
+ * activations enter the tensor cores as two fp16 terms, 22 bits); y is rounded
+ * once.  Tokens beyond 512 / top_k take several passes over the experts. */
+size_t axq_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
+int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
+                int fmt_down, const void* w_down, const float* down_scales, int dtype, const void* x, const int32_t* ids,
+                const float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
+                int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream);
+
 /* ---- .axon tensor files ---------------------------------------------------
  * Replace save_tensor / load_tensor / save_checkpoint / load_checkpoint
  * (src/core/serialize.cpp:84-203) for device buffers.  The byte format is
