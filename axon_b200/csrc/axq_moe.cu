@@ -36,19 +36,21 @@ namespace {
 
 // ---- router ---------------------------------------------------------------------
 
-constexpr int kRouteCtas = 8, kRouteWarps = 8, kRouteTokens = 4;
+constexpr int kRouteCtas = 8, kRouteWarps = 16, kRouteTokens = 4;
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// Logits in fp32 (FMAs over lanes of 128 columns, then a tree over the lanes);
-// ties go to the lowest index, NaN logits are chosen last.
+// Logits in fp32 (FMAs over lanes of 128 columns, then a tree over the lanes,
+// then the slices in order); ties go to the lowest index, NaN logits are chosen
+// last.  The cluster's 128 warps take (expert, slice of the columns) each:
+// latency counts here, so few experts are cut into slices.
 template <typename T>
 __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRouteWarps)
     moe_route_kernel(const T* __restrict__ x, const float* __restrict__ w, int* __restrict__ ids, float* __restrict__ wt,
-                     int64_t tokens, int experts, int top_k, int64_t hidden, int normalize, bool vec) {
-    extern __shared__ float logits[];  // [kRouteTokens][experts], of the cluster's first CTA
+                     int64_t tokens, int experts, int top_k, int64_t hidden, int slices, int normalize, bool vec) {
+    extern __shared__ float logits[];  // [slice][kRouteTokens][experts], of the cluster's first CTA
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouteCtas) * kRouteTokens;
@@ -56,46 +58,59 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
     cluster_sync_all();  // the first CTA's shared memory is there
     pdl_wait();
     pdl_launch_dependents();
-    for (int e = static_cast<int>(rank) * kRouteWarps + warp; e < experts; e += kRouteCtas * kRouteWarps) {
+    const int64_t per = ((hidden + slices - 1) / slices + 127) / 128 * 128;  // columns of a slice
+    for (int o = static_cast<int>(rank) * kRouteWarps + warp; o < experts * slices; o += kRouteCtas * kRouteWarps) {
+        const int e = o / slices, sl = o - e * slices;
+        const int64_t k0 = sl * per, k1 = min64(k0 + per, hidden);
         float acc[kRouteTokens] = {};
         const float* we = w + static_cast<int64_t>(e) * hidden;
+        const T* xt = x + t0 * hidden;
         if (vec) {
-            for (int64_t k = 4 * lane; k < hidden; k += 128) {
-                const float4 a = *reinterpret_cast<const float4*>(we + k);
+#pragma unroll 4
+            for (int64_t k = k0 + 4 * lane; k < k1; k += 128) {
+                const float4 a = __ldg(reinterpret_cast<const float4*>(we + k));
 #pragma unroll
                 for (int t = 0; t < kRouteTokens; ++t) {
-                    if (t >= nt) break;
-                    const T* xp = x + (t0 + t) * hidden + k;
-                    float v[4];
-                    if constexpr (sizeof(T) == 4) {
-                        const float4 b = *reinterpret_cast<const float4*>(xp);
-                        v[0] = b.x; v[1] = b.y; v[2] = b.z; v[3] = b.w;
-                    } else {
-                        const uint2 b = *reinterpret_cast<const uint2*>(xp);
-                        T h[4];
-                        memcpy(h, &b, 8);
+                    if (t < nt) {
+                        const T* xp = xt + t * hidden + k;
+                        float v[4];
+                        if constexpr (sizeof(T) == 4) {
+                            const float4 b = __ldg(reinterpret_cast<const float4*>(xp));
+                            v[0] = b.x; v[1] = b.y; v[2] = b.z; v[3] = b.w;
+                        } else {
+                            const uint2 b = __ldg(reinterpret_cast<const uint2*>(xp));
+                            T h[4];
+                            memcpy(h, &b, 8);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = Elem<T>::get(h[i]);
+                            for (int i = 0; i < 4; ++i) v[i] = Elem<T>::get(h[i]);
+                        }
+                        acc[t] = fmaf(a.x, v[0], fmaf(a.y, v[1], fmaf(a.z, v[2], fmaf(a.w, v[3], acc[t]))));
                     }
-                    acc[t] = fmaf(a.x, v[0], fmaf(a.y, v[1], fmaf(a.z, v[2], fmaf(a.w, v[3], acc[t]))));
                 }
             }
         } else {
-            for (int64_t k = lane; k < hidden; k += 32)
+            for (int64_t k = k0 + lane; k < k1; k += 32)
 #pragma unroll
                 for (int t = 0; t < kRouteTokens; ++t)
-                    if (t < nt) acc[t] = fmaf(we[k], Elem<T>::get(x[(t0 + t) * hidden + k]), acc[t]);
+                    if (t < nt) acc[t] = fmaf(we[k], Elem<T>::get(xt[t * hidden + k]), acc[t]);
         }
 #pragma unroll
         for (int t = 0; t < kRouteTokens; ++t) {
 #pragma unroll
             for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(0xFFFFFFFFu, acc[t], d);
-            if (lane == 0 && t < nt) st_cluster_f32(cluster_addr(logits + t * experts + e, 0), acc[t]);
+            if (lane == 0 && t < nt)
+                st_cluster_f32(cluster_addr(logits + (sl * kRouteTokens + t) * experts + e, 0), acc[t]);
         }
     }
     cluster_sync_all();
     if (rank != 0 || warp >= nt) return;
     float* l = logits + warp * experts;
+    for (int e = lane; e < experts; e += 32) {
+        float v = l[e];
+        for (int sl = 1; sl < slices; ++sl) v += l[sl * kRouteTokens * experts + e];
+        l[e] = v;
+    }
+    __syncwarp();
     float mx = -INFINITY;
     for (int e = lane; e < experts; e += 32) mx = fmaxf(mx, l[e]);
 #pragma unroll
@@ -241,10 +256,10 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
 constexpr int kConsumers = 8;
 constexpr int kMoeThreads = (kConsumers + 1) * 32;
 constexpr int kMoeStages = 8;  // most
-constexpr int kTileRows = 32;  // rows of a unit: two tiles of 16
 
 struct MoeBars {
     uint64_t full[kMoeStages], empty[kMoeStages];
+    uint64_t sums[2];  // the partial sums of a round are written
     int abort;
 };
 
@@ -284,90 +299,144 @@ __device__ __forceinline__ void each_pair(Fn&& f) {
     each_pair_impl(f, std::make_integer_sequence<int, 8>{});
 }
 
-// One CG of one tile (rows g and g + 8 of it at p0, p1) times NB blocks of four
-// tokens: tot[n][r] += row r's product with token 4 n + i.
-template <int F, int NB>
-__device__ __forceinline__ void moe_cg(const uint8_t* p0, const uint8_t* p1, int i, const uint8_t* const (&rec)[NB],
-                                       const float (&xs)[NB], int blocks, const float* wsc, float (&tot)[NB][2]) {
-    MoeRow<F> r0, r1;
-    r0.load(p0, i);
-    r1.load(p1, i);
-    float acc[NB][4];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
-    each_pair([&](auto MPc) {
-        constexpr int MP = decltype(MPc)::value;
-        uint4 b[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) b[n] = __ldg(reinterpret_cast<const uint4*>(rec[n] + MP * 128));
-        uint32_t x[4], y[4];
-        if constexpr (F == F_Q6_K) {
-            uint32_t xh[4], yh[4];
-            r0.template pair<MP>(x, xh);
-            r1.template pair<MP>(y, yh);
-            const uint32_t h0[4] = {xh[0], yh[0], xh[1], yh[1]}, h1[4] = {xh[2], yh[2], xh[3], yh[3]};
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                mma16816(acc[n], h0, b[n].x, b[n].y);
-                mma16816(acc[n], h1, b[n].z, b[n].w);
-            }
-        } else {
-            r0.template pair<MP>(x);
-            r1.template pair<MP>(y);
-        }
-        const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+// The same for 0 .. N - 1.
+template <int N, class Fn>
+__device__ __forceinline__ void static_for_pairs(Fn&& f) {
+    each_pair_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// Sums of codes of one tile's CG over one pair of MMAs.
+template <int F, int MP, int NB>
+__device__ __forceinline__ void moe_pair(MoeRow<F> (&r)[2], const uint4 (&b)[NB], float (&acc)[NB][4]) {
+    uint32_t x[4], y[4];
+    if constexpr (F == F_Q6_K) {
+        uint32_t xh[4], yh[4];
+        r[0].template pair<MP>(x, xh);
+        r[1].template pair<MP>(y, yh);
+        const uint32_t h0[4] = {xh[0], yh[0], xh[1], yh[1]}, h1[4] = {xh[2], yh[2], xh[3], yh[3]};
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            mma16816(acc[n], a0, b[n].x, b[n].y);
-            mma16816(acc[n], a1, b[n].z, b[n].w);
+            mma16816(acc[n], h0, b[n].x, b[n].y);
+            mma16816(acc[n], h1, b[n].z, b[n].w);
         }
-        if constexpr (F == F_Q8_0 || F == F_Q4_0) {
-            // block MP is done: its fp16 scales in fp32 (blocks past the row's end hold other rows' bytes)
-            const float d0 = r0.d(), d1 = r1.d();
-            const bool in = MP < blocks;
+    } else {
+        r[0].template pair<MP>(x);
+        r[1].template pair<MP>(y);
+    }
+    const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if (in) {
-                    tot[n][0] = fmaf(xs[n] * d0, acc[n][0] + acc[n][1], tot[n][0]);
-                    tot[n][1] = fmaf(xs[n] * d1, acc[n][2] + acc[n][3], tot[n][1]);
-                }
-                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-            }
-        }
-        if constexpr (F == F_F8 && MP % 4 == 3) {
-            const bool in = MP / 4 < blocks;
-            const float d = in ? __ldg(wsc + MP / 4) : 0.0f;
+    for (int n = 0; n < NB; ++n) {
+        mma16816(acc[n], a0, b[n].x, b[n].y);
+        mma16816(acc[n], a1, b[n].z, b[n].w);
+    }
+}
+
+// Scales of a block of rows g and g + 8 where they are per block.
+template <int F>
+__device__ __forceinline__ float2 block_scales(const MoeRow<F> (&r)[2], const float* w) {
+    if constexpr (F == F_F8) {
+        const float d = __ldg(w);
+        return make_float2(d, d);
+    } else if constexpr (F == F_Q8_0 || F == F_Q4_0) {
+        return make_float2(r[0].d(), r[1].d());
+    } else {
+        return make_float2(0.0f, 0.0f);
+    }
+}
+
+// Lines of the activation record loaded ahead of their use, as far as the
+// format's registers allow; the first are loaded before the wait for the stage.
+template <int F, int NB>
+constexpr int kAhead = (F == F_F8 ? 4 : F == F_Q8_0 || F == F_Q4_0 ? 3 : 2) / NB;
+
+template <int F, int NB>
+struct ActLines {
+    uint4 b[NB][kAhead<F, NB> + 1];
+    template <int MP>
+    __device__ __forceinline__ void load(const uint8_t* const (&rec)[NB]) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if (in) {
-                    tot[n][0] = fmaf(xs[n] * d, acc[n][0] + acc[n][1], tot[n][0]);
-                    tot[n][1] = fmaf(xs[n] * d, acc[n][2] + acc[n][3], tot[n][1]);
+        for (int n = 0; n < NB; ++n)
+            b[n][MP % (kAhead<F, NB> + 1)] = __ldg(reinterpret_cast<const uint4*>(rec[n] + MP * 128));
+    }
+};
+
+// One CG of TL tiles (rows g and g + 8 of tile t at p[t][0], p[t][1]) times NB
+// blocks of four tokens: tot[t][n][r] += row r's product with token 4 n + i.
+// Tiles taken together share the loads of the activations, whose first kAhead
+// lines are in `x`.
+template <int F, int NB, int TL>
+__device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int i, const uint8_t* const (&rec)[NB],
+                                       ActLines<F, NB>& x, const float (&xs)[NB], int blocks, const float* const* wsc,
+                                       float (*tot)[NB][2]) {
+    MoeRow<F> r[TL][2];
+    float acc[TL][NB][4];
+#pragma unroll
+    for (int t = 0; t < TL; ++t) {
+        r[t][0].load(p[t][0], i);
+        r[t][1].load(p[t][1], i);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.0f;
+    }
+    each_pair([&](auto MPc) {
+        constexpr int MP = decltype(MPc)::value;
+        constexpr int D = kAhead<F, NB>;
+        if constexpr (MP + D < 8) x.template load<MP + D>(rec);
+        uint4 b[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) b[n] = x.b[n][MP % (D + 1)];
+#pragma unroll
+        for (int t = 0; t < TL; ++t) {
+            moe_pair<F, MP, NB>(r[t], b, acc[t]);
+            if constexpr (F == F_Q8_0 || F == F_Q4_0 || (F == F_F8 && MP % 4 == 3)) {
+                // a block is done: its scales in fp32 (blocks past the row's end hold other rows' bytes)
+                constexpr int B = F == F_F8 ? MP / 4 : MP;
+                if (B < blocks) {
+                    const float2 d = block_scales<F>(r[t], wsc[t] + B);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        tot[t][n][0] = fmaf(xs[n] * d.x, acc[t][n][0] + acc[t][n][1], tot[t][n][0]);
+                        tot[t][n][1] = fmaf(xs[n] * d.y, acc[t][n][2] + acc[t][n][3], tot[t][n][1]);
+                    }
                 }
-                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.0f;
             }
         }
     });
     if constexpr (Order<F>::SUMS > 0) {
-        uint32_t m0[2], m1[2];
-        r0.mins(m0);
-        r1.mins(m1);
-        const uint32_t a[4] = {m0[0], m1[0], m0[1], m1[1]};
-        const float d0 = r0.d(), d1 = r1.d(), q0 = r0.dm(), q1 = r1.dm();
+        uint2 b[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             // the line of this lane's column and part: sums are 8 bytes where codes are 16
-            const uint8_t* line = rec[n];
-            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(line)) & 127u;  // term * 64 + i * 16
-            const uint2 b = __ldg(reinterpret_cast<const uint2*>(line - off + kRecSums + off / 2));
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(c, a, b.x, b.y);
-            tot[n][0] = fmaf(xs[n], fmaf(d0, acc[n][0] + acc[n][1], -q0 * (c[0] + c[1])), tot[n][0]);
-            tot[n][1] = fmaf(xs[n], fmaf(d1, acc[n][2] + acc[n][3], -q1 * (c[2] + c[3])), tot[n][1]);
+            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(rec[n])) & 127u;  // term * 64 + i * 16
+            b[n] = __ldg(reinterpret_cast<const uint2*>(rec[n] - off + kRecSums + off / 2));
+        }
+#pragma unroll
+        for (int t = 0; t < TL; ++t) {
+            uint32_t m0[2], m1[2];
+            r[t][0].mins(m0);
+            r[t][1].mins(m1);
+            const uint32_t a[4] = {m0[0], m1[0], m0[1], m1[1]};
+            const float2 s0 = r[t][0].scales(), s1 = r[t][1].scales();
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma16816(c, a, b[n].x, b[n].y);
+                tot[t][n][0] = fmaf(xs[n], fmaf(s0.x, acc[t][n][0] + acc[t][n][1], -s0.y * (c[0] + c[1])), tot[t][n][0]);
+                tot[t][n][1] = fmaf(xs[n], fmaf(s1.x, acc[t][n][2] + acc[t][n][3], -s1.y * (c[2] + c[3])), tot[t][n][1]);
+            }
         }
     }
 }
+
+// Tiles of a unit that a stage holds and a warp takes at once: both where the
+// decoder's state of four rows fits the registers and two stages of them fit
+// half an SM's shared memory, else one after the other.
+template <int F, int NB>
+constexpr int kStageTiles = NB == 1 && (F == F_Q4_K || F == F_Q4_0) ? 2 : 1;
+// Rows whose packed length is a multiple of 16 start on one.
+template <int F>
+constexpr bool kAlignedRows = F == F_Q4_K || F == F_Q5_K || F == F_F8;
 
 // Bounded wait of a whole warp (see MoeBars::abort).
 __device__ __forceinline__ bool moe_wait(uint64_t* bar, uint32_t parity, MoeBars* b, int* err) {
@@ -381,10 +450,43 @@ __device__ __forceinline__ bool moe_wait(uint64_t* bar, uint32_t parity, MoeBars
     return ok;
 }
 
+// Row (of the expert) of tile `tile` and row r of unit `unit`.
+__device__ __forceinline__ int64_t stage_row(const ExpertArgs& a, int unit, int tile, int r) {
+    return a.gate_up ? static_cast<int64_t>(unit) * 16 + r : static_cast<int64_t>(unit) * 32 + 16 * tile + r;
+}
+
+// Joins the warps' partial sums (rb) of a round and writes its results.
+template <int kTok>
+__device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb, int64_t rd, int64_t per, int tid) {
+    const int grp = static_cast<int>(rd / per);
+    const int t0 = static_cast<int>(rd - grp * per) * a.slots;
+    const int4 gd = a.plan.groups[grp];
+    const int unit_rows = a.gate_up ? 16 : 32;
+    const int per_unit = kTok * unit_rows;
+    for (int o = tid; o < a.slots * per_unit; o += kConsumers * 32) {
+        const int un = o / per_unit, r = o - un * per_unit;
+        const int t = r / unit_rows, rr = r - t * unit_rows;
+        const int64_t row = static_cast<int64_t>(t0 + un) * unit_rows + rr;
+        if (t0 + un >= a.tiles || row >= a.rows || t >= gd.z) continue;
+        float v[2] = {0.0f, 0.0f};
+        for (int w = un * a.wps; w < (un + 1) * a.wps; ++w) {
+            if (a.gate_up) {
+                v[0] += rb[((w * 2) * kTok + t) * 16 + rr];
+                v[1] += rb[((w * 2 + 1) * kTok + t) * 16 + rr];
+            } else {
+                v[0] += rb[((w * 2 + (rr >> 4)) * kTok + t) * 16 + (rr & 15)];
+            }
+        }
+        const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
+        a.out[static_cast<int64_t>(a.plan.pairs[gd.y + t]) * a.rows + row] = z;
+    }
+}
+
 template <int F, int NB>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const ExpertArgs a) {
     constexpr int CGB = moe_cg_bytes<F>();
     constexpr int kTok = 4 * NB;
+    constexpr int TL = kStageTiles<F, NB>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127);
     float* red = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [2][warp][tile][token][16]
@@ -395,6 +497,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
             mbar_init(&bars.full[s], 1);
             mbar_init(&bars.empty[s], kConsumers);
         }
+        mbar_init(&bars.sums[0], kConsumers);
+        mbar_init(&bars.sums[1], kConsumers);
         bars.abort = 0;
         fence_mbar_init();
     }
@@ -417,25 +521,29 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
             const int grp = static_cast<int>(rd / per);
             const int t0 = static_cast<int>(rd - grp * per) * a.slots;
             const int64_t expert = a.plan.groups[grp].x;
-            for (int k = 0; k < ksteps; ++k) {
+            for (int step = 0; step < ksteps * (2 / TL); ++step) {
+                const int k = step / (2 / TL), tile = TL == 2 ? lane >> 4 : step & 1;
                 ok = moe_wait(&bars.empty[s], par ^ 1, &bars, a.err);
                 if (!ok) break;
                 uint8_t* st = ring + s * a.stage_bytes;
                 const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
                 const int64_t seg = min64(static_cast<int64_t>(a.wps) * CGB, a.row_bytes - off);
-                // lane: stage row `lane` of every slot; the bytes come from the 16-byte rounded range around the segment
+                // A stage holds 16 TL rows of every slot; lanes take them in turn.  The bytes come from the 16-byte
+                // rounded range around a row's segment.
+                const int srows = a.slots * 16 * TL;
+                const uint8_t* w = a.w[tile];
                 uint32_t tx = 0;
-                for (int u = 0; u < a.slots; ++u) {
-                    const int64_t row = a.gate_up ? static_cast<int64_t>(t0 + u) * 16 + (lane & 15)
-                                                  : static_cast<int64_t>(t0 + u) * 32 + lane;
+                for (int sr = lane; sr < srows; sr += 32) {
+                    const int u = sr / (16 * TL), r = sr - u * (16 * TL);
+                    const int64_t row = stage_row(a, t0 + u, TL == 2 ? r >> 4 : tile, r & 15);
                     if (t0 + u >= a.tiles || row >= a.rows) continue;
                     const int64_t at = (expert * a.rows + row) * a.rb + off;
                     const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
                     if (to <= a.w_bytes) {
                         tx += static_cast<uint32_t>(to - from);
                     } else {  // the rounded end would leave the buffer: bytes one by one
-                        const uint8_t* src = a.w[lane >> 4] + at;
-                        uint8_t* dst = st + (u * kTileRows + lane) * a.rs + (at & 15);
+                        const uint8_t* src = (TL == 2 ? a.w[r >> 4] : w) + at;
+                        uint8_t* dst = st + sr * a.rs + (at & 15);
                         for (int64_t c = 0; c < seg; ++c) dst[c] = src[c];
                     }
                 }
@@ -443,15 +551,15 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
                 __syncwarp();  // bytes copied by lanes come before the arrival
                 if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], tx);
                 __syncwarp();
-                for (int u = 0; u < a.slots; ++u) {
-                    const int64_t row = a.gate_up ? static_cast<int64_t>(t0 + u) * 16 + (lane & 15)
-                                                  : static_cast<int64_t>(t0 + u) * 32 + lane;
+                for (int sr = lane; sr < srows; sr += 32) {
+                    const int u = sr / (16 * TL), r = sr - u * (16 * TL);
+                    const int64_t row = stage_row(a, t0 + u, TL == 2 ? r >> 4 : tile, r & 15);
                     if (t0 + u >= a.tiles || row >= a.rows) continue;
                     const int64_t at = (expert * a.rows + row) * a.rb + off;
                     const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
                     if (to <= a.w_bytes)
-                        bulk_g2s_hint(st + (u * kTileRows + lane) * a.rs, a.w[lane >> 4] + from,
-                                      static_cast<uint32_t>(to - from), &bars.full[s], policy);
+                        bulk_g2s_hint(st + sr * a.rs, (TL == 2 ? a.w[r >> 4] : w) + from, static_cast<uint32_t>(to - from),
+                                      &bars.full[s], policy);
                 }
                 ++issued;
                 if (++s == a.stages) {
@@ -468,68 +576,87 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
 
     const int g = lane >> 2, i = lane & 3;
     const int u = warp / a.wps, col = warp - u * a.wps;
+    constexpr int kSums = kConsumers * 2 * kTok * 16;
     int s = 0;
     uint32_t par = 0;
     bool ok = true;
     for (int64_t rd = lo; rd < hi; ++rd) {
         const int grp = static_cast<int>(rd / per);
-        const int tile = static_cast<int>(rd - grp * per) * a.slots + u;
+        const int unit = static_cast<int>(rd - grp * per) * a.slots + u;
         const int4 gd = a.plan.groups[grp];  // expert, first entry of pairs, number of them
-        // this lane's B column: term g & 1 of token 4 n + g / 2 (past the group's end: its first)
-        const uint8_t* rec0[NB];
+        // this lane's B column: term g & 1 of token 4 n + g / 2 (past the group's end: its first), and the scale of
+        // its accumulator columns, those of token 4 n + i
+        const uint8_t *rec0[NB], *scale0[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const int t = 4 * n + (g >> 1);
-            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)];
+            const int t = 4 * n + (g >> 1), ts = 4 * n + i;
+            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)], ps = a.plan.pairs[gd.y + (ts < gd.z ? ts : 0)];
             rec0[n] = a.rec + p / a.rec_div * a.rec_row + (g & 1) * 64 + i * 16;
-        }
-        // the scale of this lane's accumulator columns: token 4 n + i
-        const uint8_t* scale0[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int t = 4 * n + i;
-            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)];
-            scale0[n] = a.rec + p / a.rec_div * a.rec_row + kRecScale;
+            scale0[n] = a.rec + ps / a.rec_div * a.rec_row + kRecScale;
         }
         float tot[2][NB][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < NB; ++n) tot[t][n][0] = tot[t][n][1] = 0.0f;
+        const int64_t row0 = gd.x * a.rows + stage_row(a, unit, 0, 0);
         for (int k = 0; k < ksteps; ++k) {
-            if (ok) ok = moe_wait(&bars.full[s], par, &bars, a.err);
             const int cg = k * a.wps + col;
-            if (ok && cg < a.ncg && tile < a.tiles) {
-                const uint8_t* rec[NB];
-                float xs[NB];
+            const bool mine = cg < a.ncg && unit < a.tiles;
+            const uint8_t* rec[NB];
+            float xs[NB];
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    rec[n] = rec0[n] + static_cast<int64_t>(cg) * kRec;
-                    xs[n] = __ldg(reinterpret_cast<const float*>(scale0[n] + static_cast<int64_t>(cg) * kRec));
-                }
-                const uint8_t* st = ring + s * a.stage_bytes + u * kTileRows * a.rs + col * CGB;
-                const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int64_t row = a.gate_up ? static_cast<int64_t>(tile) * 16 : static_cast<int64_t>(tile) * 32 + 16 * t;
-                    const int64_t at = (gd.x * a.rows + row + g) * a.rb + off;
-                    const uint8_t* p0 = st + (16 * t + g) * a.rs + (at & 15);
-                    const uint8_t* p1 = st + (16 * t + g + 8) * a.rs + ((at + 8 * a.rb) & 15);
-                    constexpr int kPerCg = F == F_F8 ? 2 : 8;
-                    const float* wsc = nullptr;
-                    if constexpr (F == F_F8) wsc = a.sc[t] + ((gd.x * a.rows + min64(row, a.rows - 1)) / 128) * a.nblk + 2 * cg;
-                    moe_cg<F, NB>(p0, p1, i, rec, xs, a.nblk - kPerCg * cg, wsc, tot[t]);
-                }
+            for (int n = 0; n < NB; ++n) {
+                const int64_t at = static_cast<int64_t>(mine ? cg : 0) * kRec;
+                rec[n] = rec0[n] + at;
+                xs[n] = __ldg(reinterpret_cast<const float*>(scale0[n] + at));
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.empty[s]);
-            if (++s == a.stages) {
-                s = 0;
-                par ^= 1;
+            // bytes of the first row's segment past a multiple of 16 (low bits suffice)
+            const uint32_t ph0 = kAlignedRows<F> ? 0u : static_cast<uint32_t>(row0) * static_cast<uint32_t>(a.rb) +
+                                                            static_cast<uint32_t>(k * a.wps) * CGB;
+            // e4m3: scales of the unit's rows (16 or 32 rows from a multiple of 16, so one block of 128)
+            const int64_t sc0 = F == F_F8 ? min64(row0, (gd.x + 1) * a.rows - 1) / 128 * a.nblk + 2 * cg : 0;
+            const int blocks = a.nblk - (F == F_F8 ? 2 : 8) * cg;
+#pragma unroll
+            for (int h = 0; h < 2 / TL; ++h) {
+                ActLines<F, NB> x;
+                static_for_pairs<kAhead<F, NB>>([&](auto J) { x.template load<decltype(J)::value>(rec); });
+                if (ok) ok = moe_wait(&bars.full[s], par, &bars, a.err);
+                if (ok && mine) {
+                    const uint8_t* st = ring + s * a.stage_bytes + u * (16 * TL) * a.rs + col * CGB;
+                    const uint8_t* p[TL][2];
+                    const float* wsc[TL];
+#pragma unroll
+                    for (int t = 0; t < TL; ++t) {
+                        const int tile = TL == 2 ? t : h;
+                        p[t][0] = st + (16 * t + g) * a.rs;
+                        p[t][1] = p[t][0] + 8 * a.rs;
+                        if constexpr (!kAlignedRows<F>) {
+                            // rows start where they do within their 16 bytes in memory
+                            const uint32_t ph = ph0 + (g + (a.gate_up ? 0 : 16 * tile)) * static_cast<uint32_t>(a.rb);
+                            p[t][0] += ph & 15u;
+                            p[t][1] += (ph + 8 * static_cast<uint32_t>(a.rb)) & 15u;
+                        }
+                        wsc[t] = F == F_F8 ? a.sc[tile] + sc0 : nullptr;
+                    }
+                    moe_cg<F, NB, TL>(p, i, rec, x, xs, blocks, wsc, tot + (TL == 2 ? 0 : h));
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.empty[s]);
+                if (++s == a.stages) {
+                    s = 0;
+                    par ^= 1;
+                }
             }
         }
-        // join the warps of each unit (two buffers: the next round's sums may be written while slow warps still read)
-        float* rb = red + ((rd - lo) & 1) * (kConsumers * 2 * kTok * 16);
+        // The round before is joined only now, when its slowest warp is long done.  Two buffers of sums are enough: a
+        // warp writes this round's after its share of the round before, so whoever waits for this round's sums knows
+        // that the other buffer has been read.
+        if (rd > lo) {
+            if (ok) ok = moe_wait(&bars.sums[(rd - 1 - lo) & 1], ((rd - 1 - lo) >> 1) & 1, &bars, a.err);
+            if (ok) moe_results<kTok>(a, red + ((rd - 1 - lo) & 1) * kSums, rd - 1, per, threadIdx.x);
+        }
+        float* rb = red + ((rd - lo) & 1) * kSums;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -538,27 +665,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
                 q[g] = tot[t][n][0];
                 q[g + 8] = tot[t][n][1];
             }
-        asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
-        const int per_unit = a.gate_up ? kTok * 16 : kTok * 32;
-        for (int o = threadIdx.x; o < a.slots * per_unit; o += kConsumers * 32) {
-            const int un = o / per_unit, r = o - un * per_unit;
-            const int tl = static_cast<int>(rd - grp * per) * a.slots + un;
-            // outputs of a unit: [token][row]
-            const int t = a.gate_up ? r >> 4 : r >> 5, rr = a.gate_up ? r & 15 : r & 31;
-            const int64_t row = static_cast<int64_t>(tl) * (a.gate_up ? 16 : 32) + rr;
-            if (tl >= a.tiles || row >= a.rows || t >= gd.z) continue;
-            float v[2] = {0.0f, 0.0f};
-            for (int w = un * a.wps; w < (un + 1) * a.wps; ++w) {
-                if (a.gate_up) {
-                    v[0] += rb[((w * 2) * kTok + t) * 16 + rr];
-                    v[1] += rb[((w * 2 + 1) * kTok + t) * 16 + rr];
-                } else {
-                    v[0] += rb[((w * 2 + (rr >> 4)) * kTok + t) * 16 + (rr & 15)];
-                }
-            }
-            const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
-            a.out[static_cast<int64_t>(a.plan.pairs[gd.y + t]) * a.rows + row] = z;
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.sums[(rd - lo) & 1]);
+    }
+    if (hi > lo) {
+        const int64_t last = hi - 1;
+        if (ok) ok = moe_wait(&bars.sums[(last - lo) & 1], ((last - lo) >> 1) & 1, &bars, a.err);
+        if (ok) moe_results<kTok>(a, red + ((last - lo) & 1) * kSums, last, per, threadIdx.x);
     }
 }
 
@@ -621,7 +734,7 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     const int cgs = std::min(a.wps, a.ncg);
     a.rs = (cgs * CGB + 15 + 4 + 15) / 16 * 16;
     while (a.rs % 128 != 16) a.rs += 16;
-    a.stage_bytes = a.slots * kTileRows * a.rs;
+    a.stage_bytes = a.slots * 16 * kStageTiles<F, NB> * a.rs;
     const int red = 2 * kConsumers * 2 * 4 * NB * 16 * 4;
     const int budget = 112 * 1024 - 512 - red;  // two CTAs per SM
     a.stages = std::min(kMoeStages, budget / a.stage_bytes);
@@ -699,10 +812,12 @@ cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* id
         const bool vec = hidden % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
                          reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
         const int64_t clusters = (tokens + kRouteTokens - 1) / kRouteTokens;
-        const size_t smem = static_cast<size_t>(kRouteTokens) * experts * 4;
+        int slices = 1;
+        while (2 * slices * experts <= kRouteCtas * kRouteWarps && hidden >= 256 * slices) slices *= 2;
+        const size_t smem = static_cast<size_t>(slices) * kRouteTokens * experts * 4;
         cudaError_t e = launch_pdl(moe_route_kernel<T>, dim3(static_cast<unsigned>(clusters * kRouteCtas)),
                                    dim3(32 * kRouteWarps), smem, s, static_cast<const T*>(x), w, ids, weights, tokens,
-                                   experts, top_k, hidden, normalize, vec);
+                                   experts, top_k, hidden, slices, normalize, vec);
         return e == cudaSuccess ? cudaGetLastError() : e;
     });
 }

@@ -68,19 +68,36 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// A small integer as an fp16 pair (v, v).
-__device__ __forceinline__ uint32_t h2_of(int v) {
-    const __half2 h = __half2half2(__int2half_rn(v));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// Two integers 0 .. 1023 in the halves of v, less K, as an fp16 pair.
+template <int K>
+__device__ __forceinline__ uint32_t ints_h2(uint32_t v) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v | 0x64006400u), "r"(h2_const(-1024.0f - K)));
+    return d;
 }
-__device__ __forceinline__ uint32_t h2_of2(int lo, int hi) {
-    const __half2 h = __halves2half2(__int2half_rn(lo), __int2half_rn(hi));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// (v.low, v.low) and (v.high, v.high)
+__device__ __forceinline__ uint32_t h2_low(uint32_t v) { return __byte_perm(v, 0u, 0x1010u); }
+__device__ __forceinline__ uint32_t h2_high(uint32_t v) { return __byte_perm(v, 0u, 0x3232u); }
+__host__ __device__ constexpr uint32_t h2_pow2(int lo, int hi) {  // (2^lo, 2^hi), exponents -14 .. 15
+    return static_cast<uint32_t>((lo + 15) << 10) | (static_cast<uint32_t>((hi + 15) << 10) << 16);
 }
-// (w & MASK) | OR in one LOP3.
+constexpr uint32_t kNeg2 = 0x80008000u;  // signs of both halves
+// (w & m) | o in one LOP3: two constants do not fit its immediate, and the
+// compiler splits the expression where it is not spelled out.
+__device__ __forceinline__ uint32_t lop_and_or(uint32_t w, uint32_t m, uint32_t o) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(m), "r"(o));
+    return d;
+}
 template <uint32_t MASK, uint32_t OR>
-__device__ __forceinline__ uint32_t and_or(uint32_t w) { return (w & MASK) | OR; }
-
+__device__ __forceinline__ uint32_t and_or(uint32_t w) { return lop_and_or(w, MASK, OR); }
+// Both halves of a block header (d, dmin), subnormals as zero (the formats'
+// definition), to fp32.
+__device__ __forceinline__ float2 h2_flush(uint32_t hd) {
+    uint32_t r;
+    asm("fma.rn.ftz.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(hd), "r"(0x3C003C00u), "r"(0x80008000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&r));
+}
 constexpr uint32_t kMagic = 0x64006400u;  // 1024 in both halves
 
 // Words at a 2-byte aligned shared address: the two aligned words around each.
@@ -99,8 +116,8 @@ __device__ __forceinline__ uint32_t ld_half2b(const uint8_t* p) { return *reinte
 
 // Row<F>: one row's part of one CG.  load(p, i) reads the header; pair<MP>(a)
 // gives the fragments of MMAs 2 MP (a[0], a[1]) and 2 MP + 1 (a[2], a[3]);
-// mins(a) those of the minimums' MMA (sub-block sums of x against them); d() and
-// dm() scale the sums of codes and of minimums.
+// mins(a) those of the minimums' MMA (sub-block sums of x against them);
+// scales() those of the sums of codes and of minimums.
 template <int F> struct MoeRow;
 
 // Q4_K {d, dmin, scales[12], qs[128]}: lane part i owns qs[32i ..], the
@@ -117,23 +134,19 @@ template <int F> struct MoeRowK45 {
         const uint4 v = *reinterpret_cast<const uint4*>(p);
         hd = v.x;
         // 6-bit scales and minimums j = 2i, 2i + 1 (get_scale_min_k4): bytes 0-3 hold scales 0-3, 4-7 minimums 0-3,
-        // 8-11 the low halves of both for 4-7, whose high two bits are the top bits of the first eight bytes
-        const int by = 16 * (i & 1);  // bit offset of bytes 2i & 3 ..
-        const uint32_t s0 = v.y >> by, m0 = v.z >> by, t0 = v.w >> by;
-        int sa, sb, ma, mb;
-        if (i < 2) {
-            sa = s0 & 63; sb = (s0 >> 8) & 63;
-            ma = m0 & 63; mb = (m0 >> 8) & 63;
-        } else {
-            sa = (t0 & 15) | ((s0 >> 2) & 0x30); sb = ((t0 >> 8) & 15) | ((s0 >> 10) & 0x30);
-            ma = ((t0 >> 4) & 15) | ((m0 >> 2) & 0x30); mb = ((t0 >> 12) & 15) | ((m0 >> 10) & 0x30);
-        }
-        scl = h2_of(sa);
-        cl = hmul2(scl, h2_const(-1024.0f));
-        const uint32_t s1 = h2_of(sb);
-        sch = hmul2(s1, h2_const(0.0625f));
-        ch = hmul2(s1, h2_const(-64.0f));
-        mn = h2_of2(ma, mb);
+        // 8-11 the low halves of both for 4-7, whose high two bits are the top bits of the first eight bytes.  The
+        // two bytes of this lane go to the halves of one register.
+        const uint32_t sel = (i & 1) ? 0x4342u : 0x4140u;
+        const uint32_t x = __byte_perm(v.y, 0u, sel), y = __byte_perm(v.z, 0u, sel), t = __byte_perm(v.w, 0u, sel);
+        const uint32_t sp = i < 2 ? x & 0x003F003Fu : (t & 0x000F000Fu) | ((x >> 2) & 0x00300030u);
+        const uint32_t mp = i < 2 ? y & 0x003F003Fu : ((t >> 4) & 0x000F000Fu) | ((y >> 2) & 0x00300030u);
+        mn = ints_h2<0>(mp);
+        const uint32_t s2 = hmul2(ints_h2<0>(sp), h2_pow2(0, -4));  // the high nibbles stay in place (x 16)
+        const uint32_t c2 = hmul2(s2, h2_pow2(10, 10) | kNeg2);
+        scl = h2_low(s2);
+        sch = h2_high(s2);
+        cl = h2_low(c2);
+        ch = h2_high(c2);
         q = p + (F == F_Q4_K ? 16 : 48) + 32 * i;
         qh = p + 16;
         sh = 2 * i;
@@ -153,10 +166,10 @@ template <int F> struct MoeRowK45 {
         uint32_t t2 = and_or<0x00F000F0u, kMagic>(x), t3 = and_or<0x00F000F0u, kMagic>(y);
         if constexpr (F == F_Q5_K) {
             const uint32_t b = h[MP % 4];
-            t0 |= (b << 4) & 0x00100010u;
-            t1 |= (b >> 4) & 0x00100010u;
-            t2 |= (b << 7) & 0x01000100u;
-            t3 |= (b >> 1) & 0x01000100u;
+            t0 = lop_and_or(b << 4, 0x00100010u, t0);
+            t1 = lop_and_or(b >> 4, 0x00100010u, t1);
+            t2 = lop_and_or(b << 7, 0x01000100u, t2);
+            t3 = lop_and_or(b >> 1, 0x01000100u, t3);
         }
         a[0] = hfma2(t0, scl, cl);
         a[1] = hfma2(t1, scl, cl);
@@ -164,8 +177,7 @@ template <int F> struct MoeRowK45 {
         a[3] = hfma2(t3, sch, ch);
     }
     __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn; a[1] = 0; }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd & 0xFFFFu); }
-    __device__ __forceinline__ float dm() const { return h2f_flush(hd >> 16); }
+    __device__ __forceinline__ float2 scales() const { return h2_flush(hd); }
 };
 template <> struct MoeRow<F_Q4_K> : MoeRowK45<F_Q4_K> {};
 template <> struct MoeRow<F_Q5_K> : MoeRowK45<F_Q5_K> {};
@@ -180,17 +192,14 @@ template <> struct MoeRow<F_Q2_K> {
         hd = *reinterpret_cast<const uint32_t*>(p);
         const uint32_t* s = reinterpret_cast<const uint32_t*>(p + 4 + 8 * (i >> 1));
         const int by = 8 * (i & 1);
-        const uint32_t a = s[0] >> by, b = s[1] >> by;  // bytes 2j + (i & 1) at bits 0, 16
-        const int v[4] = {static_cast<int>(a & 255), static_cast<int>((a >> 16) & 255), static_cast<int>(b & 255),
-                          static_cast<int>((b >> 16) & 255)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t x = h2_of(v[j] & 15);
-            sc[j] = j ? hmul2(x, h2_const(1.0f / static_cast<float>(1 << (2 * j)))) : x;
-            c[j] = hmul2(x, h2_const(-1024.0f / static_cast<float>(1 << (2 * j))));
-        }
-        mn[0] = h2_of2(v[0] >> 4, v[1] >> 4);
-        mn[1] = h2_of2(v[2] >> 4, v[3] >> 4);
+        const uint32_t a = s[0] >> by, b = s[1] >> by;  // bytes 2j + (i & 1) in the halves
+        const uint32_t s01 = hmul2(ints_h2<0>(a & 0x000F000Fu), h2_pow2(0, -2));
+        const uint32_t s23 = hmul2(ints_h2<0>(b & 0x000F000Fu), h2_pow2(-4, -6));
+        const uint32_t c01 = hmul2(s01, h2_pow2(10, 10) | kNeg2), c23 = hmul2(s23, h2_pow2(10, 10) | kNeg2);
+        sc[0] = h2_low(s01); sc[1] = h2_high(s01); sc[2] = h2_low(s23); sc[3] = h2_high(s23);
+        c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
+        mn[0] = ints_h2<0>((a >> 4) & 0x000F000Fu);
+        mn[1] = ints_h2<0>((b >> 4) & 0x000F000Fu);
         q = p + 20 + 16 * i;
         rot = i;
     }
@@ -206,8 +215,7 @@ template <> struct MoeRow<F_Q2_K> {
         a[3] = hfma2(and_or<m1, kMagic>(y), sc[j + 1], c[j + 1]);
     }
     __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd & 0xFFFFu); }
-    __device__ __forceinline__ float dm() const { return h2f_flush(hd >> 16); }
+    __device__ __forceinline__ float2 scales() const { return h2_flush(hd); }
 };
 
 // Q3_K {hmask[32], qs[64], scales[12], d}: the fields of Q2_K with a third bit,
@@ -222,19 +230,17 @@ template <> struct MoeRow<F_Q3_K> {
         // scale is = 8n + 2j + lh: low 4 bits in nibble n of byte 2j + lh of the first eight, high 2 bits at
         // 2 (is >> 2) of byte 8 + (is & 3)
         const int n = i >> 1, lh = i & 1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int by = 2 * j + lh;  // 0..7
-            const uint32_t lo = (s[j >> 1] >> (8 * (2 * (j & 1) + lh) + 4 * n)) & 15u;
-            const uint32_t hi = (s[2] >> (8 * (by & 3) + 2 * (2 * n + (j >> 1)))) & 3u;
-            const int v = static_cast<int>(lo | (hi << 4)) - 32;
-            const uint32_t x = h2_of(v);
-            sc[j] = j ? hmul2(x, h2_const(1.0f / static_cast<float>(1 << (2 * j)))) : x;
-            c[j] = hmul2(x, h2_const(-1024.0f / static_cast<float>(1 << (2 * j))));
-        }
-        const uint32_t lo16 = 0x5410u;
-        mn[0] = hmul2(__byte_perm(sc[0], sc[1], lo16), 0x4C004400u);  // 4 sc of fields 0 and 1 (field 1 is kept / 4)
-        mn[1] = hmul2(__byte_perm(sc[2], sc[3], lo16), 0x5C005400u);  // fields 2 and 3 (/ 16, / 64): x 64, x 256
+        const int by = 8 * lh + 4 * n;
+        const uint32_t hb = s[2] >> by;
+        const uint32_t v01 = ((s[0] >> by) & 0x000F000Fu) | ((hb << 4) & 0x00300030u);
+        const uint32_t v23 = ((s[1] >> by) & 0x000F000Fu) | ((hb << 2) & 0x00300030u);
+        const uint32_t x01 = ints_h2<32>(v01), x23 = ints_h2<32>(v23);
+        mn[0] = hmul2(x01, h2_pow2(2, 2));
+        mn[1] = hmul2(x23, h2_pow2(2, 2));
+        const uint32_t s01 = hmul2(x01, h2_pow2(0, -2)), s23 = hmul2(x23, h2_pow2(-4, -6));
+        const uint32_t c01 = hmul2(s01, h2_pow2(10, 10) | kNeg2), c23 = hmul2(s23, h2_pow2(10, 10) | kNeg2);
+        sc[0] = h2_low(s01); sc[1] = h2_high(s01); sc[2] = h2_low(s23); sc[3] = h2_high(s23);
+        c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
         ld_words2(p + 32 + 32 * n + 16 * lh, w);
         ld_words2(p + 16 * lh, h);
 #pragma unroll
@@ -246,14 +252,16 @@ template <> struct MoeRow<F_Q3_K> {
         constexpr uint32_t m0 = 0x00030003u << (2 * j), m1 = 0x00030003u << (2 * j + 2);
         constexpr uint32_t b0 = 0x00040004u << (2 * j), b1 = 0x00040004u << (2 * j + 2);
         const uint32_t x = w[MP / 2], y = x >> 8, b = h[MP / 2];
-        a[0] = hfma2(and_or<m0, kMagic>(x) | ((b << (j + 2)) & b0), sc[j], c[j]);
-        a[1] = hfma2(and_or<m0, kMagic>(y) | ((b >> (6 - j)) & b0), sc[j], c[j]);
-        a[2] = hfma2(and_or<m1, kMagic>(x) | ((b << (j + 3)) & b1), sc[j + 1], c[j + 1]);
-        a[3] = hfma2(and_or<m1, kMagic>(y) | ((b >> (5 - j)) & b1), sc[j + 1], c[j + 1]);
+        a[0] = hfma2(lop_and_or(b << (j + 2), b0, and_or<m0, kMagic>(x)), sc[j], c[j]);
+        a[1] = hfma2(lop_and_or(b >> (6 - j), b0, and_or<m0, kMagic>(y)), sc[j], c[j]);
+        a[2] = hfma2(lop_and_or(b << (j + 3), b1, and_or<m1, kMagic>(x)), sc[j + 1], c[j + 1]);
+        a[3] = hfma2(lop_and_or(b >> (5 - j), b1, and_or<m1, kMagic>(y)), sc[j + 1], c[j + 1]);
     }
     __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
-    __device__ __forceinline__ float dm() const { return h2f_flush(hd); }
+    __device__ __forceinline__ float2 scales() const {
+        const float d = h2_flush(hd).x;
+        return make_float2(d, d);
+    }
 };
 
 // Q6_K {ql[128], qh[64], scales[16], d}: field t of lane part i is sub-block
@@ -263,19 +271,18 @@ template <> struct MoeRow<F_Q3_K> {
 // low and on the high bits; 32 sc goes through the minimums'.  Scales are kept /
 // 4, so that 1024 * sc / 4 is finite.
 template <> struct MoeRow<F_Q6_K> {
-    uint32_t hd, sc[4], mn[2], lo[8], hi[4];
+    uint32_t hd, sc[4], c[4], mn[2], lo[8], hi[4];
     __device__ __forceinline__ void load(const uint8_t* p, int i) {
         const int n = i >> 1, lh = i & 1;
         hd = ld_half2b(p + 208);
         uint32_t s[2];
         ld_words2(p + 192 + 8 * n, s);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int v = static_cast<int8_t>(s[t >> 1] >> (8 * (2 * (t & 1) + lh)));
-            sc[t] = hmul2(h2_of(v), h2_const(0.25f));
-        }
-        mn[0] = __byte_perm(sc[0], sc[1], 0x5410u);
-        mn[1] = __byte_perm(sc[2], sc[3], 0x5410u);
+        const int by = 8 * lh;
+        mn[0] = hmul2(ints_h2<128>(((s[0] >> by) & 0x00FF00FFu) ^ 0x00800080u), h2_pow2(-2, -2));
+        mn[1] = hmul2(ints_h2<128>(((s[1] >> by) & 0x00FF00FFu) ^ 0x00800080u), h2_pow2(-2, -2));
+        const uint32_t c01 = hmul2(mn[0], h2_pow2(10, 10) | kNeg2), c23 = hmul2(mn[1], h2_pow2(10, 10) | kNeg2);
+        sc[0] = h2_low(mn[0]); sc[1] = h2_high(mn[0]); sc[2] = h2_low(mn[1]); sc[3] = h2_high(mn[1]);
+        c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
         uint32_t a[4], b[4];
         ld_words2(p + 64 * n + 16 * lh, a);
         ld_words2(p + 64 * n + 32 + 16 * lh, b);
@@ -290,34 +297,24 @@ template <> struct MoeRow<F_Q6_K> {
     template <int MP>
     __device__ __forceinline__ void pair(uint32_t (&a)[4], uint32_t (&b)[4]) {
         constexpr int t = 2 * (MP % 2), v = MP / 2;
-        const uint32_t m256 = h2_const(-1024.0f), m64 = h2_const(-64.0f), s16 = h2_const(0.0625f);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {  // fields t, t + 1: the nibble at bit 0 (t = 0) or 4 (t = 2) of lo[4f + v]
-            const uint32_t x = lo[4 * f + v], y = x >> 8;
-            const uint32_t s = sc[t + f];
-            if constexpr (t == 0) {
-                const uint32_t c = hmul2(s, m256);
-                a[2 * f] = hfma2(and_or<0x000F000Fu, kMagic>(x), s, c);
-                a[2 * f + 1] = hfma2(and_or<0x000F000Fu, kMagic>(y), s, c);
-            } else {
-                const uint32_t c = hmul2(s, m64), r = hmul2(s, s16);
-                a[2 * f] = hfma2(and_or<0x00F000F0u, kMagic>(x), r, c);
-                a[2 * f + 1] = hfma2(and_or<0x00F000F0u, kMagic>(y), r, c);
-            }
-            // 2 bits at 2 (t + f) of hi[v]: 16 * s * field; in place the field is x 4^(t + f)
-            const uint32_t z = hi[v], u = z >> 8;
-            constexpr float k0 = 16.0f / static_cast<float>(1 << (2 * t)), k1 = 4.0f / static_cast<float>(1 << (2 * t));
-            const uint32_t r = hmul2(s, f ? h2_const(k1) : h2_const(k0));
-            // (1024 + field * 4^n) * r - 1024 * r: 1024 * r <= 16 * 32 * 1024 would overflow for n = 0, so subtract first
-            const uint32_t one = h2_const(-1024.0f), unit = h2_const(1.0f);
-            const uint32_t mk = f ? 0x00030003u << (2 * t + 2) : 0x00030003u << (2 * t);
-            b[2 * f] = hmul2(hfma2((z & mk) | kMagic, unit, one), r);
-            b[2 * f + 1] = hmul2(hfma2((u & mk) | kMagic, unit, one), r);
+        for (int f = 0; f < 2; ++f) {
+            const uint32_t x = lo[4 * f + v], z = hi[v];
+            const uint32_t s = sc[t + f], k = c[t + f];
+            // the nibble at bit 0 (fields 0, 1) or 4 (fields 2, 3) of bytes 0, 2, then of bytes 1, 3
+            a[2 * f] = hfma2(and_or<0x000F000Fu, kMagic>(t ? x >> 4 : x), s, k);
+            a[2 * f + 1] = hfma2(and_or<0x000F000Fu, kMagic>(t ? x >> 12 : x >> 8), s, k);
+            // the 2 bits at 2 (t + f), moved to bits 4 and 5: 16 * field
+            const int up = 4 - 2 * (t + f);
+            b[2 * f] = hfma2(and_or<0x00300030u, kMagic>(up >= 0 ? z << up : z >> -up), s, k);
+            b[2 * f + 1] = hfma2(and_or<0x00300030u, kMagic>(z >> (8 - up)), s, k);
         }
     }
     __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd) * 4.0f; }
-    __device__ __forceinline__ float dm() const { return h2f_flush(hd) * 128.0f; }
+    __device__ __forceinline__ float2 scales() const {
+        const float d = h2_flush(hd).x;
+        return make_float2(d * 4.0f, d * 128.0f);
+    }
 };
 
 // Q8_0 {d, qs[32]} x 8 and Q4_0 {d, qs[16]} x 8: a block's d is fp16, so its
@@ -341,7 +338,7 @@ template <> struct MoeRow<F_Q8_0> {
             a[2 * k + 1] = hfma2(__byte_perm(u, 0x64646464u, 0x4342u), unit, off);
         }
     }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
+    __device__ __forceinline__ float d() const { return h2_flush(hd).x; }
 };
 template <> struct MoeRow<F_Q4_0> {
     const uint8_t* p;
@@ -360,7 +357,7 @@ template <> struct MoeRow<F_Q4_0> {
         a[2] = hfma2(and_or<0x00F000F0u, kMagic>(x), s, o1);
         a[3] = hfma2(and_or<0x00F000F0u, kMagic>(y), s, o1);
     }
-    __device__ __forceinline__ float d() const { return h2f_flush(hd); }
+    __device__ __forceinline__ float d() const { return h2_flush(hd).x; }
 };
 
 // e4m3: MMAs 0-7 are the first 128 columns, 8-15 the second; each half has one
