@@ -277,7 +277,7 @@ struct ExpertArgs {
     int rs, stage_bytes, stages;
     const uint8_t* rec;    // activation records
     int64_t rec_row;       // bytes of a record row
-    int rec_div;           // record row of pair p: p / rec_div
+    int rec_token;         // a pair's record row is its token's, else its own
     float* out;            // [pair][rows]
     MoePlan plan;
     int* err;
@@ -455,30 +455,41 @@ __device__ __forceinline__ int64_t stage_row(const ExpertArgs& a, int unit, int 
     return a.gate_up ? static_cast<int64_t>(unit) * 16 + r : static_cast<int64_t>(unit) * 32 + 16 * tile + r;
 }
 
+// A round: `slots` units of one group, from unit t0.  Rounds are walked in
+// order, so no division is needed after the first.
+struct MoeRound {
+    int grp, t0;
+    __device__ __forceinline__ void next(const ExpertArgs& a) {
+        t0 += a.slots;
+        if (t0 >= a.tiles) {
+            t0 = 0;
+            ++grp;
+        }
+    }
+};
+
 // Joins the warps' partial sums (rb) of a round and writes its results.
 template <int kTok>
-__device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb, int64_t rd, int64_t per, int tid) {
-    const int grp = static_cast<int>(rd / per);
-    const int t0 = static_cast<int>(rd - grp * per) * a.slots;
-    const int4 gd = a.plan.groups[grp];
-    const int unit_rows = a.gate_up ? 16 : 32;
-    const int per_unit = kTok * unit_rows;
-    for (int o = tid; o < a.slots * per_unit; o += kConsumers * 32) {
-        const int un = o / per_unit, r = o - un * per_unit;
-        const int t = r / unit_rows, rr = r - t * unit_rows;
-        const int64_t row = static_cast<int64_t>(t0 + un) * unit_rows + rr;
-        if (t0 + un >= a.tiles || row >= a.rows || t >= gd.z) continue;
+__device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb, const MoeRound& rd, int tid) {
+    const int4 gd = a.plan.groups[rd.grp];
+    const int rs = a.gate_up ? 4 : 5;  // log2 of a unit's rows
+    for (int o = tid; o < (a.slots * kTok) << rs; o += kConsumers * 32) {
+        const int rr = o & ((1 << rs) - 1), t = (o >> rs) & (kTok - 1), un = (o >> rs) / kTok;
+        const int64_t row = (static_cast<int64_t>(rd.t0 + un) << rs) + rr;
+        if (rd.t0 + un >= a.tiles || row >= a.rows || t >= gd.z) continue;
         float v[2] = {0.0f, 0.0f};
-        for (int w = un * a.wps; w < (un + 1) * a.wps; ++w) {
-            if (a.gate_up) {
-                v[0] += rb[((w * 2) * kTok + t) * 16 + rr];
-                v[1] += rb[((w * 2 + 1) * kTok + t) * 16 + rr];
-            } else {
-                v[0] += rb[((w * 2 + (rr >> 4)) * kTok + t) * 16 + (rr & 15)];
+        const float* q = rb + (un * a.wps * 2 * kTok + t) * 16;
+        if (a.gate_up) {
+            for (int w = 0; w < a.wps; ++w) {
+                v[0] += q[w * 2 * kTok * 16 + rr];
+                v[1] += q[(w * 2 + 1) * kTok * 16 + rr];
             }
+        } else {
+            q += (rr >> 4) * kTok * 16 + (rr & 15);
+            for (int w = 0; w < a.wps; ++w) v[0] += q[w * 2 * kTok * 16];
         }
         const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
-        a.out[static_cast<int64_t>(a.plan.pairs[gd.y + t]) * a.rows + row] = z;
+        a.out[static_cast<int64_t>(a.plan.entries[gd.y + t].x) * a.rows + row] = z;
     }
 }
 
@@ -506,9 +517,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
     pdl_wait();
     pdl_launch_dependents();
     const int ngroups = *a.plan.ngroups;
-    const int64_t per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group
-    const int64_t rounds = ngroups * per;
-    const int64_t lo = rounds * blockIdx.x / gridDim.x, hi = rounds * (blockIdx.x + 1) / gridDim.x;
+    const int per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group; all fit 32 bits (checked on the host)
+    const int rounds = ngroups * per;
+    const int lo = static_cast<int>(static_cast<int64_t>(rounds) * blockIdx.x / gridDim.x);
+    const int hi = static_cast<int>(static_cast<int64_t>(rounds) * (blockIdx.x + 1) / gridDim.x);
+    MoeRound rd{lo / per, 0};
+    rd.t0 = (lo - rd.grp * per) * a.slots;
     const int ksteps = (a.ncg + a.wps - 1) / a.wps;
 
     if (warp == kConsumers) {
@@ -517,10 +531,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
         uint32_t par = 0;
         bool ok = true;
         int64_t issued = 0;
-        for (int64_t rd = lo; rd < hi && ok; ++rd) {
-            const int grp = static_cast<int>(rd / per);
-            const int t0 = static_cast<int>(rd - grp * per) * a.slots;
-            const int64_t expert = a.plan.groups[grp].x;
+        for (int n = lo; n < hi && ok; ++n, rd.next(a)) {
+            const int t0 = rd.t0;
+            const int64_t expert = a.plan.groups[rd.grp].x;
             for (int step = 0; step < ksteps * (2 / TL); ++step) {
                 const int k = step / (2 / TL), tile = TL == 2 ? lane >> 4 : step & 1;
                 ok = moe_wait(&bars.empty[s], par ^ 1, &bars, a.err);
@@ -580,19 +593,19 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
     int s = 0;
     uint32_t par = 0;
     bool ok = true;
-    for (int64_t rd = lo; rd < hi; ++rd) {
-        const int grp = static_cast<int>(rd / per);
-        const int unit = static_cast<int>(rd - grp * per) * a.slots + u;
-        const int4 gd = a.plan.groups[grp];  // expert, first entry of pairs, number of them
+    MoeRound before{};
+    for (int q = 0; q < hi - lo; ++q) {
+        const int unit = rd.t0 + u;
+        const int4 gd = a.plan.groups[rd.grp];  // expert, first entry, number of entries
         // this lane's B column: term g & 1 of token 4 n + g / 2 (past the group's end: its first), and the scale of
         // its accumulator columns, those of token 4 n + i
         const uint8_t *rec0[NB], *scale0[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const int t = 4 * n + (g >> 1), ts = 4 * n + i;
-            const int p = a.plan.pairs[gd.y + (t < gd.z ? t : 0)], ps = a.plan.pairs[gd.y + (ts < gd.z ? ts : 0)];
-            rec0[n] = a.rec + p / a.rec_div * a.rec_row + (g & 1) * 64 + i * 16;
-            scale0[n] = a.rec + ps / a.rec_div * a.rec_row + kRecScale;
+            const int2 e = a.plan.entries[gd.y + (t < gd.z ? t : 0)], es = a.plan.entries[gd.y + (ts < gd.z ? ts : 0)];
+            rec0[n] = a.rec + (a.rec_token ? e.y : e.x) * a.rec_row + (g & 1) * 64 + i * 16;
+            scale0[n] = a.rec + (a.rec_token ? es.y : es.x) * a.rec_row + kRecScale;
         }
         float tot[2][NB][2];
 #pragma unroll
@@ -652,26 +665,28 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
         // The round before is joined only now, when its slowest warp is long done.  Two buffers of sums are enough: a
         // warp writes this round's after its share of the round before, so whoever waits for this round's sums knows
         // that the other buffer has been read.
-        if (rd > lo) {
-            if (ok) ok = moe_wait(&bars.sums[(rd - 1 - lo) & 1], ((rd - 1 - lo) >> 1) & 1, &bars, a.err);
-            if (ok) moe_results<kTok>(a, red + ((rd - 1 - lo) & 1) * kSums, rd - 1, per, threadIdx.x);
+        if (q > 0) {
+            if (ok) ok = moe_wait(&bars.sums[(q - 1) & 1], ((q - 1) >> 1) & 1, &bars, a.err);
+            if (ok) moe_results<kTok>(a, red + ((q - 1) & 1) * kSums, before, threadIdx.x);
         }
-        float* rb = red + ((rd - lo) & 1) * kSums;
+        before = rd;
+        rd.next(a);
+        float* rb = red + (q & 1) * kSums;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                float* q = rb + ((warp * 2 + t) * kTok + 4 * n + i) * 16;
-                q[g] = tot[t][n][0];
-                q[g + 8] = tot[t][n][1];
+                float* to = rb + ((warp * 2 + t) * kTok + 4 * n + i) * 16;
+                to[g] = tot[t][n][0];
+                to[g + 8] = tot[t][n][1];
             }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.sums[(rd - lo) & 1]);
+        if (lane == 0) mbar_arrive(&bars.sums[q & 1]);
     }
     if (hi > lo) {
-        const int64_t last = hi - 1;
-        if (ok) ok = moe_wait(&bars.sums[(last - lo) & 1], ((last - lo) >> 1) & 1, &bars, a.err);
-        if (ok) moe_results<kTok>(a, red + ((last - lo) & 1) * kSums, last, per, threadIdx.x);
+        const int q = hi - lo - 1;
+        if (ok) ok = moe_wait(&bars.sums[q & 1], (q >> 1) & 1, &bars, a.err);
+        if (ok) moe_results<kTok>(a, red + (q & 1) * kSums, before, threadIdx.x);
     }
 }
 
@@ -836,6 +851,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         plan.npairs = static_cast<int>(p);
         plan.experts = m.experts;
         plan.group = 4 * nb;
+        plan.top_k = m.top_k;
         plan.err = t0 == 0 ? err : nullptr;
         const MoePlan made = [&] {
             MoePlan q = plan;
@@ -862,7 +878,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.gate_up = 1;
         a.rec = base + w.rec_x;
         a.rec_row = (m.hidden + 255) / 256 * kRec;
-        a.rec_div = m.top_k;
+        a.rec_token = 1;
         a.out = h;
         a.plan = made;
         a.err = err;
@@ -877,7 +893,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.gate_up = 0;
         a.rec = base + w.rec_h;
         a.rec_row = (m.ffn + 255) / 256 * kRec;
-        a.rec_div = 1;
+        a.rec_token = 0;
         a.out = z;
         if (e = launch_experts(m.fmt_down, a, m.ffn, nb, s); e != cudaSuccess) return e;
         e = with_dtype(m.dtype, [&](auto* tag) {

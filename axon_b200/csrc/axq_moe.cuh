@@ -14,18 +14,19 @@ struct MoePlan {
     const int* ids;  // null once the plan is made
     int npairs, experts, group;
     int* ngroups;
-    int4* groups;    // expert, first entry of pairs, entries
-    int* pairs;
+    int4* groups;    // expert, first entry, number of entries
+    int2* entries;   // pair and its token, sorted by expert
+    int top_k;
     int* err;        // status word to clear, or null
 };
 
-constexpr size_t kMoePlanBytes = 256 + kMoePairs * 16 + kMoePairs * 4;
+constexpr size_t kMoePlanBytes = 256 + kMoePairs * 16 + kMoePairs * 8;
 
 inline MoePlan moe_plan_at(uint8_t* p) {
     MoePlan m{};
     m.ngroups = reinterpret_cast<int*>(p);
     m.groups = reinterpret_cast<int4*>(p + 256);
-    m.pairs = reinterpret_cast<int*>(p + 256 + kMoePairs * 16);
+    m.entries = reinterpret_cast<int2*>(p + 256 + kMoePairs * 16);
     return m;
 }
 
@@ -87,7 +88,7 @@ __device__ __forceinline__ void moe_make_plan(const MoePlan& m) {
         if (static_cast<unsigned>(e) >= static_cast<unsigned>(m.experts)) continue;
         int r = first[e];
         for (int q = 0; q < p; ++q) r += ids[q] == e ? 1 : 0;
-        m.pairs[r] = p;
+        m.entries[r] = make_int2(p, p / m.top_k);
     }
 }
 
