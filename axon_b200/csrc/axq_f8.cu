@@ -18,17 +18,6 @@
 namespace axq {
 namespace {
 
-// Elements c0 .. c0+7 of a row (zero past `cols`).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T* row, int64_t c0, int64_t cols, float (&v)[8]) {
-    if (VEC && c0 + 8 <= cols) {
-        load8(row + c0, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? Elem<T>::get(row[c0 + i]) : 0.0f;
-    }
-}
-
 // 1 x 128 blocks: 16 lanes hold a block, 8 elements each; a half warp takes
 // kUnroll blocks at once so that their loads are in flight together.
 constexpr int kPackUnroll = 4;
@@ -63,21 +52,11 @@ __global__ void __launch_bounds__(256) f8_pack_rows_kernel(const T* __restrict__
 #pragma unroll
         for (int u = 0; u < kPackUnroll; ++u) {
             const uint32_t it = it0 + u * halves;
-            float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[u][i]));
-#pragma unroll
-            for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+            uint32_t w[2];
+            const float s = pack_block16(v[u], w);
             if (it >= items) continue;
             const uint32_t r = it / static_cast<uint32_t>(nkb);
             const uint32_t kb = it - r * nkb;
-            const float s = __fdiv_rn(m, kF8Max);
-            const F8Div div(s);
-            uint32_t w[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                w[i] = cvt_e4m3x2(div(v[u][4 * i]), div(v[u][4 * i + 1])) |
-                       (cvt_e4m3x2(div(v[u][4 * i + 2]), div(v[u][4 * i + 3])) << 16);
             const int64_t c0 = static_cast<int64_t>(kb) * kF8Block + 8 * l;
             if (c0 < ld) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * ld + c0) = make_uint2(w[0], w[1]);
             if (l == 0) scales[it] = s;

@@ -92,4 +92,31 @@ struct F8Div {
     }
 };
 
+// Elements c0 .. c0+7 of a row of `cols` (zero past them).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T* row, int64_t c0, int64_t cols, float (&v)[8]) {
+    if (VEC && c0 + 8 <= cols) {
+        load8(row + c0, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? Elem<T>::get(row[c0 + i]) : 0.0f;
+    }
+}
+
+// A 1 x 128 block held by 16 lanes, 8 elements each (all 32 lanes of the warp
+// call it): its scale, and the lane's 8 codes.
+__device__ __forceinline__ float pack_block16(const float (&v)[8], uint32_t (&w)[2]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    const float s = __fdiv_rn(m, kF8Max);
+    const F8Div div(s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = cvt_e4m3x2(div(v[4 * i]), div(v[4 * i + 1])) | (cvt_e4m3x2(div(v[4 * i + 2]), div(v[4 * i + 3])) << 16);
+    return s;
+}
+
 }  // namespace axq

@@ -143,6 +143,10 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
         if (int r = check_device_ptr(x, "x", fn)) return r;
         if (reinterpret_cast<uintptr_t>(x) % host_dtype_size(x_dtype))
             return fail(AXQ_ERR_INVALID, std::string(fn) + ": x is not aligned to its element type");
+        if (f8_gemm_packs(M, K, N)) {
+            l.x = x;
+            return status(f8_gemm_unpacked_dispatch(l, x_dtype, s), fn);
+        }
         l.x_ld = ld_of(K);
         uint8_t* codes = ws + kStatusBytes;
         float* scales = reinterpret_cast<float*>(codes + up256(static_cast<size_t>(N) * l.x_ld));

@@ -20,6 +20,7 @@
 //    >= N tokens its N side, and a cluster splits K; its CTAs' sums are joined
 //    through distributed shared memory in rank order.  HBM-bound on W.
 #include <algorithm>
+#include <type_traits>
 #include <cuda.h>
 
 #include "axq_common.cuh"
@@ -43,6 +44,9 @@ struct F8Args {
     int nbuf;    // TMEM buffers
     int stages;
     int tiles_n, tiles_m;  // pair kernel: token tiles, weight-row tiles
+    const void* x;         // unpacked X (skinny kernel that packs it itself)
+    int64_t K;
+    int xvec;              // its rows start on 16-byte boundaries
     int* err;
 };
 
@@ -308,18 +312,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 constexpr int skinny_warps(int nt) { return nt > 64 ? 8 : 4; }
 
-template <int NT, typename TY>
+// TX: type of an X that the kernel packs itself (every CTA its K range of all
+// tokens, while the first weight tiles arrive); void: X is packed already.
+template <int NT, typename TY, typename TX>
 __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
     f8_skinny_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, F8Args a, int splits) {
     constexpr int kEpi = skinny_warps(NT);
     constexpr int kCols = NT / (kEpi / 4);
-    constexpr int kWBytes = 128 * 128, kXBytes = NT * 128, kStage = kWBytes + kXBytes;
+    constexpr bool kPack = !std::is_void_v<TX>;
+    constexpr int kWBytes = 128 * 128, kXBytes = NT * 128, kStage = kWBytes + (kPack ? 0 : kXBytes);
     constexpr int kBuf = 2;
     constexpr uint32_t kTmem = kBuf * NT <= 32 ? 32 : kBuf * NT;
     constexpr uint32_t kIdesc = idesc_e4m3_f32(NT, 128);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* stage0 = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    float* sxs = reinterpret_cast<float*>(stage0 + a.stages * kStage);  // [kb][NT] scales of X
+    uint8_t* xs = stage0 + a.stages * kStage;  // the packed X of every K block, if the kernel packs it
+    const int most = (a.nkb + splits - 1) / splits;
+    float* sxs = reinterpret_cast<float*>(xs + (kPack ? most * kXBytes : 0));  // [kb][NT] scales of X
     float* red = reinterpret_cast<float*>(stage0);                      // [NT][128] sums, after the last MMA
     __shared__ F8Bars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -346,8 +355,9 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
     if (warp == 0) {
         // The packing of X, launched before this kernel, let it start only
         // after everything before the packing had finished, so W is there; X
-        // is waited for.
+        // is waited for.  Without a packing kernel W is waited for too.
         const int first = min(nk, a.stages);
+        if (kPack) pdl_wait();
         if (elect_one()) {
             for (int i = 0; i < first; ++i) {
                 mbar_arrive_expect_tx(&bars.full[i], kStage);
@@ -355,12 +365,14 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
             }
         }
         __syncwarp();
-        pdl_wait();
-        if (elect_one()) {
-            for (int i = 0; i < first; ++i)
-                tma_load_2d(stage0 + i * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[i]);
+        if constexpr (!kPack) {
+            pdl_wait();
+            if (elect_one()) {
+                for (int i = 0; i < first; ++i)
+                    tma_load_2d(stage0 + i * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[i]);
+            }
+            __syncwarp();
         }
-        __syncwarp();
         int s = 0;
         uint32_t par = 0;
         bool ok = true;
@@ -371,7 +383,8 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
             if (elect_one()) {
                 mbar_arrive_expect_tx(&bars.full[s], kStage);
                 tma_load_2d(stage0 + s * kStage, &mw, (kb0 + i) * 128, mt * 128, &bars.full[s]);
-                tma_load_2d(stage0 + s * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[s]);
+                if constexpr (!kPack)
+                    tma_load_2d(stage0 + s * kStage + kWBytes, &mx, (kb0 + i) * 128, 0, &bars.full[s]);
             }
             __syncwarp();
             ++issued;
@@ -387,15 +400,19 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
     } else if (warp == 1) {
         int s = 0, b = 0;
         uint32_t par = 0, bpar = 0;
+        if constexpr (kPack) {
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * kEpi + 32) : "memory");  // X is packed
+            tc_fence_after();
+        }
         for (int i = 0; i < nk; ++i) {
             if (!f8_wait(&bars.acc_empty[b], bpar ^ 1, &bars, a.err) || !f8_wait(&bars.full[s], par, &bars, a.err)) break;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t ws = smem_u32(stage0 + s * kStage);
+                const uint32_t xa = kPack ? smem_u32(xs + i * kXBytes) : ws + kWBytes;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    mma_e4m3<1>(tmem + b * NT, smem_desc_sw128(ws + 32 * k), smem_desc_sw128(ws + kWBytes + 32 * k), kIdesc,
-                                k > 0);
+                    mma_e4m3<1>(tmem + b * NT, smem_desc_sw128(ws + 32 * k), smem_desc_sw128(xa + 32 * k), kIdesc, k > 0);
                 mma_commit(&bars.done[s]);
             }
             __syncwarp();
@@ -412,9 +429,54 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
         const int q = warp & 3, g = (warp - 2) >> 2;
         const int et = threadIdx.x - 64;
         pdl_wait();
-        for (int i = et; i < nk * NT; i += 32 * kEpi) {
-            const int n = i / nk, k = i - n * nk;
-            sxs[k * NT + n] = n < a.N ? __ldg(a.sx + static_cast<int64_t>(n) * a.nkb + kb0 + k) : 0.0f;
+        if constexpr (kPack) {
+            // A wait that gives up does so after two seconds: long after this.
+            if (a.err && blockIdx.x == 0 && et == 0) *a.err = 0;
+            // 16 lanes to a block of 128; rows past N keep what the memory holds: their columns are never read
+            const TX* x = static_cast<const TX*>(a.x);
+            const int l = lane & 15;
+            constexpr int U = 4;  // blocks whose loads are in flight together
+            const int items = nk * static_cast<int>(a.N);
+            for (int i0 = (et >> 5) * 2; i0 < items; i0 += 2 * kEpi * U) {
+                float v[U][8];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i0 + u * 2 * kEpi >= items) break;
+                    const int i = i0 + u * 2 * kEpi + (lane >> 4), n = i / nk;
+                    const int64_t c0 = static_cast<int64_t>(kb0 + i - n * nk) * kF8Block + 8 * l;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+                    if (n < a.N) {
+                        if (a.xvec)
+                            load_row8<TX, true>(x + n * a.K, c0, a.K, v[u]);
+                        else
+                            load_row8<TX, false>(x + n * a.K, c0, a.K, v[u]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (i0 + u * 2 * kEpi >= items) break;
+                    const int i = i0 + u * 2 * kEpi + (lane >> 4), n = i / nk, k = i - n * nk;
+                    uint32_t w[2];
+                    const float sc = pack_block16(v[u], w);
+                    if (n < a.N) {
+                        // the 128-byte swizzle: 16-byte chunk c of row n is at chunk c ^ (n % 8)
+                        *reinterpret_cast<uint2*>(xs + k * kXBytes + n * 128 + (((l >> 1) ^ (n & 7)) << 4) + (l & 1) * 8) =
+                            make_uint2(w[0], w[1]);
+                        if (l == 0) sxs[k * NT + n] = sc;
+                    }
+                }
+            }
+            for (int i = et; i < nk * NT; i += 32 * kEpi)
+                if (i % NT >= a.N) sxs[i] = 0.0f;
+            fence_proxy_async_smem();
+            tc_fence_before();
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * kEpi + 32) : "memory");
+        } else {
+            for (int i = et; i < nk * NT; i += 32 * kEpi) {
+                const int n = i / nk, k = i - n * nk;
+                sxs[k * NT + n] = n < a.N ? __ldg(a.sx + static_cast<int64_t>(n) * a.nkb + kb0 + k) : 0.0f;
+            }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
         float acc[kCols];
@@ -561,33 +623,51 @@ cudaError_t launch_pair(const F8Linear& l, F8Args a, cudaStream_t s) {
     return launch_cluster(f8_pair_kernel<BN, TY>, 2 * pairs, kPairThreads, 0, smem, s, mx, mw, a);
 }
 
-template <int NT, typename TY>
-cudaError_t launch_skinny(const F8Linear& l, F8Args a, cudaStream_t s) {
-    constexpr int kStage = 128 * 128 + NT * 128;
-    CUtensorMap mx, mw;
-    if (cudaError_t e = byte_map(&mx, l.x, l.N, l.K, l.x_ld, NT); e != cudaSuccess) return e;
-    if (cudaError_t e = byte_map(&mw, l.w, l.M, l.K, l.w_ld, 128); e != cudaSuccess) return e;
-    const int tiles = static_cast<int>((l.M + 127) / 128);
+// Clusters of the skinny kernel: CTAs that split K so that about two per SM are
+// at work, each with at least two blocks.
+int skinny_splits(int64_t M, int nkb) {
+    const int64_t tiles = (M + 127) / 128;
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count() && splits * 4 <= a.nkb) splits *= 2;
-    const int per = (a.nkb + splits - 1) / splits;  // blocks of K of one CTA
-    // two CTAs per SM, unless the scales of X take the room
-    const int scales = (per * NT * 4 + 127) / 128 * 128;
-    int budget = 110 * 1024 - 1024 - scales;
-    if (budget < 3 * kStage) budget = 224 * 1024 - 1024 - scales;
-    a.stages = std::min({kMaxF8Stages, std::max(std::max(per, 2), NT * 512 / kStage + 1), budget / kStage});
-    if (a.stages < 2) return launch_pair<128, TY>(l, a, s);  // K so long that the scales of X fill shared memory
-    a.stages = std::max(a.stages, (NT * 512 + kStage - 1) / kStage);  // the sums need NT x 128 floats
-    const int smem = a.stages * kStage + scales + 1024;
-    static std::atomic<int> cfg[64];
-    if (cudaError_t e = ensure_dyn_smem(f8_skinny_kernel<NT, TY>, smem, cfg); e != cudaSuccess) return e;
-    return launch_cluster(f8_skinny_kernel<NT, TY>, tiles * splits, 64 + 32 * skinny_warps(NT), splits, smem, s, mx, mw, a,
-                          splits);
+    while (splits < 8 && tiles * splits * 2 <= 2 * device_sm_count() && splits * 4 <= nkb) splits *= 2;
+    return splits;
 }
 
-}  // namespace
+template <int NT, typename TY, typename TX>
+cudaError_t launch_skinny(const F8Linear& l, F8Args a, cudaStream_t s) {
+    constexpr bool kPack = !std::is_void_v<TX>;
+    constexpr int kStage = 128 * 128 + (kPack ? 0 : NT * 128);
+    CUtensorMap mx, mw;
+    if (cudaError_t e = byte_map(&mw, l.w, l.M, l.K, l.w_ld, 128); e != cudaSuccess) return e;
+    if constexpr (kPack) {
+        mx = mw;  // unused
+        a.x = l.x;
+        a.K = l.K;
+        a.xvec = reinterpret_cast<uintptr_t>(l.x) % 16 == 0 && l.K * sizeof(TX) % 16 == 0;
+    } else {
+        if (cudaError_t e = byte_map(&mx, l.x, l.N, l.K, l.x_ld, NT); e != cudaSuccess) return e;
+    }
+    const int64_t tiles = (l.M + 127) / 128;
+    const int splits = skinny_splits(l.M, a.nkb);
+    const int per = (a.nkb + splits - 1) / splits;  // blocks of K of one CTA
+    // two CTAs per SM, unless the scales of X take the room
+    const int64_t own = (static_cast<int64_t>(per) * (NT * 4 + (kPack ? NT * 128 : 0)) + 127) / 128 * 128;
+    int64_t budget = 110 * 1024 - 1024 - own;
+    if (budget < 3 * kStage) budget = 224 * 1024 - 1024 - own;
+    const int sums = (NT * 512 + kStage - 1) / kStage;  // stages that the sums take: NT x 128 floats
+    const int64_t fit = budget < 0 ? 0 : budget / kStage;
+    if (fit < std::max(2, sums)) {  // K so long that the scales of X fill shared memory
+        if constexpr (kPack) return cudaErrorInvalidConfiguration;
+        else return launch_pair<128, TY>(l, a, s);
+    }
+    a.stages = static_cast<int>(std::min<int64_t>({int64_t(kMaxF8Stages), int64_t(std::max({per, 2, sums})), fit}));
+    const int smem = static_cast<int>(a.stages * kStage + own + 1024);
+    static std::atomic<int> cfg[64];
+    if (cudaError_t e = ensure_dyn_smem(f8_skinny_kernel<NT, TY, TX>, smem, cfg); e != cudaSuccess) return e;
+    return launch_cluster(f8_skinny_kernel<NT, TY, TX>, static_cast<int>(tiles * splits), 64 + 32 * skinny_warps(NT), splits,
+                          smem, s, mx, mw, a, splits);
+}
 
-cudaError_t f8_gemm_dispatch(const F8Linear& l, cudaStream_t s) {
+F8Args args_of(const F8Linear& l) {
     F8Args a{};
     a.sx = l.x_scales;
     a.sw = l.w_scales;
@@ -597,12 +677,39 @@ cudaError_t f8_gemm_dispatch(const F8Linear& l, cudaStream_t s) {
     a.N = l.N;
     a.nkb = static_cast<int>((l.K + kF8Block - 1) / kF8Block);
     a.err = l.err;
+    return a;
+}
+
+}  // namespace
+
+// Few tokens whose K range of a CTA is at most 32 blocks: one round of loads,
+// which cost less than a packing kernel (4096 x 4096: 6.6 against 8.4 us for one
+// token); more rounds cost more (11008 x 4096, 16 tokens: 35 against 16 us).
+bool f8_gemm_packs(int64_t M, int64_t K, int64_t N) {
+    const int nkb = static_cast<int>((K + kF8Block - 1) / kF8Block);
+    const int splits = skinny_splits(M, nkb);
+    return N <= 16 && N * ((nkb + splits - 1) / splits) <= 32;
+}
+
+cudaError_t f8_gemm_unpacked_dispatch(const F8Linear& l, int x_dtype, cudaStream_t s) {
+    const F8Args a = args_of(l);
+    return with_dtype(x_dtype, [&](auto* xt) {
+        using TX = std::remove_pointer_t<decltype(xt)>;
+        return with_dtype(l.y_dtype, [&](auto* yt) {
+            using TY = std::remove_pointer_t<decltype(yt)>;
+            return launch_skinny<16, TY, TX>(l, a, s);
+        });
+    });
+}
+
+cudaError_t f8_gemm_dispatch(const F8Linear& l, cudaStream_t s) {
+    const F8Args a = args_of(l);
     return with_dtype(l.y_dtype, [&](auto* tag) {
         using TY = std::remove_pointer_t<decltype(tag)>;
-        if (l.N <= 16) return launch_skinny<16, TY>(l, a, s);
-        if (l.N <= 32) return launch_skinny<32, TY>(l, a, s);
-        if (l.N <= 64) return launch_skinny<64, TY>(l, a, s);
-        if (l.N <= 128) return launch_skinny<128, TY>(l, a, s);
+        if (l.N <= 16) return launch_skinny<16, TY, void>(l, a, s);
+        if (l.N <= 32) return launch_skinny<32, TY, void>(l, a, s);
+        if (l.N <= 64) return launch_skinny<64, TY, void>(l, a, s);
+        if (l.N <= 128) return launch_skinny<128, TY, void>(l, a, s);
         const int64_t wide = (l.N + 255) / 256 * ((l.M + 255) / 256);
         return wide * 2 >= device_sm_count() ? launch_pair<256, TY>(l, a, s) : launch_pair<128, TY>(l, a, s);
     });

@@ -88,6 +88,10 @@ struct F8Linear {
     int* err;
 };
 cudaError_t f8_gemm_dispatch(const F8Linear& a, cudaStream_t s);
+// Whether the product packs an X of this size itself: x then is the unpacked X
+// (row-major, x_dtype) and err is set to 0.
+bool f8_gemm_packs(int64_t M, int64_t K, int64_t N);
+cudaError_t f8_gemm_unpacked_dispatch(const F8Linear& a, int x_dtype, cudaStream_t s);
 
 // Mixture-of-experts layer (axq_moe.cu).
 struct MoeMlp {

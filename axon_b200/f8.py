@@ -16,9 +16,13 @@ from typing import Optional, Tuple
 import torch
 
 from ._capi import DType, F8_BLOCK, AxqError, Status, check, lib
-from .ops import _req_cuda, _stream_handle
+from .ops import _req_cuda
 
-FLOAT_TYPES = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.BF16}
+# element types as C ABI ids (plain ints: these run on every call)
+FLOAT_TYPES = {torch.float32: int(DType.F32), torch.float16: int(DType.F16), torch.bfloat16: int(DType.BF16)}
+_E4M3 = torch.float8_e4m3fn
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _up(n: int, m: int) -> int:
@@ -29,39 +33,48 @@ def _invalid(msg: str) -> AxqError:
     return AxqError(Status.ERR_INVALID, msg)
 
 
-def _float_type(t, name: str) -> DType:
-    """The element type of a contiguous CUDA float tensor."""
-    if not isinstance(t, torch.Tensor):
-        raise _invalid(f"{name} must be a torch.Tensor")
-    if t.dtype not in FLOAT_TYPES:
-        raise _invalid(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
-    _req_cuda(t, name, t.dtype)
-    return FLOAT_TYPES[t.dtype]
+def _float_type(t, name: str) -> int:
+    """The element type id of a contiguous CUDA float tensor."""
+    if isinstance(t, torch.Tensor):
+        dtype = FLOAT_TYPES.get(t.dtype)
+        if dtype is not None and t.is_cuda and t.is_contiguous():
+            return dtype
+        if dtype is None:
+            raise _invalid(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
+        _req_cuda(t, name, t.dtype)  # says what is wrong
+    raise _invalid(f"{name} must be a torch.Tensor")
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
+def _plain(t, name: str, dtype: torch.dtype) -> None:
+    """A contiguous CUDA tensor of this type."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.is_contiguous()):
+        _req_cuda(t, name, dtype)
+
+
+def _same_device(device: torch.device, names, *tensors) -> None:
+    for k, t in enumerate(tensors):
         if t is not None and t.device != device:
-            raise _invalid(f"{name} is on {t.device}, not on {device}")
+            raise _invalid(f"{names[k]} is on {t.device}, not on {device}")
 
 
-@contextlib.contextmanager
 def _on(device: torch.device, stream: Optional[torch.cuda.Stream]):
-    """The call's device and stream made current, so that what it allocates
-    belongs to that stream."""
-    with torch.cuda.device(device):
-        if stream is None:
-            yield
-        else:
-            with torch.cuda.stream(stream):
-                yield
+    """None where the call's device is current and it goes to the current
+    stream; else a context that makes both so (what the call allocates then
+    belongs to its stream)."""
+    if stream is None:
+        return None if device.index == _current_device() else torch.cuda.device(device)
+    both = contextlib.ExitStack()
+    both.enter_context(torch.cuda.device(device))
+    both.enter_context(torch.cuda.stream(stream))
+    return both
 
 
-def _scratch(nbytes: int, device: torch.device) -> Tuple[torch.Tensor, int, int]:
-    """(tensor, 256-byte aligned address, bytes from there)."""
-    buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
-    off = -buf.data_ptr() % 256
-    return buf, buf.data_ptr() + off, nbytes + 256 - off
+def _scratch(nbytes: int, like: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """(tensor on `like`'s device, 256-byte aligned address, bytes from there)."""
+    buf = like.new_empty(nbytes + 256, dtype=torch.uint8)
+    p = buf.data_ptr()
+    off = -p % 256
+    return buf, p + off, nbytes + 256 - off
 
 
 @dataclass
@@ -85,17 +98,19 @@ class F8Tensor:
 
     def _check(self, name: str) -> None:
         rows, cols = self.shape
-        if self.block_rows not in (1, F8_BLOCK):
+        d, s, br = self.data, self.scales, self.block_rows
+        if br != 1 and br != F8_BLOCK:
             raise _invalid(f"{name}: block_rows must be 1 or 128")
-        _req_cuda(self.data, f"{name}.data", torch.float8_e4m3fn)
-        _req_cuda(self.scales, f"{name}.scales", torch.float32)
-        if self.data.dim() != 2 or self.data.shape[0] != rows or self.data.shape[1] < cols or self.data.shape[1] % 16:
+        _plain(d, f"{name}.data", _E4M3)
+        _plain(s, f"{name}.scales", torch.float32)
+        if d.dim() != 2 or d.shape[0] != rows or d.shape[1] < cols or d.shape[1] % 16:
             raise _invalid(f"{name}: codes of a [{rows} x {cols}] matrix must be [{rows} x ld], ld a multiple of 16 of at "
-                           f"least {cols} (got {tuple(self.data.shape)})")
-        want = (_up(rows, self.block_rows), _up(cols, F8_BLOCK))
-        if tuple(self.scales.shape) != want:
-            raise _invalid(f"{name}: scales must be {want} (got {tuple(self.scales.shape)})")
-        _same_device(self.data.device, **{f"{name}.scales": self.scales})
+                           f"least {cols} (got {tuple(d.shape)})")
+        want = (_up(rows, br), _up(cols, F8_BLOCK))
+        if s.shape != want:
+            raise _invalid(f"{name}: scales must be {want} (got {tuple(s.shape)})")
+        if s.device != d.device:
+            raise _invalid(f"{name}.scales is on {s.device}, not on {d.device}")
 
 
 def quantize_f8(dst: F8Tensor, src: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> F8Tensor:
@@ -106,28 +121,35 @@ def quantize_f8(dst: F8Tensor, src: torch.Tensor, stream: Optional[torch.cuda.St
     if src.dim() != 2:
         raise _invalid("quantize_f8: src must be 2-D")
     dst._check("dst")
-    if tuple(src.shape) != tuple(dst.shape):
+    if src.shape != tuple(dst.shape):
         raise _invalid(f"quantize_f8: src is {tuple(src.shape)}, dst {tuple(dst.shape)}")
-    _same_device(src.device, dst=dst.data)
+    device = src.device
+    _same_device(device, ("dst",), dst.data)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return quantize_f8(dst, src)
     rows, cols = src.shape
-    with _on(src.device, stream):
-        check(lib().axq_quantize_f8(int(dtype), src.data_ptr(), dst.data.data_ptr(), dst.data.shape[1],
-                                    dst.scales.data_ptr(), rows, cols, dst.block_rows,
-                                    _stream_handle(stream, src.device)))
+    check(lib().axq_quantize_f8(dtype, src.data_ptr(), dst.data.data_ptr(), dst.data.shape[1], dst.scales.data_ptr(), rows,
+                                cols, dst.block_rows, _raw_stream(device.index)))
     return dst
 
 
 def dequantize_f8(dst: torch.Tensor, src: F8Tensor, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Decode ``src`` into ``dst`` (fp32, [rows, cols])."""
     src._check("src")
-    _req_cuda(dst, "dst", torch.float32)
-    if tuple(dst.shape) != tuple(src.shape):
+    _plain(dst, "dst", torch.float32)
+    if dst.shape != tuple(src.shape):
         raise _invalid(f"dequantize_f8: dst is {tuple(dst.shape)}, src {tuple(src.shape)}")
-    _same_device(dst.device, src=src.data)
+    device = dst.device
+    _same_device(device, ("src",), src.data)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return dequantize_f8(dst, src)
     rows, cols = src.shape
-    with _on(dst.device, stream):
-        check(lib().axq_dequantize_f8(src.data.data_ptr(), src.data.shape[1], src.scales.data_ptr(), src.block_rows,
-                                      dst.data_ptr(), rows, cols, _stream_handle(stream, dst.device)))
+    check(lib().axq_dequantize_f8(src.data.data_ptr(), src.data.shape[1], src.scales.data_ptr(), src.block_rows,
+                                  dst.data_ptr(), rows, cols, _raw_stream(device.index)))
     return dst
 
 
@@ -142,35 +164,41 @@ def linear_f8(x, w: F8Tensor, out: Optional[torch.Tensor] = None, bias: Optional
     if w.block_rows != F8_BLOCK:
         raise _invalid("linear_f8: w must be packed in 128 x 128 blocks")
     M, K = w.shape
-    packed = isinstance(x, F8Tensor)
-    if packed:
+    if isinstance(x, F8Tensor):
         x._check("x")
         if x.block_rows != 1:
             raise _invalid("linear_f8: x must be packed in 1 x 128 blocks")
-        xd, x_type, x_ld, x_scales, y_type = x.data, DType.F8, x.data.shape[1], x.scales, torch.float32
+        xd, x_type, x_ld, x_scales, y_type = x.data, int(DType.F8), x.data.shape[1], x.scales.data_ptr(), torch.float32
     else:
         x_type = _float_type(x, "x")
         xd, x_ld, x_scales, y_type = x, K, None, x.dtype
         if x.dim() != 2:
             raise _invalid("linear_f8: x must be 2-D")
-    if x.shape[1] != K:
+    N, xk = x.shape
+    if xk != K:
         raise _invalid(f"linear_f8: x must be [N x {K}]")
-    N, device = x.shape[0], xd.device
+    device = xd.device
+    bias_ptr = None
     if bias is not None:
-        _req_cuda(bias, "bias", torch.float32)
+        _plain(bias, "bias", torch.float32)
         if bias.numel() != M:
             raise _invalid(f"linear_f8: bias must have {M} elements")
-    _same_device(device, w=w.data, bias=bias, out=out)
-    with _on(device, stream):
-        if out is None:
-            out = torch.empty((N, M), dtype=y_type, device=device)
+        bias_ptr = bias.data_ptr()
+    _same_device(device, ("w", "bias", "out"), w.data, bias, out)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return linear_f8(x, w, out, bias)
+    if out is None:
+        out = xd.new_empty((N, M), dtype=y_type)
+        out_type = FLOAT_TYPES[y_type]
+    else:
         out_type = _float_type(out, "out")
-        if tuple(out.shape) != (N, M):
+        if out.shape != (N, M):
             raise _invalid(f"linear_f8: out must be [{N} x {M}]")
-        buf, wp, wbytes = _scratch(int(lib().axq_linear_f8_workspace_size(int(x_type), K, N)), device)
-        check(lib().axq_linear_f8(w.data.data_ptr(), w.data.shape[1], w.scales.data_ptr(), int(x_type), xd.data_ptr(), x_ld,
-                                  None if x_scales is None else x_scales.data_ptr(),
-                                  None if bias is None else bias.data_ptr(), int(out_type), out.data_ptr(), M, K, N, wp,
-                                  wbytes, _stream_handle(stream, device)))
-        del buf
+    L = lib()
+    buf, wp, wbytes = _scratch(L.axq_linear_f8_workspace_size(x_type, K, N), xd)
+    check(L.axq_linear_f8(w.data.data_ptr(), w.data.shape[1], w.scales.data_ptr(), x_type, xd.data_ptr(), x_ld, x_scales,
+                          bias_ptr, out_type, out.data_ptr(), M, K, N, wp, wbytes, _raw_stream(device.index)))
+    del buf
     return out

@@ -13,29 +13,25 @@ from typing import Optional, Tuple
 import torch
 
 from ._capi import BLOCK_BYTES, F8_BLOCK, F8_E4M3, check, lib
-from .f8 import F8Tensor, _float_type, _invalid, _on, _same_device, _scratch
-from .ops import QTensor, _packed_bytes, _req_cuda, _stream_handle
+from .f8 import F8Tensor, _float_type, _invalid, _on, _plain, _raw_stream, _same_device, _scratch
+from .ops import QTensor, _packed_bytes
 
 
 def _weights(w, rows: int, cols: int, name: str):
-    """(format id, codes, scales or None) of experts' weights [rows x cols]."""
-    if tuple(w.shape) != (rows, cols):
+    """(format id, codes, address of the scales or None) of experts' weights [rows x cols]."""
+    if w.shape != (rows, cols):
         raise _invalid(f"{name} must be [{rows} x {cols}] (got {tuple(w.shape)})")
     if isinstance(w, F8Tensor):
         w._check(name)
         if w.block_rows != F8_BLOCK or w.data.shape[1] != cols:
             raise _invalid(f"{name}: e4m3 experts are packed in 128 x 128 blocks, their rows without padding")
-        return F8_E4M3, w.data, w.scales
+        return F8_E4M3, w.data, w.scales.data_ptr()
     if not isinstance(w, QTensor) or w.fmt not in BLOCK_BYTES:
         raise _invalid(f"{name} must be a QTensor or an F8Tensor")
-    _req_cuda(w.data, name, torch.uint8)
+    _plain(w.data, name, torch.uint8)
     if w.data.numel() < _packed_bytes(rows, cols, w.fmt):
         raise _invalid(f"{name} is smaller than its shape")
     return int(w.fmt), w.data, None
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
 
 
 def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bool = True,
@@ -46,16 +42,20 @@ def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bo
     x is fp32, fp16 or bf16 [N, hidden], w_router fp32 [experts, hidden];
     ``normalize``: a token's weights add up to 1."""
     dtype = _float_type(x, "x")
-    _req_cuda(w_router, "w_router", torch.float32)
+    _plain(w_router, "w_router", torch.float32)
     if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
         raise _invalid("moe_route: x must be [N x hidden] and w_router [experts x hidden]")
-    _same_device(x.device, w_router=w_router)
+    device = x.device
+    _same_device(device, ("w_router",), w_router)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return moe_route(x, w_router, top_k, normalize)
     n = x.shape[0]
-    with _on(x.device, stream):
-        ids = torch.empty((n, top_k), dtype=torch.int32, device=x.device)
-        weights = torch.empty((n, top_k), dtype=torch.float32, device=x.device)
-        check(lib().axq_moe_route(int(dtype), x.data_ptr(), w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), n,
-                                  w_router.shape[0], top_k, x.shape[1], int(normalize), _stream_handle(stream, x.device)))
+    ids = x.new_empty((n, top_k), dtype=torch.int32)
+    weights = x.new_empty((n, top_k), dtype=torch.float32)
+    check(lib().axq_moe_route(dtype, x.data_ptr(), w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), n,
+                              w_router.shape[0], top_k, x.shape[1], 1 if normalize else 0, _raw_stream(device.index)))
     return ids, weights
 
 
@@ -68,8 +68,8 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
     format, w_down [experts * hidden, ffn].  Products and sums are fp32, y has x's
     type."""
     dtype = _float_type(x, "x")
-    _req_cuda(ids, "ids", torch.int32)
-    _req_cuda(weights, "weights", torch.float32)
+    _plain(ids, "ids", torch.int32)
+    _plain(weights, "weights", torch.float32)
     if x.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != weights.shape:
         raise _invalid("moe_mlp_q: x must be [N x hidden], ids and weights [N x top_k]")
     (n, hidden), top_k = x.shape, ids.shape[1]
@@ -81,17 +81,22 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
     fmt_down, down, down_s = _weights(w_down, experts * hidden, ffn, "w_down")
     if fmt != fmt_up:
         raise _invalid("moe_mlp_q: w_gate and w_up must have the same format")
-    _same_device(x.device, ids=ids, weights=weights, w_gate=gate, w_up=up, w_down=down, out=out)
-    with _on(x.device, stream):
-        if out is None:
-            out = torch.empty_like(x)
-        if _float_type(out, "out") != dtype or out.shape != x.shape:
-            raise _invalid("moe_mlp_q: out must have x's shape and type")
-        buf, wp, wbytes = _scratch(int(lib().axq_moe_workspace_size(n, top_k, hidden, ffn)), x.device)
-        check(lib().axq_moe_mlp(fmt, gate.data_ptr(), _ptr(gate_s), up.data_ptr(), _ptr(up_s), fmt_down, down.data_ptr(),
-                                _ptr(down_s), int(dtype), x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(),
-                                n, experts, top_k, hidden, ffn, wp, wbytes, _stream_handle(stream, x.device)))
-        del buf
+    device = x.device
+    _same_device(device, ("ids", "weights", "w_gate", "w_up", "w_down", "out"), ids, weights, gate, up, down, out)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, experts, out)
+    if out is None:
+        out = torch.empty_like(x)
+    elif _float_type(out, "out") != dtype or out.shape != x.shape:
+        raise _invalid("moe_mlp_q: out must have x's shape and type")
+    L = lib()
+    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn), x)
+    check(L.axq_moe_mlp(fmt, gate.data_ptr(), gate_s, up.data_ptr(), up_s, fmt_down, down.data_ptr(), down_s, dtype,
+                        x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(), n, experts, top_k, hidden, ffn, wp,
+                        wbytes, _raw_stream(device.index)))
+    del buf
     return out
 
 
