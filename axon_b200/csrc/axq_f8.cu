@@ -19,47 +19,55 @@ namespace axq {
 namespace {
 
 // 1 x 128 blocks: 16 lanes hold a block, 8 elements each; a half warp takes
-// kUnroll blocks at once so that their loads are in flight together.
-constexpr int kPackUnroll = 4;
+// kPackUnroll blocks at once so that their loads are in flight together.  A
+// block's row and place in it are walked, not divided out; 48 registers let
+// five blocks of threads share an SM (with 72 and three the loads' latency
+// showed: 34 us at 2500 x 8200 fp16).
+constexpr int kPackUnroll = 2;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) f8_pack_rows_kernel(const T* __restrict__ src, uint8_t* __restrict__ codes,
-                                                           int64_t ld, float* __restrict__ scales, int64_t rows,
-                                                           int64_t cols, int nkb, int* __restrict__ err) {
+__global__ void __launch_bounds__(256, 5) f8_pack_rows_kernel(const T* __restrict__ src, uint8_t* __restrict__ codes,
+                                                              int64_t ld, float* __restrict__ scales, int64_t rows,
+                                                              int64_t cols, int nkb, int* __restrict__ err) {
     pdl_wait();
     pdl_launch_dependents();
     if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;  // status word of the call this packing opens
-    // blocks number fewer than 2^31 (checked on the host), so 32-bit divisions serve
-    const uint32_t items = static_cast<uint32_t>(rows * nkb);
-    const uint32_t half = (blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-    const uint32_t halves = gridDim.x * blockDim.x >> 4;
+    const uint32_t halves = gridDim.x * blockDim.x >> 4, half = (blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+    const uint32_t n = static_cast<uint32_t>(nkb);
+    const uint32_t step_r = halves / n, step_k = halves - step_r * n;
+    uint32_t r = half / n, kb = half - r * n;
+    const uint32_t nr = static_cast<uint32_t>(rows);
     const int l = threadIdx.x & 15;
-    for (uint32_t it0 = half; (it0 & ~1u) < items; it0 += halves * kPackUnroll) {
-        // both halves of a warp stay in the loop together (the shuffles are warp-wide)
+    // both halves of a warp stay in the loop together (the shuffles are warp-wide)
+    while (__any_sync(0xFFFFFFFFu, r < nr)) {
         float v[kPackUnroll][8];
+        uint32_t ur[kPackUnroll], uk[kPackUnroll];
 #pragma unroll
         for (int u = 0; u < kPackUnroll; ++u) {
-            const uint32_t it = it0 + u * halves;
-            const uint32_t r = it / static_cast<uint32_t>(nkb);
-            const int64_t c0 = static_cast<int64_t>(it - r * nkb) * kF8Block + 8 * l;
-            if (it < items) {
-                load_row8<T, VEC>(src + static_cast<int64_t>(r) * cols, c0, cols, v[u]);
+            ur[u] = r;
+            uk[u] = kb;
+            if (r < nr) {
+                load_row8<T, VEC>(src + static_cast<int64_t>(r) * cols, static_cast<int64_t>(kb) * kF8Block + 8 * l, cols, v[u]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
             }
+            r += step_r;
+            kb += step_k;
+            if (kb >= n) {
+                kb -= n;
+                ++r;
+            }
         }
 #pragma unroll
         for (int u = 0; u < kPackUnroll; ++u) {
-            const uint32_t it = it0 + u * halves;
             uint32_t w[2];
             const float s = pack_block16(v[u], w);
-            if (it >= items) continue;
-            const uint32_t r = it / static_cast<uint32_t>(nkb);
-            const uint32_t kb = it - r * nkb;
-            const int64_t c0 = static_cast<int64_t>(kb) * kF8Block + 8 * l;
-            if (c0 < ld) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * ld + c0) = make_uint2(w[0], w[1]);
-            if (l == 0) scales[it] = s;
+            if (ur[u] < nr) {
+                const int64_t c0 = static_cast<int64_t>(uk[u]) * kF8Block + 8 * l;
+                if (c0 < ld) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(ur[u]) * ld + c0) = make_uint2(w[0], w[1]);
+                if (l == 0) scales[static_cast<int64_t>(ur[u]) * n + uk[u]] = s;
+            }
         }
     }
 }
@@ -110,14 +118,14 @@ __global__ void __launch_bounds__(256) f8_pack_blocks_kernel(const T* __restrict
     m = red[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
-    const float s = __fdiv_rn(m, kF8Max);
-    const F8Div div(s);
+    const float s = f8_scale(m);
     if (threadIdx.x == 0) scales[blockIdx.x] = s;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int64_t r = r0 + j;
-        const uint32_t w = cvt_e4m3x2(div(v[j][0]), div(v[j][1])) | (cvt_e4m3x2(div(v[j][2]), div(v[j][3])) << 16);
-        if (r < rows && c0 < ld) *reinterpret_cast<uint32_t*>(codes + r * ld + c0) = w;
+        uint32_t w[1];
+        f8_codes(v[j], s, w);
+        if (r < rows && c0 < ld) *reinterpret_cast<uint32_t*>(codes + r * ld + c0) = w[0];
     }
 }
 
@@ -177,8 +185,8 @@ cudaError_t f8_pack_dispatch(int dtype, const void* src, void* codes, int64_t ld
         // 16-byte loads (8 of a 16-bit type, 4 of fp32 in the block kernel's 8-byte ones) need every row aligned
         const bool vec = reinterpret_cast<uintptr_t>(src) % 16 == 0 && (cols * sizeof(T)) % 16 == 0;
         if (block_rows == 1) {
-            const int64_t halves = (rows * nkb + kPackUnroll - 1) / kPackUnroll;
-            const int64_t grid = std::min<int64_t>((halves + 15) / 16, int64_t(device_sm_count()) * 8);
+            // a half warp for each block up to a full GPU: small matrices are bound by the latency of one round
+            const int64_t grid = std::min<int64_t>((rows * nkb + 15) / 16, int64_t(device_sm_count()) * 5);
             auto k = vec ? f8_pack_rows_kernel<T, true> : f8_pack_rows_kernel<T, false>;
             cudaError_t e = launch_pdl(k, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, p, out, ld, scales, rows,
                                        cols, nkb, err);

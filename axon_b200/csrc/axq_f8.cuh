@@ -66,31 +66,49 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float a, float b) {
     return r;
 }
 
-// x / s rounded to nearest for many x and one s.  With y = RN(1/s),
-// q = RN(x*y) and r = x - q*s (exact in one FMA), RN(q + r*y) is the
-// correctly rounded quotient unless s's significand is all ones (Markstein,
-// "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990): two FMAs and a product instead of a division.  Where s
-// is outside 2^-90 .. 2^90 (r might not be exact) or all ones, the division
-// itself is used.  |x| < 2^-100 then gives a quotient below 2^-10, whose code
-// is 0 either way.
-struct F8Div {
-    float s, y;
-    bool fast;
-    __device__ __forceinline__ explicit F8Div(float scale) : s(scale) {
-        const uint32_t b = __float_as_uint(scale);
-        fast = scale > 8.0779357e-28f && scale < 1.2379400e27f && (b & 0x7FFFFFu) != 0x7FFFFFu;
-        y = __fdiv_rn(1.0f, scale);
+// a / b rounded to nearest from y = RN(1/b): with q = RN(a*y) and r = q*b - a
+// (exact in one FMA), RN(q - r*y) is the correctly rounded quotient unless b's
+// significand is all ones (Markstein, "Computation of elementary functions on
+// the IBM RISC System/6000 processor", 1990) and as long as r is exact and
+// nothing overflows.  -0 stays -0 in this order.
+__device__ __forceinline__ float div_by(float a, float b, float y) {
+    const float q = __fmul_rn(a, y);
+    return __fmaf_rn(-__fmaf_rn(q, b, -a), y, q);
+}
+
+// The cases that div_by does not cover, out of line: they are rare and their
+// code, inlined at each element, filled the instruction cache.
+static __device__ __noinline__ float div_slow(float a, float b) {
+    if (b == 0.0f) return a != a ? a : 0.0f;
+    return __fdiv_rn(a, b);
+}
+
+// Scale of a block with maximum m: RN(m / 448).
+__device__ __forceinline__ float f8_scale(float m) {
+    // outside 2^-100 .. 2^126 (0 and infinity among them) r might not be exact
+    if (m > 7.8886091e-31f && m < 8.5070592e37f) return div_by(m, kF8Max, 1.0f / kF8Max);
+    return __fdiv_rn(m, kF8Max);
+}
+
+// Codes of N elements under the scale s: two FMAs, a product and half a
+// conversion each.  Where s is outside 2^-90 .. 2^90 or its significand is all
+// ones the division itself is used; |x| < 2^-100 otherwise gives a quotient
+// below 2^-10, whose code is 0 whether r is exact or not.
+template <int N>
+__device__ __forceinline__ void f8_codes(const float (&v)[N], float s, uint32_t (&w)[N / 4]) {
+    float q[N];
+    if (s > 8.0779357e-28f && s < 1.2379400e27f && (__float_as_uint(s) & 0x7FFFFFu) != 0x7FFFFFu) {
+        const float y = __frcp_rn(s);
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = div_by(v[i], s, y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = div_slow(v[i], s);
     }
-    __device__ __forceinline__ float operator()(float x) const {
-        if (fast) {
-            const float q = __fmul_rn(x, y);
-            return __fmaf_rn(-__fmaf_rn(q, s, -x), y, q);  // in this order -0 stays -0
-        }
-        if (s == 0.0f) return x != x ? x : 0.0f;
-        return __fdiv_rn(x, s);
-    }
-};
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+        w[i] = cvt_e4m3x2(q[4 * i], q[4 * i + 1]) | (cvt_e4m3x2(q[4 * i + 2], q[4 * i + 3]) << 16);
+}
 
 // Elements c0 .. c0+7 of a row of `cols` (zero past them).
 template <typename T, bool VEC>
@@ -111,11 +129,8 @@ __device__ __forceinline__ float pack_block16(const float (&v)[8], uint32_t (&w)
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
 #pragma unroll
     for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const float s = __fdiv_rn(m, kF8Max);
-    const F8Div div(s);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        w[i] = cvt_e4m3x2(div(v[4 * i]), div(v[4 * i + 1])) | (cvt_e4m3x2(div(v[4 * i + 2]), div(v[4 * i + 3])) << 16);
+    const float s = f8_scale(m);
+    f8_codes(v, s, w);
     return s;
 }
 

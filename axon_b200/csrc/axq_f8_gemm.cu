@@ -310,15 +310,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 // ---- few tokens ---------------------------------------------------------------
 
-constexpr int skinny_warps(int nt) { return nt > 64 ? 8 : 4; }
+constexpr int kSkinnyThreads = 192;  // producer warp, MMA warp, four epilogue warps
 
 // TX: type of an X that the kernel packs itself (every CTA its K range of all
 // tokens, while the first weight tiles arrive); void: X is packed already.
 template <int NT, typename TY, typename TX>
-__global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
+__global__ void __launch_bounds__(kSkinnyThreads)
     f8_skinny_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, F8Args a, int splits) {
-    constexpr int kEpi = skinny_warps(NT);
-    constexpr int kCols = NT / (kEpi / 4);
+    constexpr int kEpi = 4;  // epilogue warps: a TMEM lane quarter each
+    constexpr int kCols = NT;
     constexpr bool kPack = !std::is_void_v<TX>;
     constexpr int kWBytes = 128 * 128, kXBytes = NT * 128, kStage = kWBytes + (kPack ? 0 : kXBytes);
     constexpr int kBuf = 2;
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
             }
         }
     } else {
-        const int q = warp & 3, g = (warp - 2) >> 2;
+        const int q = warp & 3;
         const int et = threadIdx.x - 64;
         pdl_wait();
         if constexpr (kPack) {
@@ -491,8 +491,8 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
             if (i + 1 < nk) nw = __ldg(sw + i + 1);
             if (!f8_wait(&bars.done[s], par, &bars, a.err)) break;
             tc_fence_after();
-            const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * NT + g * kCols;
-            const float* sc = sxs + i * NT + g * kCols;
+            const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + b * NT;
+            const float* sc = sxs + i * NT;
 #pragma unroll
             for (int c = 0; c < kCols; c += 16) {
                 float v[16];
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(64 + 32 * skinny_warps(NT))
         // so their memory holds the sums now: [token][weight row]
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpi) : "memory");
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) red[(g * kCols + i) * 128 + 32 * q + lane] = acc[i];
+        for (int i = 0; i < kCols; ++i) red[i * 128 + 32 * q + lane] = acc[i];
     }
     tc_fence_before();
     __syncthreads();
@@ -663,7 +663,7 @@ cudaError_t launch_skinny(const F8Linear& l, F8Args a, cudaStream_t s) {
     const int smem = static_cast<int>(a.stages * kStage + own + 1024);
     static std::atomic<int> cfg[64];
     if (cudaError_t e = ensure_dyn_smem(f8_skinny_kernel<NT, TY, TX>, smem, cfg); e != cudaSuccess) return e;
-    return launch_cluster(f8_skinny_kernel<NT, TY, TX>, static_cast<int>(tiles * splits), 64 + 32 * skinny_warps(NT), splits,
+    return launch_cluster(f8_skinny_kernel<NT, TY, TX>, static_cast<int>(tiles * splits), kSkinnyThreads, splits,
                           smem, s, mx, mw, a, splits);
 }
 
@@ -709,7 +709,8 @@ cudaError_t f8_gemm_dispatch(const F8Linear& l, cudaStream_t s) {
         if (l.N <= 16) return launch_skinny<16, TY, void>(l, a, s);
         if (l.N <= 32) return launch_skinny<32, TY, void>(l, a, s);
         if (l.N <= 64) return launch_skinny<64, TY, void>(l, a, s);
-        if (l.N <= 128) return launch_skinny<128, TY, void>(l, a, s);
+        // more tokens: the pair kernel is faster even where half of its 256 rows are padding (128 tokens: 28672 x 8192
+        // 76 against 93 us, 4096 x 4096 18 against 32)
         const int64_t wide = (l.N + 255) / 256 * ((l.M + 255) / 256);
         return wide * 2 >= device_sm_count() ? launch_pair<256, TY>(l, a, s) : launch_pair<128, TY>(l, a, s);
     });
