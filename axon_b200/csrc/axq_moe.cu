@@ -4,17 +4,18 @@
 //            e = ids[t][j].
 //
 // HBM-bound on the packed bytes of the experts that some token chose; each is
-// read once per group of up to 4 NB of its tokens.
+// read once per group of up to 8 of its tokens.
 //
 //  * moe_route_kernel: a cluster of 8 CTAs per 4 tokens splits the experts, its
 //    first CTA picks the top_k.
 //  * moe_prep_kernel: the plan (tokens' choices sorted by expert, in groups), and
-//    records of x: per 256 elements two fp16 terms (x 2^-e ~ hi + lo, 22 bits) in
-//    the order of the weights' MMA fragments, and sums for the minimums.
+//    records of x: per 256 elements one or two fp16 terms (x 2^-e = hi or ~ hi +
+//    lo, 22 bits) in the order of the weights' MMA fragments, and sums for the
+//    minimums.
 //  * moe_expert_kernel: a producer warp streams packed rows through a ring of
 //    shared-memory stages (bulk copies); eight consumer warps decode them into
 //    exact fp16 fragments (axq_moe_decode.cuh) and multiply with mma.sync
-//    m16n8k16, whose 8 columns are the two terms of four tokens.  Runs twice: gate
+//    m16n8k16, whose 8 columns are eight tokens or the two terms of four.  Runs twice: gate
 //    and up (tile 0 and 1 of a unit are 16 rows of each, joined by silu), and
 //    down (32 rows).  mma.sync and not tcgen05: the weights are decoded in
 //    registers, and with at most 8 columns the tensor pipe is idle most of the
@@ -167,10 +168,14 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
 
 // ---- plan and activation records ---------------------------------------------------
 
-// Record of one row and CG: eight 128-byte lines (one for each pair of MMAs:
-// [term][lane part][16 bytes]), the sums [term][lane part][8 bytes], the scale.
-constexpr int kRec = 1152;
-constexpr int kRecSums = 1024, kRecScale = 1088;
+// Record of one row and CG with T terms: eight lines (one for each pair of MMAs:
+// [term][lane part][16 bytes]), the sums as two terms [2][lane part][8 bytes],
+// the scale.
+// One term holds fp16 and bf16 activations exactly (down to 2^-33 of the largest
+// of the 256), two hold fp32 ones to 22 bits.
+template <int T> constexpr int kRecSums = 512 * T;
+template <int T> constexpr int kRecScale = kRecSums<T> + 64;
+template <int T> constexpr int kRec = (kRecScale<T> + 4 + 63) / 64 * 64;
 
 // Two fp16 terms of v (already scaled): v = hi + lo within 2^-22 of it.
 __device__ __forceinline__ void split2(float v, __half& hi, __half& lo) {
@@ -180,7 +185,7 @@ __device__ __forceinline__ void split2(float v, __half& hi, __half& lo) {
 }
 
 // One warp: the record of 256 elements in s (shared memory, zero past the end).
-template <int F>
+template <int F, int T>
 __device__ __forceinline__ void write_record(const float* s, uint8_t* rec, int lane) {
     float m = 0.0f;
 #pragma unroll
@@ -198,32 +203,40 @@ __device__ __forceinline__ void write_record(const float* s, uint8_t* rec, int l
         const int el = Order<F>::elem(2 * mp + (k >> 2), i, k & 3);
         split2(s[el] * up, hi[k], lo[k]);
     }
-    uint4 a, b;
+    uint4 a;
     memcpy(&a, hi, 16);
-    memcpy(&b, lo, 16);
-    *reinterpret_cast<uint4*>(rec + mp * 128 + i * 16) = a;
-    *reinterpret_cast<uint4*>(rec + mp * 128 + 64 + i * 16) = b;
+    *reinterpret_cast<uint4*>(rec + mp * 64 * T + i * 16) = a;
+    if constexpr (T == 2) {
+        memcpy(&a, lo, 16);
+        *reinterpret_cast<uint4*>(rec + mp * 64 * T + 64 + i * 16) = a;
+    }
     if constexpr (Order<F>::SUMS > 0) {
         if (lane < 16) {  // lane part lane / 4, slot lane % 4
             constexpr int N = 256 / Order<F>::SUMS;
             const int sb = Order<F>::sum(lane >> 2, lane & 3);
             float v = 0.0f;
-            if (sb >= 0)
-                for (int k = 0; k < N; ++k) v += s[sb * N + ((k + lane) & (N - 1))];
+            if (sb >= 0) {
+                for (int k = 0; k < N; ++k) {
+                    const float x = s[sb * N + ((k + lane) & (N - 1))];
+                    // what the codes are multiplied with: with one term, its rounding
+                    v += T == 2 ? x : __half2float(__float2half_rn(x * up));
+                }
+            }
             __half h, l;
-            split2(v * up, h, l);
-            reinterpret_cast<__half*>(rec + kRecSums)[lane] = h;
-            reinterpret_cast<__half*>(rec + kRecSums + 32)[lane] = l;
+            split2(T == 2 ? v * up : v, h, l);
+            reinterpret_cast<__half*>(rec + kRecSums<T>)[lane] = h;
+            reinterpret_cast<__half*>(rec + kRecSums<T> + 32)[lane] = l;
         }
     }
-    if (lane == 0) *reinterpret_cast<float*>(rec + kRecScale) = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    if (lane == 0)
+        *reinterpret_cast<float*>(rec + kRecScale<T>) = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
 constexpr int kPrepWarps = 8;
 
 // Rows of x (or h) -> records; block 0 also makes the plan when ids are given.
 // need (may be null): rows whose expert id is out of range are skipped.
-template <int F, typename T>
+template <int F, int TERMS, typename T>
 __global__ void __launch_bounds__(32 * kPrepWarps)
     moe_prep_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int ncg, uint8_t* __restrict__ rec,
                     const int* __restrict__ need, int experts, MoePlan plan) {
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
         buf[warp][32 * j + lane] = k < cols ? Elem<T>::get(x[r * cols + k]) : 0.0f;
     }
     __syncwarp();
-    write_record<F>(buf[warp], rec + it * kRec, lane);
+    write_record<F, TERMS>(buf[warp], rec + it * kRec<TERMS>, lane);
 }
 
 // ---- experts -------------------------------------------------------------------------
@@ -344,30 +357,49 @@ __device__ __forceinline__ float2 block_scales(const MoeRow<F> (&r)[2], const fl
     }
 }
 
+// Columns of an MMA with T terms: column c is term c % T of token c / T.  A lane
+// reads column g = lane / 4 of B and holds columns 2 i and 2 i + 1 of the sums:
+// two tokens, or the two terms of one.
+template <int T>
+struct Cols {
+    static constexpr int kTokens = 8 / T;  // of a block of columns
+    static constexpr int kOwn = 2 / T;     // of a lane's sums
+    __device__ __forceinline__ static int token(int g) { return g / T; }
+    __device__ __forceinline__ static int own(int i, int u) { return kOwn * i + u; }
+    __device__ __forceinline__ static int offset(int g, int i) { return (T == 2 ? (g & 1) * 64 : 0) + i * 16; }
+    // the lane's sums of row r (0: g, 1: g + 8)
+    __device__ __forceinline__ static float sum(const float (&c)[4], int r, int u) {
+        return T == 2 ? c[2 * r] + c[2 * r + 1] : c[2 * r + u];
+    }
+};
+
 // Lines of the activation record loaded ahead of their use, as far as the
 // format's registers allow; the first are loaded before the wait for the stage.
+// e4m3, whose decoder needs next to none, holds all eight of a CG for both tiles.
 template <int F, int NB>
-constexpr int kAhead = (F == F_F8 ? 4 : F == F_Q8_0 || F == F_Q4_0 ? 3 : 2) / NB;
+constexpr int kAhead = (F == F_F8 ? 8 : F == F_Q8_0 || F == F_Q4_0 ? 3 : 2) / NB;
 
-template <int F, int NB>
+template <int F, int T, int NB>
 struct ActLines {
     uint4 b[NB][kAhead<F, NB> + 1];
     template <int MP>
     __device__ __forceinline__ void load(const uint8_t* const (&rec)[NB]) {
 #pragma unroll
         for (int n = 0; n < NB; ++n)
-            b[n][MP % (kAhead<F, NB> + 1)] = __ldg(reinterpret_cast<const uint4*>(rec[n] + MP * 128));
+            b[n][MP % (kAhead<F, NB> + 1)] = __ldg(reinterpret_cast<const uint4*>(rec[n] + MP * 64 * T));
     }
 };
 
 // One CG of TL tiles (rows g and g + 8 of tile t at p[t][0], p[t][1]) times NB
-// blocks of four tokens: tot[t][n][r] += row r's product with token 4 n + i.
+// blocks of eight columns: tot[t][n][r][u] += row r's product with this lane's
+// u-th token of block n (see Cols).
 // Tiles taken together share the loads of the activations, whose first kAhead
 // lines are in `x`.
-template <int F, int NB, int TL>
-__device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int i, const uint8_t* const (&rec)[NB],
-                                       ActLines<F, NB>& x, const float (&xs)[NB], int blocks, const float* const* wsc,
-                                       float (*tot)[NB][2]) {
+template <int F, int T, int NB, int TL>
+__device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int g, int i, const uint8_t* const (&rec)[NB],
+                                       ActLines<F, T, NB>& x, const float (&xs)[NB][Cols<T>::kOwn], int blocks,
+                                       const float* const* wsc, float (*tot)[NB][2][Cols<T>::kOwn]) {
+    using C = Cols<T>;
     MoeRow<F> r[TL][2];
     float acc[TL][NB][4];
 #pragma unroll
@@ -393,10 +425,12 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int i, cons
                 if (B < blocks) {
                     const float2 d = block_scales<F>(r[t], wsc[t] + B);
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        tot[t][n][0] = fmaf(xs[n] * d.x, acc[t][n][0] + acc[t][n][1], tot[t][n][0]);
-                        tot[t][n][1] = fmaf(xs[n] * d.y, acc[t][n][2] + acc[t][n][3], tot[t][n][1]);
-                    }
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int u = 0; u < C::kOwn; ++u) {
+                            tot[t][n][0][u] = fmaf(xs[n][u] * d.x, C::sum(acc[t][n], 0, u), tot[t][n][0][u]);
+                            tot[t][n][1][u] = fmaf(xs[n][u] * d.y, C::sum(acc[t][n], 1, u), tot[t][n][1][u]);
+                        }
                 }
 #pragma unroll
                 for (int n = 0; n < NB; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.0f;
@@ -404,12 +438,13 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int i, cons
         }
     });
     if constexpr (Order<F>::SUMS > 0) {
-        uint2 b[NB];
+        // the sums of this lane's column and part: with one term the two terms of a sum are two MMAs
+        uint2 b[NB], bl[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            // the line of this lane's column and part: sums are 8 bytes where codes are 16
-            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(rec[n])) & 127u;  // term * 64 + i * 16
-            b[n] = __ldg(reinterpret_cast<const uint2*>(rec[n] - off + kRecSums + off / 2));
+            const uint8_t* q = rec[n] + (kRecSums<T> - C::offset(g, i)) + (T == 2 ? (g & 1) * 32 : 0) + i * 8;
+            b[n] = __ldg(reinterpret_cast<const uint2*>(q));
+            if constexpr (T == 1) bl[n] = __ldg(reinterpret_cast<const uint2*>(q + 32));
         }
 #pragma unroll
         for (int t = 0; t < TL; ++t) {
@@ -422,8 +457,14 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int i, cons
             for (int n = 0; n < NB; ++n) {
                 float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 mma16816(c, a, b[n].x, b[n].y);
-                tot[t][n][0] = fmaf(xs[n], fmaf(s0.x, acc[t][n][0] + acc[t][n][1], -s0.y * (c[0] + c[1])), tot[t][n][0]);
-                tot[t][n][1] = fmaf(xs[n], fmaf(s1.x, acc[t][n][2] + acc[t][n][3], -s1.y * (c[2] + c[3])), tot[t][n][1]);
+                if constexpr (T == 1) mma16816(c, a, bl[n].x, bl[n].y);
+#pragma unroll
+                for (int u = 0; u < C::kOwn; ++u) {
+                    tot[t][n][0][u] =
+                        fmaf(xs[n][u], fmaf(s0.x, C::sum(acc[t][n], 0, u), -s0.y * C::sum(c, 0, u)), tot[t][n][0][u]);
+                    tot[t][n][1][u] =
+                        fmaf(xs[n][u], fmaf(s1.x, C::sum(acc[t][n], 1, u), -s1.y * C::sum(c, 1, u)), tot[t][n][1][u]);
+                }
             }
         }
     }
@@ -493,10 +534,11 @@ __device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb
     }
 }
 
-template <int F, int NB>
+template <int F, int T, int NB>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const ExpertArgs a) {
+    using C = Cols<T>;
     constexpr int CGB = moe_cg_bytes<F>();
-    constexpr int kTok = 4 * NB;
+    constexpr int kTok = C::kTokens * NB;
     constexpr int TL = kStageTiles<F, NB>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127);
@@ -597,32 +639,39 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
     for (int q = 0; q < hi - lo; ++q) {
         const int unit = rd.t0 + u;
         const int4 gd = a.plan.groups[rd.grp];  // expert, first entry, number of entries
-        // this lane's B column: term g & 1 of token 4 n + g / 2 (past the group's end: its first), and the scale of
-        // its accumulator columns, those of token 4 n + i
-        const uint8_t *rec0[NB], *scale0[NB];
+        // this lane's B column, and the scales of its sums' columns (columns past the group's end: its first token's)
+        const uint8_t *rec0[NB], *scale0[NB][C::kOwn];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const int t = 4 * n + (g >> 1), ts = 4 * n + i;
-            const int2 e = a.plan.entries[gd.y + (t < gd.z ? t : 0)], es = a.plan.entries[gd.y + (ts < gd.z ? ts : 0)];
-            rec0[n] = a.rec + (a.rec_token ? e.y : e.x) * a.rec_row + (g & 1) * 64 + i * 16;
-            scale0[n] = a.rec + (a.rec_token ? es.y : es.x) * a.rec_row + kRecScale;
+            const int t = n * C::kTokens + C::token(g);
+            const int2 e = a.plan.entries[gd.y + (t < gd.z ? t : 0)];
+            rec0[n] = a.rec + (a.rec_token ? e.y : e.x) * a.rec_row + C::offset(g, i);
+#pragma unroll
+            for (int v = 0; v < C::kOwn; ++v) {
+                const int ts = n * C::kTokens + C::own(i, v);
+                const int2 es = a.plan.entries[gd.y + (ts < gd.z ? ts : 0)];
+                scale0[n][v] = a.rec + (a.rec_token ? es.y : es.x) * a.rec_row + kRecScale<T>;
+            }
         }
-        float tot[2][NB][2];
+        float tot[2][NB][2][C::kOwn];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int n = 0; n < NB; ++n) tot[t][n][0] = tot[t][n][1] = 0.0f;
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < C::kOwn; ++v) tot[t][n][0][v] = tot[t][n][1][v] = 0.0f;
         const int64_t row0 = gd.x * a.rows + stage_row(a, unit, 0, 0);
         for (int k = 0; k < ksteps; ++k) {
             const int cg = k * a.wps + col;
             const bool mine = cg < a.ncg && unit < a.tiles;
             const uint8_t* rec[NB];
-            float xs[NB];
+            float xs[NB][C::kOwn];
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const int64_t at = static_cast<int64_t>(mine ? cg : 0) * kRec;
+                const int64_t at = static_cast<int64_t>(mine ? cg : 0) * kRec<T>;
                 rec[n] = rec0[n] + at;
-                xs[n] = __ldg(reinterpret_cast<const float*>(scale0[n] + at));
+#pragma unroll
+                for (int v = 0; v < C::kOwn; ++v) xs[n][v] = __ldg(reinterpret_cast<const float*>(scale0[n][v] + at));
             }
             // bytes of the first row's segment past a multiple of 16 (low bits suffice)
             const uint32_t ph0 = kAlignedRows<F> ? 0u : static_cast<uint32_t>(row0) * static_cast<uint32_t>(a.rb) +
@@ -630,10 +679,11 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
             // e4m3: scales of the unit's rows (16 or 32 rows from a multiple of 16, so one block of 128)
             const int64_t sc0 = F == F_F8 ? min64(row0, (gd.x + 1) * a.rows - 1) / 128 * a.nblk + 2 * cg : 0;
             const int blocks = a.nblk - (F == F_F8 ? 2 : 8) * cg;
+            ActLines<F, T, NB> x;
 #pragma unroll
             for (int h = 0; h < 2 / TL; ++h) {
-                ActLines<F, NB> x;
-                static_for_pairs<kAhead<F, NB>>([&](auto J) { x.template load<decltype(J)::value>(rec); });
+                if (h == 0 || kAhead<F, NB> < 8)
+                    static_for_pairs<kAhead<F, NB>>([&](auto J) { x.template load<decltype(J)::value>(rec); });
                 if (ok) ok = moe_wait(&bars.full[s], par, &bars, a.err);
                 if (ok && mine) {
                     const uint8_t* st = ring + s * a.stage_bytes + u * (16 * TL) * a.rs + col * CGB;
@@ -652,7 +702,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
                         }
                         wsc[t] = F == F_F8 ? a.sc[tile] + sc0 : nullptr;
                     }
-                    moe_cg<F, NB, TL>(p, i, rec, x, xs, blocks, wsc, tot + (TL == 2 ? 0 : h));
+                    moe_cg<F, T, NB, TL>(p, g, i, rec, x, xs, blocks, wsc, tot + (TL == 2 ? 0 : h));
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.empty[s]);
@@ -675,11 +725,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                float* to = rb + ((warp * 2 + t) * kTok + 4 * n + i) * 16;
-                to[g] = tot[t][n][0];
-                to[g + 8] = tot[t][n][1];
-            }
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int v = 0; v < C::kOwn; ++v) {
+                    float* to = rb + ((warp * 2 + t) * kTok + n * C::kTokens + C::own(i, v)) * 16;
+                    to[g] = tot[t][n][0][v];
+                    to[g + 8] = tot[t][n][1][v];
+                }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.sums[q & 1]);
     }
@@ -727,7 +779,7 @@ cudaError_t with_moe_fmt(int fmt, Fn&& f) {
     }
 }
 
-template <int F, int NB>
+template <int F, int T, int NB>
 cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     constexpr int CGB = moe_cg_bytes<F>();
     a.ncg = static_cast<int>((cols + 255) / 256);
@@ -750,7 +802,7 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     a.rs = (cgs * CGB + 15 + 4 + 15) / 16 * 16;
     while (a.rs % 128 != 16) a.rs += 16;
     a.stage_bytes = a.slots * 16 * kStageTiles<F, NB> * a.rs;
-    const int red = 2 * kConsumers * 2 * 4 * NB * 16 * 4;
+    const int red = 2 * kConsumers * 2 * (8 / T) * NB * 16 * 4;
     const int budget = 112 * 1024 - 512 - red;  // two CTAs per SM
     a.stages = std::min(kMoeStages, budget / a.stage_bytes);
     int per_sm = 2;
@@ -761,28 +813,32 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     if (a.stages < 2) return cudaErrorInvalidConfiguration;
     const int smem = a.stages * a.stage_bytes + red + 128;
     static std::atomic<int> cfg[64];
-    if (cudaError_t e = ensure_dyn_smem(moe_expert_kernel<F, NB>, smem, cfg); e != cudaSuccess) return e;
-    cudaError_t e = launch_pdl(moe_expert_kernel<F, NB>, dim3(static_cast<unsigned>(device_sm_count() * per_sm)),
+    if (cudaError_t e = ensure_dyn_smem(moe_expert_kernel<F, T, NB>, smem, cfg); e != cudaSuccess) return e;
+    cudaError_t e = launch_pdl(moe_expert_kernel<F, T, NB>, dim3(static_cast<unsigned>(device_sm_count() * per_sm)),
                                dim3(kMoeThreads), smem, s, a);
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int nb, cudaStream_t s) {
+// Groups are of 8 tokens where one term holds them; with two terms of 4, or of 8
+// (two blocks of columns) where the experts have more on average.
+cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int terms, int group, cudaStream_t s) {
     return with_moe_fmt(fmt, [&](auto f) {
         constexpr int F = decltype(f)::value;
-        return nb == 1 ? launch_expert<F, 1>(a, cols, s) : launch_expert<F, 2>(a, cols, s);
+        return terms == 1 ? launch_expert<F, 1, 1>(a, cols, s)
+               : group == 4 ? launch_expert<F, 2, 1>(a, cols, s) : launch_expert<F, 2, 2>(a, cols, s);
     });
 }
 
 template <typename T>
-cudaError_t launch_prep(int fmt, const T* x, int64_t rows, int64_t cols, uint8_t* rec, const int* need, int experts,
-                        const MoePlan& plan, cudaStream_t s) {
+cudaError_t launch_prep(int fmt, int terms, const T* x, int64_t rows, int64_t cols, uint8_t* rec, const int* need,
+                        int experts, const MoePlan& plan, cudaStream_t s) {
     const int ncg = static_cast<int>((cols + 255) / 256);
     const int64_t grid = (rows * ncg + kPrepWarps - 1) / kPrepWarps + (plan.ids ? 1 : 0);
     return with_moe_fmt(fmt, [&](auto f) {
         constexpr int F = decltype(f)::value;
-        cudaError_t e = launch_pdl(moe_prep_kernel<F, T>, dim3(static_cast<unsigned>(grid)), dim3(32 * kPrepWarps), 0, s, x,
-                                   rows, cols, ncg, rec, need, experts, plan);
+        auto k = terms == 1 ? moe_prep_kernel<F, 1, T> : moe_prep_kernel<F, 2, T>;
+        cudaError_t e = launch_pdl(k, dim3(static_cast<unsigned>(grid)), dim3(32 * kPrepWarps), 0, s, x, rows, cols, ncg, rec,
+                                   need, experts, plan);
         return e == cudaSuccess ? cudaGetLastError() : e;
     });
 }
@@ -806,8 +862,8 @@ MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
         return r;
     };
     w.plan = take(kMoePlanBytes);
-    w.rec_x = take(static_cast<size_t>(t) * ((hidden + 255) / 256) * kRec);
-    w.rec_h = take(static_cast<size_t>(p) * ((ffn + 255) / 256) * kRec);
+    w.rec_x = take(static_cast<size_t>(t) * ((hidden + 255) / 256) * kRec<2>);
+    w.rec_h = take(static_cast<size_t>(p) * ((ffn + 255) / 256) * kRec<2>);
     w.h = take(static_cast<size_t>(p) * ffn * 4);
     w.z = take(static_cast<size_t>(p) * hidden * 4);
     w.total = at;
@@ -844,13 +900,14 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
     const int size = host_dtype_size(m.dtype);
     for (int64_t t0 = 0; t0 < m.tokens; t0 += step) {
         const int64_t t = std::min(step, m.tokens - t0), p = t * m.top_k;
-        // groups of 4 tokens unless the experts have more on average: the second block of columns costs registers
-        const int nb = p > 4 * m.experts ? 2 : 1;
+        // 16-bit x is one term; so are the hidden activations of a bf16 result, whose own rounding is 8 times theirs
+        const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = m.dtype == AXQ_DT_BF16 ? 1 : 2;
+        const int group = terms_x == 1 || p > 4 * m.experts ? 8 : 4;
         MoePlan plan = moe_plan_at(base + w.plan);
         plan.ids = m.ids + t0 * m.top_k;
         plan.npairs = static_cast<int>(p);
         plan.experts = m.experts;
-        plan.group = 4 * nb;
+        plan.group = group;
         plan.top_k = m.top_k;
         plan.err = t0 == 0 ? err : nullptr;
         const MoePlan made = [&] {
@@ -864,7 +921,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         float* z = reinterpret_cast<float*>(base + w.z);
         cudaError_t e = with_dtype(m.dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            return launch_prep<T>(m.fmt, static_cast<const T*>(x), t, m.hidden, base + w.rec_x, nullptr, m.experts, plan, s);
+            return launch_prep<T>(m.fmt, terms_x, static_cast<const T*>(x), t, m.hidden, base + w.rec_x, nullptr, m.experts, plan, s);
         });
         if (e != cudaSuccess) return e;
         ExpertArgs a{};
@@ -877,13 +934,13 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.rows = m.ffn;
         a.gate_up = 1;
         a.rec = base + w.rec_x;
-        a.rec_row = (m.hidden + 255) / 256 * kRec;
+        a.rec_row = (m.hidden + 255) / 256 * (terms_x == 1 ? kRec<1> : kRec<2>);
         a.rec_token = 1;
         a.out = h;
         a.plan = made;
         a.err = err;
-        if (e = launch_experts(m.fmt, a, m.hidden, nb, s); e != cudaSuccess) return e;
-        e = launch_prep<float>(m.fmt_down, h, p, m.ffn, base + w.rec_h, plan.ids, m.experts, made, s);
+        if (e = launch_experts(m.fmt, a, m.hidden, terms_x, group, s); e != cudaSuccess) return e;
+        e = launch_prep<float>(m.fmt_down, terms_h, h, p, m.ffn, base + w.rec_h, plan.ids, m.experts, made, s);
         if (e != cudaSuccess) return e;
         a.w[0] = a.w[1] = static_cast<const uint8_t*>(m.w_down);
         a.sc[0] = a.sc[1] = m.s_down;
@@ -892,10 +949,10 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.rows = m.hidden;
         a.gate_up = 0;
         a.rec = base + w.rec_h;
-        a.rec_row = (m.ffn + 255) / 256 * kRec;
+        a.rec_row = (m.ffn + 255) / 256 * (terms_h == 1 ? kRec<1> : kRec<2>);
         a.rec_token = 0;
         a.out = z;
-        if (e = launch_experts(m.fmt_down, a, m.ffn, nb, s); e != cudaSuccess) return e;
+        if (e = launch_experts(m.fmt_down, a, m.ffn, terms_h, group, s); e != cudaSuccess) return e;
         e = with_dtype(m.dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             const int64_t grid = std::min<int64_t>((t * m.hidden + 255) / 256, int64_t(device_sm_count()) * 8);

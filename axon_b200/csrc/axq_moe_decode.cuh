@@ -220,9 +220,12 @@ template <> struct MoeRow<F_Q2_K> {
 
 // Q3_K {hmask[32], qs[64], scales[12], d}: the fields of Q2_K with a third bit,
 // bit 4(i/2) + j of hmask[16(i%2) + l]; value = d * sc * (code - 4), sc = 6 bits
-// - 32.  The codes (0..7) go through the MMAs, 4 sc through the minimums'.
+// - 32.  The codes (0..7) go through the MMAs, 4 sc through the minimums'.  A
+// word's 16 fields and their high bits are merged into two words of 3-bit codes:
+// fields 0 and 2 at bits 0 and 4 of each byte, fields 1 and 3 likewise.
 template <> struct MoeRow<F_Q3_K> {
     uint32_t hd, sc[4], c[4], mn[2], w[4], h[4];
+    uint32_t e, o;  // fields 0, 2 and 1, 3 of the word at work
     __device__ __forceinline__ void load(const uint8_t* p, int i) {
         hd = ld_half2b(p + 108);
         uint32_t s[3];
@@ -237,9 +240,9 @@ template <> struct MoeRow<F_Q3_K> {
         const uint32_t x01 = ints_h2<32>(v01), x23 = ints_h2<32>(v23);
         mn[0] = hmul2(x01, h2_pow2(2, 2));
         mn[1] = hmul2(x23, h2_pow2(2, 2));
-        const uint32_t s01 = hmul2(x01, h2_pow2(0, -2)), s23 = hmul2(x23, h2_pow2(-4, -6));
-        const uint32_t c01 = hmul2(s01, h2_pow2(10, 10) | kNeg2), c23 = hmul2(s23, h2_pow2(10, 10) | kNeg2);
-        sc[0] = h2_low(s01); sc[1] = h2_high(s01); sc[2] = h2_low(s23); sc[3] = h2_high(s23);
+        const uint32_t s23 = hmul2(x23, h2_pow2(-4, -4));  // fields 2 and 3 stay in place (x 16)
+        const uint32_t c01 = hmul2(x01, h2_pow2(10, 10) | kNeg2), c23 = hmul2(s23, h2_pow2(10, 10) | kNeg2);
+        sc[0] = h2_low(x01); sc[1] = h2_high(x01); sc[2] = h2_low(s23); sc[3] = h2_high(s23);
         c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
         ld_words2(p + 32 + 32 * n + 16 * lh, w);
         ld_words2(p + 16 * lh, h);
@@ -248,14 +251,18 @@ template <> struct MoeRow<F_Q3_K> {
     }
     template <int MP>
     __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
-        constexpr int j = 2 * (MP % 2);
-        constexpr uint32_t m0 = 0x00030003u << (2 * j), m1 = 0x00030003u << (2 * j + 2);
-        constexpr uint32_t b0 = 0x00040004u << (2 * j), b1 = 0x00040004u << (2 * j + 2);
-        const uint32_t x = w[MP / 2], y = x >> 8, b = h[MP / 2];
-        a[0] = hfma2(lop_and_or(b << (j + 2), b0, and_or<m0, kMagic>(x)), sc[j], c[j]);
-        a[1] = hfma2(lop_and_or(b >> (6 - j), b0, and_or<m0, kMagic>(y)), sc[j], c[j]);
-        a[2] = hfma2(lop_and_or(b << (j + 3), b1, and_or<m1, kMagic>(x)), sc[j + 1], c[j + 1]);
-        a[3] = hfma2(lop_and_or(b >> (5 - j), b1, and_or<m1, kMagic>(y)), sc[j + 1], c[j + 1]);
+        if constexpr (MP % 2 == 0) {
+            // high bits 0 / 2 to bits 2 / 6 in one multiply: x * 20 puts bit 0 at bits 2 and 4 and bit 2 at bits 4 and 6;
+            // bits 4-5 (the sum of the two, never carrying into bit 6) are taken from w.  Likewise bits 1 / 3 by 10.
+            e = lop_and_or(w[MP / 2], 0x33333333u, ((h[MP / 2] & 0x05050505u) * 20u) & 0x44444444u);
+            o = lop_and_or(w[MP / 2] >> 2, 0x33333333u, ((h[MP / 2] & 0x0A0A0A0Au) * 10u) & 0x44444444u);
+        }
+        constexpr int j = 2 * (MP % 2);  // fields j, j + 1
+        constexpr uint32_t m = j ? 0x00700070u : 0x00070007u;
+        a[0] = hfma2(and_or<m, kMagic>(e), sc[j], c[j]);
+        a[1] = hfma2(and_or<m, kMagic>(e >> 8), sc[j], c[j]);
+        a[2] = hfma2(and_or<m, kMagic>(o), sc[j + 1], c[j + 1]);
+        a[3] = hfma2(and_or<m, kMagic>(o >> 8), sc[j + 1], c[j + 1]);
     }
     __device__ __forceinline__ void mins(uint32_t (&a)[2]) const { a[0] = mn[0]; a[1] = mn[1]; }
     __device__ __forceinline__ float2 scales() const {

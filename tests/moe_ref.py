@@ -57,6 +57,8 @@ def layer(x, ids, p, gate, up, down, eps):
             dh = 1.1 * dg * (np.abs(u) + du) + np.abs(silu(g)) * du + 8 * 2.0 ** -24 * np.abs(h)
             z = down.value[e] @ h
             dz = c2 * (down.size[e] @ (np.abs(h) + dh)) + np.abs(down.value[e]) @ dh
+            if eps == 2.0 ** -7:  # a bf16 result: h enters the second product as one fp16 (half a step: 2^-11 of it)
+                dz = dz + 2.0 ** -11 * (np.abs(down.value[e]) @ (np.abs(h) + dh))
             dz = dz + 2.0 ** -33 * (np.abs(h) + dh).max(initial=0) * down.size[e].sum(1)
             w = float(p[t, j])
             y[t] += w * z
