@@ -121,6 +121,8 @@ SIGNATURES = {
     "axq_moe_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "axq_moe_mlp": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp, _vp,
                                    _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "axq_moe": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp, _vp,
+                               ctypes.c_int, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "axq_axon_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_uint32)]),
     "axq_axon_info": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp]),
     "axq_axon_read": (ctypes.c_int, [_vp, ctypes.c_uint32, _vp, _sz, _vp]),

@@ -101,8 +101,10 @@ struct MoeMlp {
     int64_t gate_bytes, down_bytes;  // of all experts' packed rows
     int dtype;
     const void* x;
-    const int* ids;
-    const float* weights;
+    const float* w_router;  // null: ids and weights are given, else they are written first
+    int normalize;
+    int* ids;
+    float* weights;
     void* y;
     int64_t tokens, hidden, ffn;
     int experts, top_k;

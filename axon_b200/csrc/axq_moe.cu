@@ -35,6 +35,117 @@
 namespace axq {
 namespace {
 
+// ---- activation records -----------------------------------------------------------
+
+// Record of one row and CG with T terms: eight lines (one for each pair of MMAs:
+// [term][lane part][16 bytes]), the sums as two terms [2][lane part][8 bytes],
+// the scale.
+// One term holds fp16 and bf16 activations exactly (down to 2^-33 of the largest
+// of the 256), two hold fp32 ones to 22 bits.
+template <int T> constexpr int kRecSums = 512 * T;
+template <int T> constexpr int kRecScale = kRecSums<T> + 64;
+template <int T> constexpr int kRec = (kRecScale<T> + 4 + 63) / 64 * 64;
+__host__ __device__ __forceinline__ int rec_bytes(int terms) { return terms == 1 ? kRec<1> : kRec<2>; }
+
+// Two fp16 terms of v (already scaled): v = hi + lo within 2^-22 of it.
+__device__ __forceinline__ void split2(float v, __half& hi, __half& lo) {
+    hi = __float2half_rn(v);
+    const float r = v - __half2float(hi);
+    lo = __float2half_rn(isfinite(r) ? r : 0.0f);
+}
+
+// One warp: the record of 256 elements in s (shared memory, zero past the end)
+// for weights of format fmt.
+__device__ __forceinline__ void write_record(int fmt, int terms, const float* s, uint8_t* rec, int lane) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(s[32 * j + lane]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    // A power of two brings the largest element to [2^8, 2^9): fp16 then holds
+    // sums of 32 elements, and terms down to 2^-33 of the largest.
+    const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127 - 8, -118), 118);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    const int mp = lane >> 2, i = lane & 3;
+    __half hi[8], lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) split2(s[order_elem(fmt, 2 * mp + (k >> 2), i, k & 3)] * up, hi[k], lo[k]);
+    uint4 a;
+    memcpy(&a, hi, 16);
+    *reinterpret_cast<uint4*>(rec + mp * 64 * terms + i * 16) = a;
+    if (terms == 2) {
+        memcpy(&a, lo, 16);
+        *reinterpret_cast<uint4*>(rec + mp * 128 + 64 + i * 16) = a;
+    }
+    const int sums = order_sums(fmt), at = 512 * terms;
+    if (sums && lane < 16) {  // lane part lane / 4, slot lane % 4
+        const int n = 256 / sums, sb = order_sum(fmt, lane >> 2, lane & 3);
+        float v = 0.0f;
+        if (sb >= 0) {
+            for (int k = 0; k < n; ++k) {
+                const float x = s[sb * n + ((k + lane) & (n - 1))] * up;
+                // what the codes are multiplied with: with one term, its rounding
+                v += terms == 2 ? x : __half2float(__float2half_rn(x));
+            }
+        }
+        __half h, l;
+        split2(v, h, l);
+        reinterpret_cast<__half*>(rec + at)[lane] = h;
+        reinterpret_cast<__half*>(rec + at + 32)[lane] = l;
+    }
+    if (lane == 0) *reinterpret_cast<float*>(rec + at + 64) = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// Records of rows of x (or of the hidden activations).
+struct RecordArgs {
+    int fmt, terms;
+    int64_t rows, cols;
+    int ncg;
+    uint8_t* rec;
+    const int* need;  // rows whose expert id is out of range are skipped; null: none
+    int experts;
+    int* clear;       // counters of the kernels behind this one, set to 0
+    int nclear;
+};
+
+// Record `it` (row-major over rows and CGs) by one warp, through its 256 floats.
+template <typename T>
+__device__ __forceinline__ void record_of(const RecordArgs& a, const T* x, int64_t it, float* buf, int lane) {
+    if (it >= a.rows * a.ncg) return;
+    const int64_t r = it / a.ncg;
+    const int cg = static_cast<int>(it - r * a.ncg);
+    if (a.need && static_cast<unsigned>(a.need[r]) >= static_cast<unsigned>(a.experts)) return;
+    const int64_t k0 = static_cast<int64_t>(cg) * 256;
+    const T* xr = x + r * a.cols;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int64_t k = k0 + 32 * j + lane;
+        buf[32 * j + lane] = k < a.cols ? Elem<T>::get(xr[k]) : 0.0f;
+    }
+    __syncwarp();
+    write_record(a.fmt, a.terms, buf, a.rec + it * rec_bytes(a.terms), lane);
+}
+
+constexpr int kPrepWarps = 8;
+
+// Records of all rows; block 0 also makes the plan when ids are given.
+template <typename T>
+__global__ void __launch_bounds__(32 * kPrepWarps) moe_prep_kernel(const T* __restrict__ x, RecordArgs a, MoePlan plan) {
+    __shared__ float buf[kPrepWarps][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (plan.ids && blockIdx.x == 0) {
+        moe_make_plan(plan);
+        return;
+    }
+    if (plan.err && !plan.ids && blockIdx.x == 0 && threadIdx.x == 0) *plan.err = 0;
+    const int64_t b = blockIdx.x - (plan.ids ? 1 : 0);
+    for (int64_t c = b * (32 * kPrepWarps) + threadIdx.x; c < a.nclear; c += static_cast<int64_t>(gridDim.x) * (32 * kPrepWarps))
+        a.clear[c] = 0;
+    record_of(a, x, b * kPrepWarps + warp, buf[warp], lane);
+}
+
 // ---- router ---------------------------------------------------------------------
 
 constexpr int kRouteCtas = 8, kRouteWarps = 16, kRouteTokens = 4;
@@ -50,11 +161,25 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
 template <typename T>
 __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRouteWarps)
     moe_route_kernel(const T* __restrict__ x, const float* __restrict__ w, int* __restrict__ ids, float* __restrict__ wt,
-                     int64_t tokens, int experts, int top_k, int64_t hidden, int slices, int normalize, bool vec) {
+                     int64_t tokens, int experts, int top_k, int64_t hidden, int slices, int normalize, bool vec,
+                     RecordArgs records, int* err) {
     extern __shared__ float logits[];  // [slice][kRouteTokens][experts], of the cluster's first CTA
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int64_t t0 = static_cast<int64_t>(blockIdx.x / kRouteCtas) * kRouteTokens;
+    if (t0 >= tokens) {
+        // clusters past the tokens': the layer's activation records, which do not wait for the choice of experts
+        __shared__ float buf[kRouteWarps][256];
+        const int first = static_cast<int>((tokens + kRouteTokens - 1) / kRouteTokens) * kRouteCtas;
+        const int b = static_cast<int>(blockIdx.x) - first;
+        pdl_wait();
+        pdl_launch_dependents();
+        if (b == 0 && threadIdx.x == 0) *err = 0;
+        for (int c = b * (32 * kRouteWarps) + threadIdx.x; c < records.nclear; c += (gridDim.x - first) * (32 * kRouteWarps))
+            records.clear[c] = 0;
+        record_of(records, x, static_cast<int64_t>(b) * kRouteWarps + warp, buf[warp], lane);
+        return;
+    }
     const int nt = static_cast<int>(min64(kRouteTokens, tokens - t0));
     cluster_sync_all();  // the first CTA's shared memory is there
     pdl_wait();
@@ -166,113 +291,15 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
     }
 }
 
-// ---- plan and activation records ---------------------------------------------------
-
-// Record of one row and CG with T terms: eight lines (one for each pair of MMAs:
-// [term][lane part][16 bytes]), the sums as two terms [2][lane part][8 bytes],
-// the scale.
-// One term holds fp16 and bf16 activations exactly (down to 2^-33 of the largest
-// of the 256), two hold fp32 ones to 22 bits.
-template <int T> constexpr int kRecSums = 512 * T;
-template <int T> constexpr int kRecScale = kRecSums<T> + 64;
-template <int T> constexpr int kRec = (kRecScale<T> + 4 + 63) / 64 * 64;
-
-// Two fp16 terms of v (already scaled): v = hi + lo within 2^-22 of it.
-__device__ __forceinline__ void split2(float v, __half& hi, __half& lo) {
-    hi = __float2half_rn(v);
-    const float r = v - __half2float(hi);
-    lo = __float2half_rn(isfinite(r) ? r : 0.0f);
-}
-
-// One warp: the record of 256 elements in s (shared memory, zero past the end).
-template <int F, int T>
-__device__ __forceinline__ void write_record(const float* s, uint8_t* rec, int lane) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(s[32 * j + lane]));
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    // A power of two brings the largest element to [2^8, 2^9): fp16 then holds
-    // sums of 32 elements, and terms down to 2^-33 of the largest.
-    const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127 - 8, -118), 118);
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const int mp = lane >> 2, i = lane & 3;
-    __half hi[8], lo[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int el = Order<F>::elem(2 * mp + (k >> 2), i, k & 3);
-        split2(s[el] * up, hi[k], lo[k]);
-    }
-    uint4 a;
-    memcpy(&a, hi, 16);
-    *reinterpret_cast<uint4*>(rec + mp * 64 * T + i * 16) = a;
-    if constexpr (T == 2) {
-        memcpy(&a, lo, 16);
-        *reinterpret_cast<uint4*>(rec + mp * 64 * T + 64 + i * 16) = a;
-    }
-    if constexpr (Order<F>::SUMS > 0) {
-        if (lane < 16) {  // lane part lane / 4, slot lane % 4
-            constexpr int N = 256 / Order<F>::SUMS;
-            const int sb = Order<F>::sum(lane >> 2, lane & 3);
-            float v = 0.0f;
-            if (sb >= 0) {
-                for (int k = 0; k < N; ++k) {
-                    const float x = s[sb * N + ((k + lane) & (N - 1))];
-                    // what the codes are multiplied with: with one term, its rounding
-                    v += T == 2 ? x : __half2float(__float2half_rn(x * up));
-                }
-            }
-            __half h, l;
-            split2(T == 2 ? v * up : v, h, l);
-            reinterpret_cast<__half*>(rec + kRecSums<T>)[lane] = h;
-            reinterpret_cast<__half*>(rec + kRecSums<T> + 32)[lane] = l;
-        }
-    }
-    if (lane == 0)
-        *reinterpret_cast<float*>(rec + kRecScale<T>) = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-}
-
-constexpr int kPrepWarps = 8;
-
-// Rows of x (or h) -> records; block 0 also makes the plan when ids are given.
-// need (may be null): rows whose expert id is out of range are skipped.
-template <int F, int TERMS, typename T>
-__global__ void __launch_bounds__(32 * kPrepWarps)
-    moe_prep_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int ncg, uint8_t* __restrict__ rec,
-                    const int* __restrict__ need, int experts, MoePlan plan) {
-    __shared__ float buf[kPrepWarps][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_launch_dependents();
-    if (plan.ids && blockIdx.x == 0) {
-        moe_make_plan(plan);
-        return;
-    }
-    const int64_t b = blockIdx.x - (plan.ids ? 1 : 0);
-    const int64_t it = b * kPrepWarps + warp;
-    if (it >= rows * ncg) return;
-    const int64_t r = it / ncg;
-    const int cg = static_cast<int>(it - r * ncg);
-    if (need && static_cast<unsigned>(need[r]) >= static_cast<unsigned>(experts)) return;
-    const int64_t k0 = static_cast<int64_t>(cg) * 256;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int64_t k = k0 + 32 * j + lane;
-        buf[warp][32 * j + lane] = k < cols ? Elem<T>::get(x[r * cols + k]) : 0.0f;
-    }
-    __syncwarp();
-    write_record<F, TERMS>(buf[warp], rec + it * kRec<TERMS>, lane);
-}
-
 // ---- experts -------------------------------------------------------------------------
 
 constexpr int kConsumers = 8;
-constexpr int kMoeThreads = (kConsumers + 1) * 32;
+constexpr int kMoeThreads = (kConsumers + 2) * 32;  // and the producer and the finisher
 constexpr int kMoeStages = 8;  // most
 
 struct MoeBars {
     uint64_t full[kMoeStages], empty[kMoeStages];
-    uint64_t sums[2];  // the partial sums of a round are written
+    uint64_t sums[2], joined[2];  // a round's partial sums are written, and joined
     int abort;
 };
 
@@ -292,8 +319,25 @@ struct ExpertArgs {
     int64_t rec_row;       // bytes of a record row
     int rec_token;         // a pair's record row is its token's, else its own
     float* out;            // [pair][rows]
-    MoePlan plan;
+    MoePlan plan;          // ids set: few choices, planned by every CTA
+    // With few choices whoever finishes the last part of something finishes it:
+    // the records of 256 hidden activations (gate and up), or 32 columns of y
+    // (down).  counters count the parts done.
+    int* counters;
+    int h_fmt, h_terms, h_ncg;
+    uint8_t* h_rec;
+    const float* wt;
+    void* y;
+    int y_dtype;
+    int64_t tokens;
     int* err;
+};
+
+// The plan as a CTA uses it, from the plan kernel's memory or its own.
+struct PlanView {
+    const int4* groups;
+    const int2* entries;
+    int ngroups;
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -491,6 +535,29 @@ __device__ __forceinline__ bool moe_wait(uint64_t* bar, uint32_t parity, MoeBars
     return ok;
 }
 
+// sum_j p[t][j] z[t top_k + j][c], j in order; ids out of range add nothing.
+// Loads of four choices are in flight together (z has a row for every choice,
+// written or not).
+__device__ __forceinline__ float moe_combined(const float* z, const int* ids, const float* wt, int64_t t, int64_t c,
+                                              int64_t hidden, int top_k, int experts) {
+    float v = 0.0f;
+    for (int j0 = 0; j0 < top_k; j0 += 4) {
+        int id[4];
+        float w[4], x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t p = t * top_k + min(j0 + j, top_k - 1);
+            id[j] = j0 + j < top_k ? __ldg(ids + p) : -1;
+            w[j] = __ldg(wt + p);
+            x[j] = __ldcg(z + p * hidden + c);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (static_cast<unsigned>(id[j]) < static_cast<unsigned>(experts)) v = fmaf(w[j], x[j], v);
+    }
+    return v;
+}
+
 // Row (of the expert) of tile `tile` and row r of unit `unit`.
 __device__ __forceinline__ int64_t stage_row(const ExpertArgs& a, int unit, int tile, int r) {
     return a.gate_up ? static_cast<int64_t>(unit) * 16 + r : static_cast<int64_t>(unit) * 32 + 16 * tile + r;
@@ -509,33 +576,85 @@ struct MoeRound {
     }
 };
 
-// Joins the warps' partial sums (rb) of a round and writes its results.
+// Joins the warps' partial sums (rb) of a round and writes its results (one warp).
 template <int kTok>
-__device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb, const MoeRound& rd, int tid) {
-    const int4 gd = a.plan.groups[rd.grp];
+__device__ __forceinline__ void moe_results(const ExpertArgs& a, const PlanView& pl, const float* rb, const MoeRound& rd,
+                                            int lane) {
+    const int4 gd = pl.groups[rd.grp];
     const int rs = a.gate_up ? 4 : 5;  // log2 of a unit's rows
-    for (int o = tid; o < (a.slots * kTok) << rs; o += kConsumers * 32) {
-        const int rr = o & ((1 << rs) - 1), t = (o >> rs) & (kTok - 1), un = (o >> rs) / kTok;
-        const int64_t row = (static_cast<int64_t>(rd.t0 + un) << rs) + rr;
-        if (rd.t0 + un >= a.tiles || row >= a.rows || t >= gd.z) continue;
-        float v[2] = {0.0f, 0.0f};
-        const float* q = rb + (un * a.wps * 2 * kTok + t) * 16;
+    const int outputs = gd.z << rs;    // of a unit
+    for (int un = 0; un < a.slots && rd.t0 + un < a.tiles; ++un) {
+#pragma unroll 2
+        for (int o = lane; o < outputs; o += 32) {
+            const int rr = o & ((1 << rs) - 1), t = o >> rs;
+            const int64_t row = (static_cast<int64_t>(rd.t0 + un) << rs) + rr;
+            float v[2] = {0.0f, 0.0f};
+            const float* q = rb + (un * a.wps * 2 * kTok + t) * 16;
+            if (a.gate_up) {
+                for (int w = 0; w < a.wps; ++w) {
+                    v[0] += q[w * 2 * kTok * 16 + rr];
+                    v[1] += q[(w * 2 + 1) * kTok * 16 + rr];
+                }
+            } else {
+                q += (rr >> 4) * kTok * 16 + (rr & 15);
+                for (int w = 0; w < a.wps; ++w) v[0] += q[w * 2 * kTok * 16];
+            }
+            const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
+            if (row < a.rows) a.out[static_cast<int64_t>(pl.entries[gd.y + t].x) * a.rows + row] = z;
+        }
+    }
+}
+
+__device__ __forceinline__ void store_y(const ExpertArgs& a, int64_t at, float v) {
+    if (a.y_dtype == AXQ_DT_F32) static_cast<float*>(a.y)[at] = v;
+    else if (a.y_dtype == AXQ_DT_F16) static_cast<__half*>(a.y)[at] = Elem<__half>::put(v);
+    else static_cast<__nv_bfloat16*>(a.y)[at] = Elem<__nv_bfloat16>::put(v);
+}
+
+// After a round's results, with few choices: counts the units done, and finishes
+// what this round completed (one warp).
+__device__ __forceinline__ void moe_finish(const ExpertArgs& a, const PlanView& pl, const MoeRound& rd, float* buf, int lane) {
+    for (int un = 0; un < a.slots && rd.t0 + un < a.tiles; ++un) {
+        const int unit = rd.t0 + un;
+        __threadfence();  // the results, before the count
+        __syncwarp();
+        int done = 0;
+        if (lane == 0) {
+            const int at = a.gate_up ? rd.grp * a.h_ncg + (unit >> 4) : unit;
+            const int parts = a.gate_up ? min(16, a.tiles - (unit & ~15)) : pl.ngroups;
+            done = atomicAdd(a.counters + at, 1) == parts - 1;
+        }
+        if (!__shfl_sync(0xFFFFFFFFu, done, 0)) continue;
+        __threadfence();  // the count, before the others' results
         if (a.gate_up) {
-            for (int w = 0; w < a.wps; ++w) {
-                v[0] += q[w * 2 * kTok * 16 + rr];
-                v[1] += q[(w * 2 + 1) * kTok * 16 + rr];
+            // the records of the group's 256 hidden activations
+            const int4 gd = pl.groups[rd.grp];
+            const int cg = unit >> 4;
+            for (int t = 0; t < gd.z; ++t) {
+                const int64_t p = pl.entries[gd.y + t].x;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t k = cg * 256 + 32 * j + lane;
+                    buf[32 * j + lane] = k < a.rows ? __ldcg(a.out + p * a.rows + k) : 0.0f;
+                }
+                __syncwarp();
+                write_record(a.h_fmt, a.h_terms, buf, a.h_rec + (p * a.h_ncg + cg) * rec_bytes(a.h_terms), lane);
+                __syncwarp();
             }
         } else {
-            q += (rr >> 4) * kTok * 16 + (rr & 15);
-            for (int w = 0; w < a.wps; ++w) v[0] += q[w * 2 * kTok * 16];
+            const int64_t c = static_cast<int64_t>(unit) * 32 + lane;
+            if (c < a.rows) {
+#pragma unroll 2
+                for (int64_t t = 0; t < a.tokens; ++t)
+                    store_y(a, t * a.rows + c, moe_combined(a.out, a.plan.ids, a.wt, t, c, a.rows, a.plan.top_k, a.plan.experts));
+            }
+            __syncwarp();
         }
-        const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
-        a.out[static_cast<int64_t>(a.plan.entries[gd.y + t].x) * a.rows + row] = z;
     }
 }
 
 template <int F, int T, int NB>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const ExpertArgs a) {
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid_constant__ ExpertArgs a) {
     using C = Cols<T>;
     constexpr int CGB = moe_cg_bytes<F>();
     constexpr int kTok = C::kTokens * NB;
@@ -550,17 +669,31 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
             mbar_init(&bars.full[s], 1);
             mbar_init(&bars.empty[s], kConsumers);
         }
-        mbar_init(&bars.sums[0], kConsumers);
-        mbar_init(&bars.sums[1], kConsumers);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bars.sums[s], kConsumers);
+            mbar_init(&bars.joined[s], 1);
+        }
         bars.abort = 0;
         fence_mbar_init();
     }
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int ngroups = *a.plan.ngroups;
+    __shared__ MoeFewPlan few;
+    __shared__ int last[4];
+    PlanView pl{a.plan.groups, a.plan.entries, 0};
+    if (a.plan.ids) {
+        moe_few_plan(few, a.plan);
+        pl = PlanView{few.groups, few.entries, few.ngroups};
+        if (pl.ngroups == 0 && !a.gate_up)  // no token chose an expert of this layer
+            for (int64_t o = static_cast<int64_t>(blockIdx.x) * kMoeThreads + threadIdx.x; o < a.tokens * a.rows;
+                 o += static_cast<int64_t>(gridDim.x) * kMoeThreads)
+                store_y(a, o, 0.0f);
+    } else {
+        pl.ngroups = *a.plan.ngroups;
+    }
     const int per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group; all fit 32 bits (checked on the host)
-    const int rounds = ngroups * per;
+    const int rounds = pl.ngroups * per;
     const int lo = static_cast<int>(static_cast<int64_t>(rounds) * blockIdx.x / gridDim.x);
     const int hi = static_cast<int>(static_cast<int64_t>(rounds) * (blockIdx.x + 1) / gridDim.x);
     MoeRound rd{lo / per, 0};
@@ -575,7 +708,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
         int64_t issued = 0;
         for (int n = lo; n < hi && ok; ++n, rd.next(a)) {
             const int t0 = rd.t0;
-            const int64_t expert = a.plan.groups[rd.grp].x;
+            const int64_t expert = pl.groups[rd.grp].x;
             for (int step = 0; step < ksteps * (2 / TL); ++step) {
                 const int k = step / (2 / TL), tile = TL == 2 ? lane >> 4 : step & 1;
                 ok = moe_wait(&bars.empty[s], par ^ 1, &bars, a.err);
@@ -629,27 +762,39 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
         return;
     }
 
+    constexpr int kSums = kConsumers * 2 * kTok * 16;
+    if (warp > kConsumers) {
+        // The finisher joins each round's sums beside the consumers, which go on; it needs no registers that the SM has
+        // not left over (18 and 20 warps share its schedulers alike).
+        for (int q = 0; q < hi - lo; ++q, rd.next(a)) {
+            if (!moe_wait(&bars.sums[q & 1], (q >> 1) & 1, &bars, a.err)) break;
+            moe_results<kTok>(a, pl, red + (q & 1) * kSums, rd, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.joined[q & 1]);
+            if (a.plan.ids) moe_finish(a, pl, rd, red + 2 * kSums, lane);
+        }
+        return;
+    }
+
     const int g = lane >> 2, i = lane & 3;
     const int u = warp / a.wps, col = warp - u * a.wps;
-    constexpr int kSums = kConsumers * 2 * kTok * 16;
     int s = 0;
     uint32_t par = 0;
     bool ok = true;
-    MoeRound before{};
-    for (int q = 0; q < hi - lo; ++q) {
+    for (int q = 0; q < hi - lo; ++q, rd.next(a)) {
         const int unit = rd.t0 + u;
-        const int4 gd = a.plan.groups[rd.grp];  // expert, first entry, number of entries
+        const int4 gd = pl.groups[rd.grp];  // expert, first entry, number of entries
         // this lane's B column, and the scales of its sums' columns (columns past the group's end: its first token's)
         const uint8_t *rec0[NB], *scale0[NB][C::kOwn];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const int t = n * C::kTokens + C::token(g);
-            const int2 e = a.plan.entries[gd.y + (t < gd.z ? t : 0)];
+            const int2 e = pl.entries[gd.y + (t < gd.z ? t : 0)];
             rec0[n] = a.rec + (a.rec_token ? e.y : e.x) * a.rec_row + C::offset(g, i);
 #pragma unroll
             for (int v = 0; v < C::kOwn; ++v) {
                 const int ts = n * C::kTokens + C::own(i, v);
-                const int2 es = a.plan.entries[gd.y + (ts < gd.z ? ts : 0)];
+                const int2 es = pl.entries[gd.y + (ts < gd.z ? ts : 0)];
                 scale0[n][v] = a.rec + (a.rec_token ? es.y : es.x) * a.rec_row + kRecScale<T>;
             }
         }
@@ -712,15 +857,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
                 }
             }
         }
-        // The round before is joined only now, when its slowest warp is long done.  Two buffers of sums are enough: a
-        // warp writes this round's after its share of the round before, so whoever waits for this round's sums knows
-        // that the other buffer has been read.
-        if (q > 0) {
-            if (ok) ok = moe_wait(&bars.sums[(q - 1) & 1], ((q - 1) >> 1) & 1, &bars, a.err);
-            if (ok) moe_results<kTok>(a, red + ((q - 1) & 1) * kSums, before, threadIdx.x);
-        }
-        before = rd;
-        rd.next(a);
+        // the sums of two rounds before, in the same buffer, have been joined
+        if (ok && q > 1) ok = moe_wait(&bars.joined[q & 1], ((q >> 1) - 1) & 1, &bars, a.err);
         float* rb = red + (q & 1) * kSums;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -735,14 +873,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const Expert
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.sums[q & 1]);
     }
-    if (hi > lo) {
-        const int q = hi - lo - 1;
-        if (ok) ok = moe_wait(&bars.sums[q & 1], (q >> 1) & 1, &bars, a.err);
-        if (ok) moe_results<kTok>(a, red + (q & 1) * kSums, before, threadIdx.x);
-    }
 }
 
-// y[t][c] = sum_j p[t][j] z[t top_k + j][c], j in order; ids out of range add nothing.
 template <typename T>
 __global__ void __launch_bounds__(256) moe_combine_kernel(const float* __restrict__ z, const int* __restrict__ ids,
                                                           const float* __restrict__ wt, T* __restrict__ y, int64_t tokens,
@@ -753,12 +885,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const float* __restric
     for (int64_t o = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; o < n;
          o += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t t = o / hidden, c = o - t * hidden;
-        float v = 0.0f;
-        for (int j = 0; j < top_k; ++j) {
-            const int64_t p = t * top_k + j;
-            if (static_cast<unsigned>(ids[p]) < static_cast<unsigned>(experts)) v = fmaf(wt[p], z[p * hidden + c], v);
-        }
-        y[o] = Elem<T>::put(v);
+        y[o] = Elem<T>::put(moe_combined(z, ids, wt, t, c, hidden, top_k, experts));
     }
 }
 
@@ -802,7 +929,8 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     a.rs = (cgs * CGB + 15 + 4 + 15) / 16 * 16;
     while (a.rs % 128 != 16) a.rs += 16;
     a.stage_bytes = a.slots * 16 * kStageTiles<F, NB> * a.rs;
-    const int red = 2 * kConsumers * 2 * (8 / T) * NB * 16 * 4;
+    // sums of two rounds, and with few choices 256 hidden activations on their way into a record
+    const int red = 2 * kConsumers * 2 * (8 / T) * NB * 16 * 4 + (a.plan.ids && a.gate_up ? 1024 : 0);
     const int budget = 112 * 1024 - 512 - red;  // two CTAs per SM
     a.stages = std::min(kMoeStages, budget / a.stage_bytes);
     int per_sm = 2;
@@ -830,18 +958,15 @@ cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int terms
 }
 
 template <typename T>
-cudaError_t launch_prep(int fmt, int terms, const T* x, int64_t rows, int64_t cols, uint8_t* rec, const int* need,
-                        int experts, const MoePlan& plan, cudaStream_t s) {
-    const int ncg = static_cast<int>((cols + 255) / 256);
-    const int64_t grid = (rows * ncg + kPrepWarps - 1) / kPrepWarps + (plan.ids ? 1 : 0);
-    return with_moe_fmt(fmt, [&](auto f) {
-        constexpr int F = decltype(f)::value;
-        auto k = terms == 1 ? moe_prep_kernel<F, 1, T> : moe_prep_kernel<F, 2, T>;
-        cudaError_t e = launch_pdl(k, dim3(static_cast<unsigned>(grid)), dim3(32 * kPrepWarps), 0, s, x, rows, cols, ncg, rec,
-                                   need, experts, plan);
-        return e == cudaSuccess ? cudaGetLastError() : e;
-    });
+cudaError_t launch_prep(const T* x, const RecordArgs& a, const MoePlan& plan, cudaStream_t s) {
+    const int64_t grid = (a.rows * a.ncg + kPrepWarps - 1) / kPrepWarps + (plan.ids ? 1 : 0);
+    cudaError_t e = launch_pdl(moe_prep_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(32 * kPrepWarps), 0, s, x, a, plan);
+    return e == cudaSuccess ? cudaGetLastError() : e;
 }
+
+// One warp writes the hidden records of a group and one the columns of y: more
+// tokens are faster with kernels of their own.
+constexpr int64_t kMoeFewTokens = 8;
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -849,7 +974,8 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 int64_t pass_tokens(int top_k) { return std::max<int64_t>(1, kMoePairs / top_k); }
 
 struct MoeSpace {
-    size_t plan, rec_x, rec_h, h, z, total;
+    size_t plan, counters, rec_x, rec_h, h, z, total;
+    int64_t ncounters;
 };
 
 MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
@@ -862,12 +988,33 @@ MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
         return r;
     };
     w.plan = take(kMoePlanBytes);
+    w.ncounters = kMoeFew * ((ffn + 255) / 256) + (hidden + 31) / 32;
+    w.counters = take(static_cast<size_t>(w.ncounters) * 4);
     w.rec_x = take(static_cast<size_t>(t) * ((hidden + 255) / 256) * kRec<2>);
     w.rec_h = take(static_cast<size_t>(p) * ((ffn + 255) / 256) * kRec<2>);
     w.h = take(static_cast<size_t>(p) * ffn * 4);
     w.z = take(static_cast<size_t>(p) * hidden * 4);
     w.total = at;
     return w;
+}
+
+cudaError_t launch_route(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens, int experts,
+                         int top_k, int64_t hidden, int normalize, const RecordArgs& records, int* err, cudaStream_t s) {
+    return with_dtype(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        const bool vec = hidden % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                         reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
+        const int64_t clusters = (tokens + kRouteTokens - 1) / kRouteTokens;
+        const int64_t nrec = records.rows * records.ncg;
+        const int64_t extra = (nrec + kRouteWarps * kRouteCtas - 1) / (kRouteWarps * kRouteCtas);  // clusters
+        int slices = 1;
+        while (2 * slices * experts <= kRouteCtas * kRouteWarps && hidden >= 256 * slices) slices *= 2;
+        const size_t smem = static_cast<size_t>(slices) * kRouteTokens * experts * 4;
+        cudaError_t e = launch_pdl(moe_route_kernel<T>, dim3(static_cast<unsigned>((clusters + extra) * kRouteCtas)),
+                                   dim3(32 * kRouteWarps), smem, s, static_cast<const T*>(x), w, ids, weights, tokens,
+                                   experts, top_k, hidden, slices, normalize, vec, records, err);
+        return e == cudaSuccess ? cudaGetLastError() : e;
+    });
 }
 
 }  // namespace
@@ -878,30 +1025,28 @@ size_t moe_workspace_bytes(int64_t tokens, int top_k, int64_t hidden, int64_t ff
 
 cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens,
                                int experts, int top_k, int64_t hidden, int normalize, cudaStream_t s) {
-    return with_dtype(dtype, [&](auto* tag) {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        const bool vec = hidden % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
-                         reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;
-        const int64_t clusters = (tokens + kRouteTokens - 1) / kRouteTokens;
-        int slices = 1;
-        while (2 * slices * experts <= kRouteCtas * kRouteWarps && hidden >= 256 * slices) slices *= 2;
-        const size_t smem = static_cast<size_t>(slices) * kRouteTokens * experts * 4;
-        cudaError_t e = launch_pdl(moe_route_kernel<T>, dim3(static_cast<unsigned>(clusters * kRouteCtas)),
-                                   dim3(32 * kRouteWarps), smem, s, static_cast<const T*>(x), w, ids, weights, tokens,
-                                   experts, top_k, hidden, slices, normalize, vec);
-        return e == cudaSuccess ? cudaGetLastError() : e;
-    });
+    return launch_route(dtype, x, w, ids, weights, tokens, experts, top_k, hidden, normalize, RecordArgs{}, nullptr, s);
 }
 
+// Passes of up to kMoePairs choices.  Few choices (kMoeFew) take three kernels:
+// router (if given) and records of x, gate and up with the records of the hidden
+// activations, down with y; more take a plan and separate kernels for the hidden
+// records and for y, whose cost is small beside the experts'.
 cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s) {
     const MoeSpace w = moe_space(m.tokens, m.top_k, m.hidden, m.ffn);
     auto* base = static_cast<uint8_t*>(ws);
     const int64_t step = pass_tokens(m.top_k);
     const int size = host_dtype_size(m.dtype);
+    // 16-bit x is one term; so are the hidden activations of a bf16 result, whose own rounding is 8 times theirs
+    const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = m.dtype == AXQ_DT_BF16 ? 1 : 2;
+    const bool few = m.tokens <= kMoeFewTokens && m.tokens * m.top_k <= kMoeFew;
+    if (m.w_router && !few) {
+        cudaError_t e = moe_route_dispatch(m.dtype, m.x, m.w_router, m.ids, m.weights, m.tokens, m.experts, m.top_k, m.hidden,
+                                           m.normalize, s);
+        if (e != cudaSuccess) return e;
+    }
     for (int64_t t0 = 0; t0 < m.tokens; t0 += step) {
         const int64_t t = std::min(step, m.tokens - t0), p = t * m.top_k;
-        // 16-bit x is one term; so are the hidden activations of a bf16 result, whose own rounding is 8 times theirs
-        const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = m.dtype == AXQ_DT_BF16 ? 1 : 2;
         const int group = terms_x == 1 || p > 4 * m.experts ? 8 : 4;
         MoePlan plan = moe_plan_at(base + w.plan);
         plan.ids = m.ids + t0 * m.top_k;
@@ -910,19 +1055,33 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         plan.group = group;
         plan.top_k = m.top_k;
         plan.err = t0 == 0 ? err : nullptr;
-        const MoePlan made = [&] {
-            MoePlan q = plan;
-            q.ids = nullptr;
-            return q;
-        }();
+        MoePlan made = plan;  // as the kernels behind the plan see it
+        if (!few) made.ids = nullptr;
         const void* x = static_cast<const uint8_t*>(m.x) + t0 * m.hidden * size;
         void* y = static_cast<uint8_t*>(m.y) + t0 * m.hidden * size;
         float* h = reinterpret_cast<float*>(base + w.h);
         float* z = reinterpret_cast<float*>(base + w.z);
-        cudaError_t e = with_dtype(m.dtype, [&](auto* tag) {
-            using T = std::remove_pointer_t<decltype(tag)>;
-            return launch_prep<T>(m.fmt, terms_x, static_cast<const T*>(x), t, m.hidden, base + w.rec_x, nullptr, m.experts, plan, s);
-        });
+        int* counters = reinterpret_cast<int*>(base + w.counters);
+        RecordArgs rx{};
+        rx.fmt = m.fmt;
+        rx.terms = terms_x;
+        rx.rows = t;
+        rx.cols = m.hidden;
+        rx.ncg = static_cast<int>((m.hidden + 255) / 256);
+        rx.rec = base + w.rec_x;
+        rx.clear = counters;
+        rx.nclear = few ? static_cast<int>(w.ncounters) : 0;
+        cudaError_t e;
+        if (m.w_router && few) {
+            e = launch_route(m.dtype, x, m.w_router, m.ids, m.weights, t, m.experts, m.top_k, m.hidden, m.normalize, rx, err, s);
+        } else {
+            MoePlan first = plan;
+            if (few) first.ids = nullptr;  // records only
+            e = with_dtype(m.dtype, [&](auto* tag) {
+                using T = std::remove_pointer_t<decltype(tag)>;
+                return launch_prep<T>(static_cast<const T*>(x), rx, first, s);
+            });
+        }
         if (e != cudaSuccess) return e;
         ExpertArgs a{};
         a.w[0] = static_cast<const uint8_t*>(m.w_gate);
@@ -933,32 +1092,54 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.w_bytes = m.gate_bytes;
         a.rows = m.ffn;
         a.gate_up = 1;
-        a.rec = base + w.rec_x;
-        a.rec_row = (m.hidden + 255) / 256 * (terms_x == 1 ? kRec<1> : kRec<2>);
+        a.rec = rx.rec;
+        a.rec_row = static_cast<int64_t>(rx.ncg) * rec_bytes(terms_x);
         a.rec_token = 1;
         a.out = h;
         a.plan = made;
+        a.counters = counters;
+        a.h_fmt = m.fmt_down;
+        a.h_terms = terms_h;
+        a.h_ncg = static_cast<int>((m.ffn + 255) / 256);
+        a.h_rec = base + w.rec_h;
         a.err = err;
         if (e = launch_experts(m.fmt, a, m.hidden, terms_x, group, s); e != cudaSuccess) return e;
-        e = launch_prep<float>(m.fmt_down, terms_h, h, p, m.ffn, base + w.rec_h, plan.ids, m.experts, made, s);
-        if (e != cudaSuccess) return e;
+        if (!few) {
+            RecordArgs rh{};
+            rh.fmt = m.fmt_down;
+            rh.terms = terms_h;
+            rh.rows = p;
+            rh.cols = m.ffn;
+            rh.ncg = a.h_ncg;
+            rh.rec = a.h_rec;
+            rh.need = plan.ids;
+            rh.experts = m.experts;
+            made.err = nullptr;
+            if (e = launch_prep<float>(h, rh, made, s); e != cudaSuccess) return e;
+        }
         a.w[0] = a.w[1] = static_cast<const uint8_t*>(m.w_down);
         a.sc[0] = a.sc[1] = m.s_down;
         a.rb = m.ffn;
         a.w_bytes = m.down_bytes;
         a.rows = m.hidden;
         a.gate_up = 0;
-        a.rec = base + w.rec_h;
-        a.rec_row = (m.ffn + 255) / 256 * (terms_h == 1 ? kRec<1> : kRec<2>);
+        a.rec = a.h_rec;
+        a.rec_row = static_cast<int64_t>(a.h_ncg) * rec_bytes(terms_h);
         a.rec_token = 0;
         a.out = z;
+        a.counters = counters + kMoeFew * a.h_ncg;
+        a.wt = m.weights + t0 * m.top_k;
+        a.y = y;
+        a.y_dtype = m.dtype;
+        a.tokens = t;
         if (e = launch_experts(m.fmt_down, a, m.ffn, terms_h, group, s); e != cudaSuccess) return e;
+        if (few) continue;
         e = with_dtype(m.dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             const int64_t grid = std::min<int64_t>((t * m.hidden + 255) / 256, int64_t(device_sm_count()) * 8);
             cudaError_t r = launch_pdl(moe_combine_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s,
-                                       static_cast<const float*>(z), plan.ids, m.weights + t0 * m.top_k, static_cast<T*>(y),
-                                       t, m.hidden, m.top_k, m.experts);
+                                       static_cast<const float*>(z), static_cast<const int*>(plan.ids), a.wt, static_cast<T*>(y), t, m.hidden, m.top_k,
+                                       m.experts);
             return r == cudaSuccess ? cudaGetLastError() : r;
         });
         if (e != cudaSuccess) return e;

@@ -8,6 +8,7 @@
 namespace axq {
 
 constexpr int kMoePairs = 512;     // choices of one pass, at most
+constexpr int kMoeFew = 64;        // choices that each CTA plans for itself, at most
 constexpr int kMoeExperts = 1024;  // experts, at most
 
 struct MoePlan {
@@ -19,6 +20,48 @@ struct MoePlan {
     int top_k;
     int* err;        // status word to clear, or null
 };
+
+// The plan of few choices, made by every CTA in its shared memory (no kernel
+// has to come between the choice of experts and their products).
+struct MoeFewPlan {
+    int4 groups[kMoeFew];
+    int2 entries[kMoeFew];
+    int ids[kMoeFew], rank[kMoeFew];
+    int ngroups;
+};
+
+// All threads of the block (at least kMoeFew) call it.
+__device__ __forceinline__ void moe_few_plan(MoeFewPlan& p, const MoePlan& m) {
+    const int tid = threadIdx.x;
+    if (tid < kMoeFew) p.ids[tid] = tid < m.npairs ? m.ids[tid] : -1;
+    __syncthreads();
+    const int mine = tid < kMoeFew ? p.ids[tid] : -1;
+    const bool valid = static_cast<unsigned>(mine) < static_cast<unsigned>(m.experts);
+    int before = 0, rank = 0, total = 0;
+    if (valid) {
+        for (int q = 0; q < m.npairs; ++q) {
+            const int e = p.ids[q];
+            before += (e >= 0 && e < mine) || (e == mine && q < tid) ? 1 : 0;
+            rank += e == mine && q < tid ? 1 : 0;
+            total += e == mine ? 1 : 0;
+        }
+    }
+    if (tid < kMoeFew) p.rank[tid] = valid ? rank % m.group : -1;
+    __syncthreads();
+    int starts = 0;  // groups that begin before this pair, and in all
+    int all = 0;
+    for (int q = 0; q < m.npairs; ++q) {
+        const int e = p.ids[q], s = p.rank[q] == 0 ? 1 : 0;
+        all += s;
+        starts += s && (e < mine || (e == mine && q < tid)) ? 1 : 0;
+    }
+    if (valid) {
+        p.entries[before] = make_int2(tid, tid / m.top_k);
+        if (rank % m.group == 0) p.groups[starts] = make_int4(mine, before, min(m.group, total - rank), 0);
+    }
+    if (tid == 0) p.ngroups = all;
+    __syncthreads();
+}
 
 constexpr size_t kMoePlanBytes = 256 + kMoePairs * 16 + kMoePairs * 8;
 

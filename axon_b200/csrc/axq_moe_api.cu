@@ -10,7 +10,7 @@
 namespace axq {
 namespace {
 
-constexpr int64_t kMaxDim = int64_t(1) << 24;
+constexpr int64_t kMaxDim = int64_t(1) << 20;
 
 int fail(int code, const std::string& msg) {
     set_last_error(msg);
@@ -84,28 +84,39 @@ size_t axq_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int
     return moe_workspace_bytes(tokens, static_cast<int>(top_k), hidden, ffn);
 }
 
-int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
-                int fmt_down, const void* w_down, const float* down_scales, int dtype, const void* x, const int32_t* ids,
-                const float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
-                int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream) {
-    const char* fn = "axq_moe_mlp";
+static int moe_call(const char* fn, int fmt, const void* w_gate, const float* gate_scales, const void* w_up,
+                    const float* up_scales, int fmt_down, const void* w_down, const float* down_scales, int dtype,
+                    const void* x, const float* w_router, int normalize, int32_t* ids, float* weights, void* y,
+                    int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden, int64_t ffn, void* workspace,
+                    size_t workspace_bytes, axq_stream_t stream) {
     for (int f : {fmt, fmt_down})
         if (f != AXQ_F8_E4M3 && !host_block_elems(f))
             return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": unsupported format " + std::to_string(f));
     if (!host_dtype_size(dtype)) return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": unsupported dtype " + std::to_string(dtype));
     if (int r = check_sizes(tokens, experts, top_k, hidden, ffn, fn)) return r;
+    if (w_router && top_k > experts)
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": top_k is larger than the number of experts");
     if (tokens == 0 || hidden == 0) return AXQ_OK;
     if ((fmt == AXQ_F8_E4M3 || fmt_down == AXQ_F8_E4M3) && (hidden % kF8Block || ffn % kF8Block))
         return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": e4m3 experts need hidden and ffn to be multiples of 128");
     if (int r = check_aligned(y, "y", host_dtype_size(dtype), fn)) return r;
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (ffn == 0) return status(cudaMemsetAsync(y, 0, static_cast<size_t>(tokens * hidden) * host_dtype_size(dtype), s), fn);
-    if (int r = check_weights(fmt, w_gate, gate_scales, "w_gate", fn)) return r;
-    if (int r = check_weights(fmt, w_up, up_scales, "w_up", fn)) return r;
-    if (int r = check_weights(fmt_down, w_down, down_scales, "w_down", fn)) return r;
     if (int r = check_aligned(x, "x", host_dtype_size(dtype), fn)) return r;
     if (int r = check_aligned(ids, "ids", 4, fn)) return r;
     if (int r = check_aligned(weights, "weights", 4, fn)) return r;
+    if (w_router)
+        if (int r = check_aligned(w_router, "w_router", 4, fn)) return r;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (ffn == 0) {
+        if (w_router) {
+            cudaError_t e = moe_route_dispatch(dtype, x, w_router, ids, weights, tokens, static_cast<int>(experts),
+                                               static_cast<int>(top_k), hidden, normalize, s);
+            if (e != cudaSuccess) return status(e, fn);
+        }
+        return status(cudaMemsetAsync(y, 0, static_cast<size_t>(tokens * hidden) * host_dtype_size(dtype), s), fn);
+    }
+    if (int r = check_weights(fmt, w_gate, gate_scales, "w_gate", fn)) return r;
+    if (int r = check_weights(fmt, w_up, up_scales, "w_up", fn)) return r;
+    if (int r = check_weights(fmt_down, w_down, down_scales, "w_down", fn)) return r;
     const size_t need = axq_moe_workspace_size(tokens, top_k, hidden, ffn);
     if (!workspace || workspace_bytes < need)
         return fail(AXQ_ERR_WORKSPACE, std::string(fn) + ": workspace of " + std::to_string(need) + " bytes required");
@@ -124,6 +135,8 @@ int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const voi
     if (m.gate_bytes < 0 || m.down_bytes < 0) return fail(AXQ_ERR_INVALID, std::string(fn) + ": shape too large");
     m.dtype = dtype;
     m.x = x;
+    m.w_router = w_router;
+    m.normalize = normalize;
     m.ids = ids;
     m.weights = weights;
     m.y = y;
@@ -133,6 +146,25 @@ int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const voi
     m.experts = static_cast<int>(experts);
     m.top_k = static_cast<int>(top_k);
     return status(moe_mlp_dispatch(m, workspace, reinterpret_cast<int*>(workspace), s), fn);
+}
+
+int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
+                int fmt_down, const void* w_down, const float* down_scales, int dtype, const void* x, const int32_t* ids,
+                const float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
+                int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream) {
+    // without a router ids and weights are only read
+    return moe_call("axq_moe_mlp", fmt, w_gate, gate_scales, w_up, up_scales, fmt_down, w_down, down_scales, dtype, x, nullptr,
+                    0, const_cast<int32_t*>(ids), const_cast<float*>(weights), y, tokens, experts, top_k, hidden, ffn,
+                    workspace, workspace_bytes, stream);
+}
+
+int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, int fmt_down,
+            const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
+            int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
+            int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream) {
+    if (!w_router && tokens > 0 && hidden > 0) return fail(AXQ_ERR_INVALID, "axq_moe: w_router is NULL");
+    return moe_call("axq_moe", fmt, w_gate, gate_scales, w_up, up_scales, fmt_down, w_down, down_scales, dtype, x, w_router,
+                    normalize, ids, weights, y, tokens, experts, top_k, hidden, ffn, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

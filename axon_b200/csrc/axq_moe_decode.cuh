@@ -4,7 +4,7 @@
 // A column group (CG) is 256 elements of a row.  Lane (g, i) = (lane / 4,
 // lane % 4) of a warp holds, of each of its rows, 64 of a CG's elements: which
 // ones is each format's choice, as long as the activation records hold x in the
-// same order (Order<F>::elem).  In the formats with integer sub-block scales a
+// same order (order_elem).  In the formats with integer sub-block scales a
 // lane owns whole sub-blocks, so that it decodes only their scales.
 //
 // fp16 holds integers up to 2048 exactly, and 0x6400 | c is 1024 + c.  So
@@ -23,32 +23,40 @@ namespace axq {
 
 constexpr int F_F8 = 64;  // AXQ_F8_E4M3: e4m3 codes with 128 x 128 scales
 
-// Element (0..255) of the CG at slot 0..3 of MMA m (0..15) of lane part i.
-// Slots 0, 1 are the low and high half of the first fragment register, 2, 3 of
-// the second.  SUMS: sub-blocks whose sums of x weigh the minimums (0: none);
-// sum(i, j) is the sub-block at slot j of lane part i, -1 where there is none.
+// Order of a CG's elements and sub-blocks over the lanes, by format.
+//
+// SUMS: sub-blocks whose sums of x weigh the minimums (0: none).
 template <int F> struct Order {
     static constexpr bool K4 = F == F_Q4_K || F == F_Q5_K;
     static constexpr bool K16 = F == F_Q2_K || F == F_Q3_K || F == F_Q6_K;
     static constexpr int SUMS = K4 ? 8 : K16 ? 16 : 0;
-    __host__ __device__ static constexpr int elem(int m, int i, int slot) {
-        const int bo = slot == 1 ? 2 : slot == 2 ? 1 : slot;  // bytes 0, 2 of a word, then 1, 3
-        if (K4) return 64 * i + 32 * (m & 1) + 4 * (m >> 1) + bo;
-        if (K16) {
-            // Q2_K: lane part i starts at word i of its four (conflict-free loads)
-            const int v = F == F_Q2_K ? ((m >> 2) + i) & 3 : m >> 2;
-            return 128 * (i >> 1) + 32 * (m & 3) + 16 * (i & 1) + 4 * v + bo;
-        }
-        if (F == F_Q8_0) return 32 * (m >> 1) + 8 * i + 4 * (m & 1) + slot;
-        if (F == F_Q4_0) return 32 * (m >> 1) + 2 * (4 * i + bo) + (m & 1);
-        return 128 * (m >> 3) + 32 * i + 4 * (m & 7) + slot;  // e4m3
-    }
-    __host__ __device__ static constexpr int sum(int i, int j) {
-        if (K4) return j < 2 ? 2 * i + j : -1;
-        if (K16) return 8 * (i >> 1) + 2 * j + (i & 1);
-        return -1;
-    }
 };
+
+// Element (0..255) of the CG at slot 0..3 of MMA m (0..15) of lane part i.
+// Slots 0, 1 are the low and high half of the first fragment register, 2, 3 of
+// the second.
+__device__ __forceinline__ int order_elem(int fmt, int m, int i, int slot) {
+    const int bo = slot == 1 ? 2 : slot == 2 ? 1 : slot;  // bytes 0, 2 of a word, then 1, 3
+    if (fmt == F_Q4_K || fmt == F_Q5_K) return 64 * i + 32 * (m & 1) + 4 * (m >> 1) + bo;
+    if (fmt == F_Q2_K || fmt == F_Q3_K || fmt == F_Q6_K) {
+        // Q2_K: lane part i starts at word i of its four (conflict-free loads)
+        const int v = fmt == F_Q2_K ? ((m >> 2) + i) & 3 : m >> 2;
+        return 128 * (i >> 1) + 32 * (m & 3) + 16 * (i & 1) + 4 * v + bo;
+    }
+    if (fmt == F_Q8_0) return 32 * (m >> 1) + 8 * i + 4 * (m & 1) + slot;
+    if (fmt == F_Q4_0) return 32 * (m >> 1) + 2 * (4 * i + bo) + (m & 1);
+    return 128 * (m >> 3) + 32 * i + 4 * (m & 7) + slot;  // e4m3
+}
+
+// Sub-blocks of the format that have sums (0: none), and the one at slot j of
+// lane part i (-1: none).
+__device__ __forceinline__ int order_sums(int fmt) {
+    return fmt == F_Q4_K || fmt == F_Q5_K ? 8 : fmt == F_Q2_K || fmt == F_Q3_K || fmt == F_Q6_K ? 16 : 0;
+}
+__device__ __forceinline__ int order_sum(int fmt, int i, int j) {
+    if (fmt == F_Q4_K || fmt == F_Q5_K) return j < 2 ? 2 * i + j : -1;
+    return 8 * (i >> 1) + 2 * j + (i & 1);
+}
 
 template <int F> constexpr int moe_cg_bytes() {
     return F == F_F8 ? 256 : F == F_Q8_0 ? 8 * 34 : F == F_Q4_0 ? 8 * 18 : Traits<F == F_F8 ? F_Q4_K : F>::BB;

@@ -59,6 +59,27 @@ def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bo
     return ids, weights
 
 
+def _experts(w_gate, w_up, w_down, experts: int, hidden: int):
+    """(ffn, their arguments of the C entry points, their tensors)."""
+    if experts < 1 or w_gate.shape[0] % experts:
+        raise _invalid("w_gate must have experts * ffn rows")
+    ffn = w_gate.shape[0] // experts
+    fmt, gate, gate_s = _weights(w_gate, experts * ffn, hidden, "w_gate")
+    fmt_up, up, up_s = _weights(w_up, experts * ffn, hidden, "w_up")
+    fmt_down, down, down_s = _weights(w_down, experts * hidden, ffn, "w_down")
+    if fmt != fmt_up:
+        raise _invalid("w_gate and w_up must have the same format")
+    return (ffn, (fmt, gate.data_ptr(), gate_s, up.data_ptr(), up_s, fmt_down, down.data_ptr(), down_s), (gate, up, down))
+
+
+def _out(x: torch.Tensor, out: Optional[torch.Tensor], dtype: int) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(x)
+    if _float_type(out, "out") != dtype or out.shape != x.shape:
+        raise _invalid("out must have x's shape and type")
+    return out
+
+
 def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate, w_up, w_down, experts: int,
               out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * W_down[e] . (silu(W_gate[e] . x[t]) * (W_up[e] . x[t])), e = ids[t, j].
@@ -72,30 +93,18 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
     _plain(weights, "weights", torch.float32)
     if x.dim() != 2 or ids.dim() != 2 or ids.shape[0] != x.shape[0] or ids.shape != weights.shape:
         raise _invalid("moe_mlp_q: x must be [N x hidden], ids and weights [N x top_k]")
-    (n, hidden), top_k = x.shape, ids.shape[1]
-    if experts < 1 or w_gate.shape[0] % experts:
-        raise _invalid("moe_mlp_q: w_gate must have experts * ffn rows")
-    ffn = w_gate.shape[0] // experts
-    fmt, gate, gate_s = _weights(w_gate, experts * ffn, hidden, "w_gate")
-    fmt_up, up, up_s = _weights(w_up, experts * ffn, hidden, "w_up")
-    fmt_down, down, down_s = _weights(w_down, experts * hidden, ffn, "w_down")
-    if fmt != fmt_up:
-        raise _invalid("moe_mlp_q: w_gate and w_up must have the same format")
-    device = x.device
-    _same_device(device, ("ids", "weights", "w_gate", "w_up", "w_down", "out"), ids, weights, gate, up, down, out)
+    (n, hidden), top_k, device = x.shape, ids.shape[1], x.device
+    ffn, w, tensors = _experts(w_gate, w_up, w_down, experts, hidden)
+    _same_device(device, ("ids", "weights", "out", "w_gate", "w_up", "w_down"), ids, weights, out, *tensors)
     on = _on(device, stream)
     if on is not None:
         with on:
             return moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, experts, out)
-    if out is None:
-        out = torch.empty_like(x)
-    elif _float_type(out, "out") != dtype or out.shape != x.shape:
-        raise _invalid("moe_mlp_q: out must have x's shape and type")
+    out = _out(x, out, dtype)
     L = lib()
     buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn), x)
-    check(L.axq_moe_mlp(fmt, gate.data_ptr(), gate_s, up.data_ptr(), up_s, fmt_down, down.data_ptr(), down_s, dtype,
-                        x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(), n, experts, top_k, hidden, ffn, wp,
-                        wbytes, _raw_stream(device.index)))
+    check(L.axq_moe_mlp(*w, dtype, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(), n, experts, top_k, hidden,
+                        ffn, wp, wbytes, _raw_stream(device.index)))
     del buf
     return out
 
@@ -103,7 +112,25 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
 def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: int, normalize: bool = True,
           out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None
           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """The whole layer: :func:`moe_route`, then :func:`moe_mlp_q`.  Returns (y, ids, weights)."""
-    ids, weights = moe_route(x, w_router, top_k, normalize, stream)
-    y = moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, w_router.shape[0], out=out, stream=stream)
-    return y, ids, weights
+    """The whole layer: what :func:`moe_route` and then :func:`moe_mlp_q` give, in
+    three kernels where N * top_k is at most 64.  Returns (y, ids, weights)."""
+    dtype = _float_type(x, "x")
+    _plain(w_router, "w_router", torch.float32)
+    if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
+        raise _invalid("moe_q: x must be [N x hidden] and w_router [experts x hidden]")
+    (n, hidden), experts, device = x.shape, w_router.shape[0], x.device
+    ffn, w, tensors = _experts(w_gate, w_up, w_down, experts, hidden)
+    _same_device(device, ("w_router", "out", "w_gate", "w_up", "w_down"), w_router, out, *tensors)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return moe_q(x, w_router, w_gate, w_up, w_down, top_k, normalize, out)
+    out = _out(x, out, dtype)
+    ids = x.new_empty((n, top_k), dtype=torch.int32)
+    weights = x.new_empty((n, top_k), dtype=torch.float32)
+    L = lib()
+    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn), x)
+    check(L.axq_moe(*w, dtype, x.data_ptr(), w_router.data_ptr(), 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
+                    out.data_ptr(), n, experts, top_k, hidden, ffn, wp, wbytes, _raw_stream(device.index)))
+    del buf
+    return out, ids, weights

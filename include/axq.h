@@ -315,13 +315,22 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
  * the rows are codes without padding and *_scales their 128 x 128 scales (hidden
  * and ffn multiples of 128); otherwise *_scales are NULL.  x and y are [tokens x
  * hidden] in dtype F32, F16 or BF16.  Products and sums are fp32 (x and the hidden
- * activations enter the tensor cores as two fp16 terms, 22 bits); y is rounded
- * once.  Tokens beyond 512 / top_k take several passes over the experts. */
+ * activations enter the tensor cores as fp16: one term for 16-bit x, which it holds,
+ * two of 22 bits for fp32 x and for the hidden activations, one of 11 bits for those
+ * of a bf16 y); y is rounded once.  Tokens beyond 512 / top_k take several passes
+ * over the experts; tokens, hidden and ffn are at most 2^20. */
 size_t axq_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
 int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
                 int fmt_down, const void* w_down, const float* down_scales, int dtype, const void* x, const int32_t* ids,
                 const float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
                 int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream);
+
+/* The whole layer: axq_moe_route into ids and weights, then axq_moe_mlp, in three
+ * kernels where tokens * top_k is at most 64. */
+int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, int fmt_down,
+            const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
+            int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
+            int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream);
 
 /* ---- .axon tensor files ---------------------------------------------------
  * Replace save_tensor / load_tensor / save_checkpoint / load_checkpoint
