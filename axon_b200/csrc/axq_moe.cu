@@ -706,31 +706,41 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         uint32_t par = 0;
         bool ok = true;
         int64_t issued = 0;
+        constexpr int kMost = TL == 2 ? 4 : 2;  // rows of a stage that a lane copies, at most (four slots)
+        const int srows = a.slots * 16 * TL;
         for (int n = lo; n < hi && ok; ++n, rd.next(a)) {
-            const int t0 = rd.t0;
+            // where this lane's rows of a stage begin (of tile 0, if a stage holds one tile); -1: no such row
             const int64_t expert = pl.groups[rd.grp].x;
+            int64_t at0[kMost];
+#pragma unroll
+            for (int j = 0; j < kMost; ++j) {
+                const int sr = lane + 32 * j, u = sr / (16 * TL), r = sr & (16 * TL - 1);
+                const int64_t row = stage_row(a, rd.t0 + u, TL == 2 ? r >> 4 : 0, r & 15);
+                at0[j] = sr < srows && rd.t0 + u < a.tiles && row < a.rows ? (expert * a.rows + row) * a.rb : -1;
+            }
             for (int step = 0; step < ksteps * (2 / TL); ++step) {
-                const int k = step / (2 / TL), tile = TL == 2 ? lane >> 4 : step & 1;
+                const int k = step / (2 / TL), tile = step & 1;  // the tile counts where a stage holds one
+                // tile 1 of the down product is 16 rows on, and may lie past the last row
+                const int64_t skip = TL == 1 && tile && !a.gate_up ? 16 * a.rb : 0;
+                const int64_t end = (expert + 1) * a.rows * a.rb;
+                const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
+                const int64_t seg = min64(static_cast<int64_t>(a.wps) * CGB, a.row_bytes - off);
                 ok = moe_wait(&bars.empty[s], par ^ 1, &bars, a.err);
                 if (!ok) break;
                 uint8_t* st = ring + s * a.stage_bytes;
-                const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
-                const int64_t seg = min64(static_cast<int64_t>(a.wps) * CGB, a.row_bytes - off);
-                // A stage holds 16 TL rows of every slot; lanes take them in turn.  The bytes come from the 16-byte
-                // rounded range around a row's segment.
-                const int srows = a.slots * 16 * TL;
-                const uint8_t* w = a.w[tile];
-                uint32_t tx = 0;
-                for (int sr = lane; sr < srows; sr += 32) {
-                    const int u = sr / (16 * TL), r = sr - u * (16 * TL);
-                    const int64_t row = stage_row(a, t0 + u, TL == 2 ? r >> 4 : tile, r & 15);
-                    if (t0 + u >= a.tiles || row >= a.rows) continue;
-                    const int64_t at = (expert * a.rows + row) * a.rb + off;
+                // The bytes come from the 16-byte rounded range around a row's segment.
+                uint32_t tx = 0, len[kMost];
+#pragma unroll
+                for (int j = 0; j < kMost; ++j) {
+                    len[j] = 0;
+                    const int64_t at = at0[j] + skip + off;
+                    if (at0[j] < 0 || at0[j] + skip >= end) continue;
                     const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
+                    const int sr = lane + 32 * j;
                     if (to <= a.w_bytes) {
-                        tx += static_cast<uint32_t>(to - from);
+                        tx += len[j] = static_cast<uint32_t>(to - from);
                     } else {  // the rounded end would leave the buffer: bytes one by one
-                        const uint8_t* src = (TL == 2 ? a.w[r >> 4] : w) + at;
+                        const uint8_t* src = a.w[TL == 2 ? (sr >> 4) & 1 : tile] + at;
                         uint8_t* dst = st + sr * a.rs + (at & 15);
                         for (int64_t c = 0; c < seg; ++c) dst[c] = src[c];
                     }
@@ -739,14 +749,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                 __syncwarp();  // bytes copied by lanes come before the arrival
                 if (lane == 0) mbar_arrive_expect_tx(&bars.full[s], tx);
                 __syncwarp();
-                for (int sr = lane; sr < srows; sr += 32) {
-                    const int u = sr / (16 * TL), r = sr - u * (16 * TL);
-                    const int64_t row = stage_row(a, t0 + u, TL == 2 ? r >> 4 : tile, r & 15);
-                    if (t0 + u >= a.tiles || row >= a.rows) continue;
-                    const int64_t at = (expert * a.rows + row) * a.rb + off;
-                    const int64_t from = at & ~int64_t(15), to = (at + seg + 15) & ~int64_t(15);
-                    if (to <= a.w_bytes)
-                        bulk_g2s_hint(st + sr * a.rs, (TL == 2 ? a.w[r >> 4] : w) + from, static_cast<uint32_t>(to - from),
+#pragma unroll
+                for (int j = 0; j < kMost; ++j) {
+                    const int sr = lane + 32 * j;
+                    if (len[j])
+                        bulk_g2s_hint(st + sr * a.rs,
+                                      a.w[TL == 2 ? (sr >> 4) & 1 : tile] + ((at0[j] + skip + off) & ~int64_t(15)), len[j],
                                       &bars.full[s], policy);
                 }
                 ++issued;
