@@ -181,9 +181,10 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
         return;
     }
     const int nt = static_cast<int>(min64(kRouteTokens, tokens - t0));
-    cluster_sync_all();  // the first CTA's shared memory is there
+    cluster_arrive();  // waited for before the first store to the first CTA's shared memory
     pdl_wait();
     pdl_launch_dependents();
+    bool there = false;
     const int64_t per = ((hidden + slices - 1) / slices + 127) / 128 * 128;  // columns of a slice
     for (int o = static_cast<int>(rank) * kRouteWarps + warp; o < experts * slices; o += kRouteCtas * kRouteWarps) {
         const int e = o / slices, sl = o - e * slices;
@@ -220,74 +221,73 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
                 for (int t = 0; t < kRouteTokens; ++t)
                     if (t < nt) acc[t] = fmaf(we[k], Elem<T>::get(xt[t * hidden + k]), acc[t]);
         }
+        if (!there) cluster_wait();
+        there = true;
 #pragma unroll
         for (int t = 0; t < kRouteTokens; ++t) {
+            if (t >= nt) break;
 #pragma unroll
             for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(0xFFFFFFFFu, acc[t], d);
-            if (lane == 0 && t < nt)
+            if (lane == 0)
                 st_cluster_f32(cluster_addr(logits + (sl * kRouteTokens + t) * experts + e, 0), acc[t]);
         }
     }
+    if (!there) cluster_wait();
     cluster_sync_all();
     if (rank != 0 || warp >= nt) return;
-    float* l = logits + warp * experts;
+    // One warp per token.  Logits become keys whose order as integers is theirs
+    // (NaN 1, chosen ones 0); lane e % 32 holds the best of its own.
+    uint32_t* keys = reinterpret_cast<uint32_t*>(logits) + warp * experts;
+    uint32_t best = 0;
+    int best_e = INT32_MAX;
     for (int e = lane; e < experts; e += 32) {
-        float v = l[e];
-        for (int sl = 1; sl < slices; ++sl) v += l[sl * kRouteTokens * experts + e];
-        l[e] = v;
+        const float* l = logits + warp * experts + e;
+        float v = l[0];
+        for (int sl = 1; sl < slices; ++sl) v += l[sl * kRouteTokens * experts];
+        const uint32_t b = __float_as_uint(v);
+        const uint32_t k = isnan(v) ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+        keys[e] = k;
+        if (k > best) {
+            best = k;
+            best_e = e;
+        }
     }
-    __syncwarp();
-    float mx = -INFINITY;
-    for (int e = lane; e < experts; e += 32) mx = fmaxf(mx, l[e]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-    float all = 0.0f;
-    for (int e = lane; e < experts; e += 32) all += expf(l[e] - mx);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, d);
-    float mine = 0.0f, sum = 0.0f;
+    auto value = [](uint32_t k) {
+        return k == 1u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+    };
+    float mine = 0.0f, sum = 0.0f, mx = 0.0f;
     int my_id = 0;
-    for (int j = 0; j < top_k; ++j) {
-        // best of the experts not yet chosen (chosen ones are marked by a bit of `taken`)
-        float bv = 0.0f;
-        int bi = INT32_MAX;
-        for (int e = lane; e < experts; e += 32) {
-            const float v = l[e];
-            const bool first = bi == INT32_MAX;
-            // order: greater value first, NaN after everything, then the lower index
-            const bool better = first || (isnan(bv) ? !isnan(v) : v > bv);
-            if (__float_as_uint(v) != 0xFFFFDEADu && better) {
-                bv = v;
-                bi = e;
-            }
-        }
+    if (!normalize) {  // the sum over all experts, before the chosen ones are marked
+        mx = value(__reduce_max_sync(0xFFFFFFFFu, best));
+        for (int e = lane; e < experts; e += 32) sum += expf(value(keys[e]) - mx);
 #pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            const float ov = __shfl_xor_sync(0xFFFFFFFFu, bv, d);
-            const int oi = __shfl_xor_sync(0xFFFFFFFFu, bi, d);
-            bool take;
-            if (oi == INT32_MAX) take = false;
-            else if (bi == INT32_MAX) take = true;
-            else if (isnan(ov) || isnan(bv)) take = isnan(ov) == isnan(bv) ? oi < bi : isnan(bv);
-            else take = ov > bv || (ov == bv && oi < bi);
-            if (take) {
-                bv = ov;
-                bi = oi;
-            }
-        }
-        const float p = expf(bv - mx);
-        sum += p;
-        if (lane == j % 32) {
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    }
+    for (int j = 0; j < top_k; ++j) {
+        const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
+        const int e = __reduce_min_sync(0xFFFFFFFFu, best == m ? best_e : INT32_MAX);  // ties: the lowest index
+        if (j == 0) mx = value(m);
+        const float p = expf(value(m) - mx);
+        if (normalize) sum += p;
+        if (lane == j) {
             mine = p;
-            my_id = bi;
+            my_id = e;
         }
-        __syncwarp();
-        if (lane == 0) l[bi] = __uint_as_float(0xFFFFDEADu);  // a NaN no product gives
+        if (lane == (e & 31)) {
+            keys[e] = 0;
+            best = 0;
+            best_e = INT32_MAX;
+            for (int q = lane; q < experts; q += 32)
+                if (keys[q] > best) {
+                    best = keys[q];
+                    best_e = q;
+                }
+        }
         __syncwarp();
     }
     if (lane < top_k) {
         ids[(t0 + warp) * top_k + lane] = my_id;
-        wt[(t0 + warp) * top_k + lane] = mine / (normalize ? sum : all);
+        wt[(t0 + warp) * top_k + lane] = mine / sum;
     }
 }
 
