@@ -584,20 +584,22 @@ __device__ __forceinline__ void moe_results(const ExpertArgs& a, const PlanView&
     const int rs = a.gate_up ? 4 : 5;  // log2 of a unit's rows
     const int outputs = gd.z << rs;    // of a unit
     for (int un = 0; un < a.slots && rd.t0 + un < a.tiles; ++un) {
-#pragma unroll 2
         for (int o = lane; o < outputs; o += 32) {
             const int rr = o & ((1 << rs) - 1), t = o >> rs;
             const int64_t row = (static_cast<int64_t>(rd.t0 + un) << rs) + rr;
+            // the warps' parts are loaded together and added in order
+            float part[2][kConsumers];
+            const float* q = rb + (un * a.wps * 2 * kTok + t) * 16 + (a.gate_up ? rr : (rr >> 4) * kTok * 16 + (rr & 15));
+#pragma unroll
+            for (int w = 0; w < kConsumers; ++w) {
+                part[0][w] = w < a.wps ? q[w * 2 * kTok * 16] : 0.0f;
+                part[1][w] = a.gate_up && w < a.wps ? q[(w * 2 + 1) * kTok * 16] : 0.0f;
+            }
             float v[2] = {0.0f, 0.0f};
-            const float* q = rb + (un * a.wps * 2 * kTok + t) * 16;
-            if (a.gate_up) {
-                for (int w = 0; w < a.wps; ++w) {
-                    v[0] += q[w * 2 * kTok * 16 + rr];
-                    v[1] += q[(w * 2 + 1) * kTok * 16 + rr];
-                }
-            } else {
-                q += (rr >> 4) * kTok * 16 + (rr & 15);
-                for (int w = 0; w < a.wps; ++w) v[0] += q[w * 2 * kTok * 16];
+#pragma unroll
+            for (int w = 0; w < kConsumers; ++w) {
+                v[0] += part[0][w];
+                v[1] += part[1][w];
             }
             const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
             if (row < a.rows) a.out[static_cast<int64_t>(pl.entries[gd.y + t].x) * a.rows + row] = z;
@@ -661,7 +663,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
     constexpr int TL = kStageTiles<F, NB>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127);
-    float* red = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [2][warp][tile][token][16]
+    float* red = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // the warps' sums of two rounds
     __shared__ MoeBars bars;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         return;
     }
 
-    constexpr int kSums = kConsumers * 2 * kTok * 16;
+    constexpr int kSums = kConsumers * 2 * kTok * 16;  // [warp][tile][token][16 rows]
     if (warp > kConsumers) {
         // The finisher joins each round's sums beside the consumers, which go on; it needs no registers that the SM has
         // not left over (18 and 20 warps share its schedulers alike).
@@ -865,7 +867,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                 }
             }
         }
-        // the sums of two rounds before, in the same buffer, have been joined
+        // The sums of two rounds before, in the same buffer, have been joined.  (One buffer and a deeper ring were slower:
+        // 90 against 77 us for 16 tokens on e4m3 experts.)
         if (ok && q > 1) ok = moe_wait(&bars.joined[q & 1], ((q >> 1) - 1) & 1, &bars, a.err);
         float* rb = red + (q & 1) * kSums;
 #pragma unroll
@@ -1036,10 +1039,10 @@ cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* id
     return launch_route(dtype, x, w, ids, weights, tokens, experts, top_k, hidden, normalize, RecordArgs{}, nullptr, s);
 }
 
-// Passes of up to kMoePairs choices.  Few choices (kMoeFew) take three kernels:
-// router (if given) and records of x, gate and up with the records of the hidden
-// activations, down with y; more take a plan and separate kernels for the hidden
-// records and for y, whose cost is small beside the experts'.
+// Passes of up to kMoePairs choices.  Few choices (kMoeFew) of few tokens take
+// three kernels: router (if given) and records of x, gate and up with the records
+// of the hidden activations, down with y; more take kernels of their own for the
+// plan, the hidden records and y, whose cost is small beside the experts'.
 cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s) {
     const MoeSpace w = moe_space(m.tokens, m.top_k, m.hidden, m.ffn);
     auto* base = static_cast<uint8_t*>(ws);
@@ -1048,7 +1051,8 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
     // 16-bit x is one term; so are the hidden activations of a bf16 result, whose own rounding is 8 times theirs
     const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = m.dtype == AXQ_DT_BF16 ? 1 : 2;
     const bool few = m.tokens <= kMoeFewTokens && m.tokens * m.top_k <= kMoeFew;
-    if (m.w_router && !few) {
+    const bool several = m.tokens > step;  // passes
+    if (m.w_router && several) {
         cudaError_t e = moe_route_dispatch(m.dtype, m.x, m.w_router, m.ids, m.weights, m.tokens, m.experts, m.top_k, m.hidden,
                                            m.normalize, s);
         if (e != cudaSuccess) return e;
@@ -1080,9 +1084,14 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         rx.clear = counters;
         rx.nclear = few ? static_cast<int>(w.ncounters) : 0;
         cudaError_t e;
-        if (m.w_router && few) {
+        const bool routed = m.w_router && !several;  // the router's kernel writes the records too
+        if (routed) {
             e = launch_route(m.dtype, x, m.w_router, m.ids, m.weights, t, m.experts, m.top_k, m.hidden, m.normalize, rx, err, s);
-        } else {
+            if (e != cudaSuccess) return e;
+            rx.rows = 0;
+            plan.err = nullptr;
+        }
+        if (!routed || !few) {
             MoePlan first = plan;
             if (few) first.ids = nullptr;  // records only
             e = with_dtype(m.dtype, [&](auto* tag) {
