@@ -108,17 +108,27 @@ __device__ __forceinline__ float2 h2_flush(uint32_t hd) {
 }
 constexpr uint32_t kMagic = 0x64006400u;  // 1024 in both halves
 
-// Words at a 2-byte aligned shared address: the two aligned words around each.
-template <int N>
-__device__ __forceinline__ void ld_words2(const uint8_t* p, uint32_t (&out)[N]) {
-    const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
-    const uint32_t* b = reinterpret_cast<const uint32_t*>(p - mis);
-    uint32_t w[N + 1];
+// Words of a block at a 2-byte aligned shared address: one aligned base for the
+// whole block, since every offset asked for is a multiple of 4; each word is cut
+// out of the two aligned ones around it.
+struct Words2 {
+    const uint32_t* b;
+    uint32_t sh;
+    __device__ __forceinline__ explicit Words2(const uint8_t* p) {
+        // the base by pointer arithmetic keeps a shared pointer shared
+        const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 3u;
+        b = reinterpret_cast<const uint32_t*>(p - mis);
+        sh = mis * 8;
+    }
+    template <int N>
+    __device__ __forceinline__ void load(int off, uint32_t (&out)[N]) const {
+        uint32_t w[N + 1];
 #pragma unroll
-    for (int k = 0; k <= N; ++k) w[k] = b[k];
+        for (int k = 0; k <= N; ++k) w[k] = b[off / 4 + k];
 #pragma unroll
-    for (int k = 0; k < N; ++k) out[k] = __funnelshift_r(w[k], w[k + 1], mis * 8);
-}
+        for (int k = 0; k < N; ++k) out[k] = __funnelshift_r(w[k], w[k + 1], sh);
+    }
+};
 
 __device__ __forceinline__ uint32_t ld_half2b(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
 
@@ -236,8 +246,9 @@ template <> struct MoeRow<F_Q3_K> {
     uint32_t e, o;  // fields 0, 2 and 1, 3 of the word at work
     __device__ __forceinline__ void load(const uint8_t* p, int i) {
         hd = ld_half2b(p + 108);
+        const Words2 words(p);
         uint32_t s[3];
-        ld_words2(p + 96, s);
+        words.load(96, s);
         // scale is = 8n + 2j + lh: low 4 bits in nibble n of byte 2j + lh of the first eight, high 2 bits at
         // 2 (is >> 2) of byte 8 + (is & 3)
         const int n = i >> 1, lh = i & 1;
@@ -252,8 +263,8 @@ template <> struct MoeRow<F_Q3_K> {
         const uint32_t c01 = hmul2(x01, h2_pow2(10, 10) | kNeg2), c23 = hmul2(s23, h2_pow2(10, 10) | kNeg2);
         sc[0] = h2_low(x01); sc[1] = h2_high(x01); sc[2] = h2_low(s23); sc[3] = h2_high(s23);
         c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
-        ld_words2(p + 32 + 32 * n + 16 * lh, w);
-        ld_words2(p + 16 * lh, h);
+        words.load(32 + 16 * i, w);
+        words.load(16 * lh, h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[k] >>= 4 * n;
     }
@@ -290,8 +301,9 @@ template <> struct MoeRow<F_Q6_K> {
     __device__ __forceinline__ void load(const uint8_t* p, int i) {
         const int n = i >> 1, lh = i & 1;
         hd = ld_half2b(p + 208);
+        const Words2 words(p);
         uint32_t s[2];
-        ld_words2(p + 192 + 8 * n, s);
+        words.load(192 + 8 * n, s);
         const int by = 8 * lh;
         mn[0] = hmul2(ints_h2<128>(((s[0] >> by) & 0x00FF00FFu) ^ 0x00800080u), h2_pow2(-2, -2));
         mn[1] = hmul2(ints_h2<128>(((s[1] >> by) & 0x00FF00FFu) ^ 0x00800080u), h2_pow2(-2, -2));
@@ -299,9 +311,9 @@ template <> struct MoeRow<F_Q6_K> {
         sc[0] = h2_low(mn[0]); sc[1] = h2_high(mn[0]); sc[2] = h2_low(mn[1]); sc[3] = h2_high(mn[1]);
         c[0] = h2_low(c01); c[1] = h2_high(c01); c[2] = h2_low(c23); c[3] = h2_high(c23);
         uint32_t a[4], b[4];
-        ld_words2(p + 64 * n + 16 * lh, a);
-        ld_words2(p + 64 * n + 32 + 16 * lh, b);
-        ld_words2(p + 128 + 32 * n + 16 * lh, hi);
+        words.load(64 * n + 16 * lh, a);
+        words.load(64 * n + 32 + 16 * lh, b);
+        words.load(128 + 16 * i, hi);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             lo[k] = a[k];      // fields 0 (low nibbles) and 2 (high)
@@ -344,7 +356,7 @@ template <> struct MoeRow<F_Q8_0> {
     __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
         hd = ld_half2b(p + 34 * MP);
         uint32_t w[2];
-        ld_words2(p + 34 * MP + 2 + 8 * i, w);
+        Words2(p + 34 * MP + 2 + 8 * i).load(0, w);
         const uint32_t off = h2_const(-1152.0f), unit = h2_const(1.0f);  // 1024 + 128
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -364,7 +376,7 @@ template <> struct MoeRow<F_Q4_0> {
     __device__ __forceinline__ void pair(uint32_t (&a)[4]) {
         hd = ld_half2b(p + 18 * MP);
         uint32_t w[1];
-        ld_words2(p + 18 * MP + 2 + 4 * i, w);
+        Words2(p + 18 * MP + 2 + 4 * i).load(0, w);
         const uint32_t x = w[0], y = x >> 8;
         const uint32_t unit = h2_const(1.0f), o0 = h2_const(-1032.0f), s = h2_const(0.0625f), o1 = h2_const(-72.0f);
         a[0] = hfma2(and_or<0x000F000Fu, kMagic>(x), unit, o0);
