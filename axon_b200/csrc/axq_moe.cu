@@ -682,7 +682,6 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
     pdl_wait();
     pdl_launch_dependents();
     __shared__ MoeFewPlan few;
-    __shared__ int last[4];
     PlanView pl{a.plan.groups, a.plan.entries, 0};
     if (a.plan.ids) {
         moe_few_plan(few, a.plan);
@@ -942,7 +941,8 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     a.stage_bytes = a.slots * 16 * kStageTiles<F, NB> * a.rs;
     // sums of two rounds, and with few choices 256 hidden activations on their way into a record
     const int red = 2 * kConsumers * 2 * (8 / T) * NB * 16 * 4 + (a.plan.ids && a.gate_up ? 1024 : 0);
-    const int budget = 112 * 1024 - 512 - red;  // two CTAs per SM
+    // two CTAs per SM, each with up to 3 KB besides (barriers, the plan of few choices, the driver's 1 KB)
+    const int budget = 109 * 1024 - 512 - red;
     a.stages = std::min(kMoeStages, budget / a.stage_bytes);
     int per_sm = 2;
     if (a.stages < 2) {

@@ -196,6 +196,67 @@ def test_whole_layer_beside_linear_f8(cuda, orc):
     assert torch.equal(y2, y)
 
 
+@pytest.mark.parametrize("T", [1, 8, 9, 70, 300])
+def test_whole_layer_is_its_parts(cuda, orc, T):
+    """moe_q against moe_route and moe_mlp_q, bit by bit, for every form of the call: three kernels, one pass, several."""
+    rng = np.random.default_rng(T)
+    E, K, hidden, ffn = 6, 2, 300, 520
+    q = [_q(Weights(orc, f, E, r, c, rng)) for f, r, c in
+         (("Q5_K", ffn, hidden), ("Q5_K", ffn, hidden), ("Q4_0", hidden, ffn))]
+    wr = torch.from_numpy(rng.standard_normal((E, hidden)).astype(np.float32)).cuda()
+    for dtype in TYPES.values():
+        x = torch.from_numpy((rng.standard_normal((T, hidden)) * 0.05).astype(np.float32)).to(dtype).cuda()
+        for normalize in (True, False):
+            y, ids, p = ax.moe_q(x, wr, *q, K, normalize=normalize)
+            ids2, p2 = ax.moe_route(x, wr, K, normalize=normalize)
+            assert torch.equal(ids, ids2) and torch.equal(p, p2)
+            assert torch.equal(y, ax.moe_mlp_q(x, ids, p, *q, experts=E))
+
+
+def test_first_call_inside_a_capture(cuda):
+    """In a fresh process: nothing that a call looks up once may keep it from being captured."""
+    import subprocess
+    import sys
+
+    code = """
+import torch, axon_b200 as ax
+x = torch.randn(40, 512, device='cuda'); few = torch.randn(2, 512, device='cuda'); many = torch.randn(300, 512, device='cuda')
+w = ax.quantize_f8(ax.F8Tensor.empty(512, 512), torch.randn(512, 512, device='cuda'))
+e = ax.quantize_f8(ax.F8Tensor.empty(4 * 512, 512), torch.randn(2048, 512, device='cuda'))
+r = torch.randn(4, 512, device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = [ax.linear_f8(v, w) for v in (x, few, many)] + [ax.moe_q(v, r, e, e, e, 2)[0] for v in (few, x)]
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, [ax.linear_f8(v, w) for v in (x, few, many)] + [ax.moe_q(v, r, e, e, e, 2)[0] for v in (few, x)]):
+    assert torch.equal(a, b)
+print('captured')
+"""
+    from conftest import ROOT
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
+
+
+def test_two_streams_at_once(cuda, orc):
+    """Two calls that overlap on the GPU, each on its own stream: results as alone."""
+    rng = np.random.default_rng(21)
+    q = [_q(Weights(orc, f, 4, r, c, rng)) for f, r, c in (("Q4_K", 512, 768), ("Q4_K", 512, 768), ("Q6_K", 768, 512))]
+    wr = torch.randn(4, 768, device="cuda")
+    xs = [torch.randn(n, 768, device="cuda") * 0.05 for n in (3, 20)]
+    alone = [ax.moe_q(x, wr, *q, 2)[0] for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            outs[i].append(ax.moe_q(xs[i], wr, *q, 2, stream=streams[i])[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
 def test_empty(cuda, orc):
     rng = np.random.default_rng(1)
     q = _q(Weights(orc, "Q4_K", 2, 32, 64, rng))
