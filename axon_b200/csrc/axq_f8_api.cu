@@ -49,6 +49,11 @@ int check_blocks(int64_t rows, int64_t cols, int block_rows, const char* fn) {
     return AXQ_OK;
 }
 
+int64_t codes_span(int64_t rows, int64_t cols, int64_t ld) { return (rows - 1) * ld + cols; }
+int64_t scales_span(int64_t rows, int64_t cols, int block_rows) {
+    return (rows + block_rows - 1) / block_rows * nkb_of(cols) * 4;
+}
+
 }  // namespace
 }  // namespace axq
 
@@ -66,6 +71,10 @@ int axq_quantize_f8(int dtype, const void* src, void* codes, int64_t ld, float* 
     if (reinterpret_cast<uintptr_t>(src) % host_dtype_size(dtype))
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": src is not aligned to its element type");
     if (int r = check_codes(codes, ld, scales, cols, "codes", fn)) return r;
+    const int64_t src_span = rows * cols * host_dtype_size(dtype), scales_bytes = scales_span(rows, cols, block_rows);
+    if (overlap(src, src_span, codes, codes_span(rows, cols, ld)) || overlap(src, src_span, scales, scales_bytes) ||
+        overlap(codes, codes_span(rows, cols, ld), scales, scales_bytes))
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": src, codes and scales must not overlap");
     return status(f8_pack_dispatch(dtype, src, codes, ld, scales, rows, cols, block_rows, nullptr,
                                    reinterpret_cast<cudaStream_t>(stream)), fn);
 }
@@ -78,6 +87,9 @@ int axq_dequantize_f8(const void* codes, int64_t ld, const float* scales, int bl
     if (int r = check_codes(codes, ld, scales, cols, "codes", fn)) return r;
     if (int r = check_device_ptr(dst, "dst", fn)) return r;
     if (reinterpret_cast<uintptr_t>(dst) % 4) return fail(AXQ_ERR_INVALID, std::string(fn) + ": dst must be 4-byte aligned");
+    if (overlap(dst, rows * cols * 4, codes, codes_span(rows, cols, ld)) ||
+        overlap(dst, rows * cols * 4, scales, scales_span(rows, cols, block_rows)))
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": dst must not overlap the codes or their scales");
     return status(f8_dequant_dispatch(codes, ld, scales, block_rows, dst, rows, cols, reinterpret_cast<cudaStream_t>(stream)),
                   fn);
 }
@@ -116,11 +128,16 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
     if (int r = check_device_ptr(workspace, "workspace", fn)) return r;
     if (reinterpret_cast<uintptr_t>(workspace) % 256)
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": workspace must be 256-byte aligned");
+    const int64_t y_span = N * M * host_dtype_size(y_dtype);
+    if (overlap(y, y_span, workspace, static_cast<int64_t>(need)) || (bias && overlap(y, y_span, bias, M * 4)))
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap the workspace or the bias");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     auto* ws = static_cast<uint8_t*>(workspace);
     int* err = reinterpret_cast<int*>(ws);
     if (K == 0) return status(f8_fill_bias_dispatch(y_dtype, y, bias, M, N, err, s), fn);
     if (int r = check_codes(w_codes, w_ld, w_scales, K, "w", fn)) return r;
+    if (overlap(y, y_span, w_codes, codes_span(M, K, w_ld)) || overlap(y, y_span, w_scales, scales_span(M, K, kF8Block)))
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap w");
     F8Linear l{};
     l.w = w_codes;
     l.w_scales = w_scales;
@@ -134,6 +151,8 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
     l.err = err;
     if (packed) {
         if (int r = check_codes(x, x_ld, x_scales, K, "x", fn)) return r;
+        if (overlap(y, y_span, x, codes_span(N, K, x_ld)) || overlap(y, y_span, x_scales, scales_span(N, K, 1)))
+            return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap x");
         l.x = x;
         l.x_scales = x_scales;
         l.x_ld = x_ld;
@@ -143,6 +162,8 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
         if (int r = check_device_ptr(x, "x", fn)) return r;
         if (reinterpret_cast<uintptr_t>(x) % host_dtype_size(x_dtype))
             return fail(AXQ_ERR_INVALID, std::string(fn) + ": x is not aligned to its element type");
+        if (overlap(y, y_span, x, N * K * host_dtype_size(x_dtype)))
+            return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap x");
         if (f8_gemm_packs(M, K, N)) {
             l.x = x;
             return status(f8_gemm_unpacked_dispatch(l, x_dtype, s), fn);

@@ -27,6 +27,12 @@ int validate_matmul_ptrs(int fmt, const void* a_q, const void* b, const void* ou
 // NULL, host-only and other-device pointers -> AXQ_ERR_INVALID with a message.
 int check_device_ptr(const void* p, const char* what, const char* fn);
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
 cudaError_t pack_dispatch(int fmt, const float* src, void* dst, int64_t rows, int64_t cols, cudaStream_t s);
 cudaError_t dequant_dispatch(int fmt, const void* src, float* dst, int64_t rows, int64_t cols, cudaStream_t s);
 

@@ -105,6 +105,10 @@ static int moe_call(const char* fn, int fmt, const void* w_gate, const float* ga
     if (int r = check_aligned(weights, "weights", 4, fn)) return r;
     if (w_router)
         if (int r = check_aligned(w_router, "w_router", 4, fn)) return r;
+    const int64_t y_span = tokens * hidden * host_dtype_size(dtype), choices = tokens * top_k * 4;
+    if (overlap(y, y_span, x, y_span) || overlap(y, y_span, ids, choices) || overlap(y, y_span, weights, choices) ||
+        (w_router && overlap(ids, choices, weights, choices)))
+        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y, x, ids and weights must not overlap");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (ffn == 0) {
         if (w_router) {
@@ -162,7 +166,8 @@ int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w
             const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
             int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
             int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream) {
-    if (!w_router && tokens > 0 && hidden > 0) return fail(AXQ_ERR_INVALID, "axq_moe: w_router is NULL");
+    if (hidden == 0 && tokens > 0) return fail(AXQ_ERR_INVALID, "axq_moe: hidden must be positive");  // as the router
+    if (!w_router && tokens > 0) return fail(AXQ_ERR_INVALID, "axq_moe: w_router is NULL");
     return moe_call("axq_moe", fmt, w_gate, gate_scales, w_up, up_scales, fmt_down, w_down, down_scales, dtype, x, w_router,
                     normalize, ids, weights, y, tokens, experts, top_k, hidden, ffn, workspace, workspace_bytes, stream);
 }

@@ -269,7 +269,8 @@ enum axq_dtype { AXQ_DT_F32 = 0, AXQ_DT_F16 = 1, AXQ_DT_BF16 = 2, AXQ_DT_F8 = 3 
  * even in that order, codes saturating at 448.  A block whose scale is 0 has
  * codes 0; NaN elements get the NaN code and do not enter the maximum; an
  * infinity makes the block's scale infinite (it decodes to NaN).  Bytes between
- * cols and ld that lie in the last block of 128 columns are set to 0. */
+ * cols and ld that lie in the last block of 128 columns are set to 0.  src, codes
+ * and scales overlap nowhere. */
 int axq_quantize_f8(int dtype, const void* src, void* codes, int64_t ld, float* scales, int64_t rows, int64_t cols,
                     int block_rows, axq_stream_t stream);
 
@@ -282,9 +283,10 @@ int axq_dequantize_f8(const void* codes, int64_t ld, const float* scales, int bl
  * 128 x 128 blocks.  x is [tokens x in_features] in x_dtype: F32, F16 or BF16
  * (row-major, x_ld = in_features, x_scales NULL; packed into 1 x 128 blocks by
  * the call, as axq_quantize_f8 does), or F8 (already packed so, x_ld its row
- * stride).  Sums are fp32; the result is rounded once.  The workspace holds the
- * status word and the packed x (256-byte aligned); a bounded wait that gave up
- * is reported by axq_workspace_status. */
+ * stride).  Sums are fp32; the result is rounded once.  y
+ * overlaps no operand.  The workspace holds the status word and the packed x
+ * (256-byte aligned; calls that share one must be ordered); a bounded wait that
+ * gave up is reported by axq_workspace_status. */
 size_t axq_linear_f8_workspace_size(int x_dtype, int64_t in_features, int64_t tokens);
 int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int x_dtype, const void* x, int64_t x_ld,
                   const float* x_scales, const float* bias, int y_dtype, void* y, int64_t out_features,
@@ -318,7 +320,9 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
  * activations enter the tensor cores as fp16: one term for 16-bit x, which it holds,
  * two of 22 bits for fp32 x and for the hidden activations, one of 11 bits for those
  * of a bf16 y); y is rounded once.  Tokens beyond 512 / top_k take several passes
- * over the experts; tokens, hidden and ffn are at most 2^20. */
+ * over the experts; tokens, hidden and ffn are at most 2^20.  y
+ * overlaps neither x nor ids nor weights.  Calls that share a workspace (256-byte
+ * aligned) must be ordered; its status is read by axq_workspace_status. */
 size_t axq_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
 int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
                 int fmt_down, const void* w_down, const float* down_scales, int dtype, const void* x, const int32_t* ids,
@@ -326,7 +330,7 @@ int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const voi
                 int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream);
 
 /* The whole layer: axq_moe_route into ids and weights, then axq_moe_mlp, in three
- * kernels where tokens * top_k is at most 64. */
+ * kernels for up to 8 tokens with at most 64 choices. */
 int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, int fmt_down,
             const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
             int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,

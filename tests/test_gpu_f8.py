@@ -234,3 +234,28 @@ def test_refusals(cuda):
     st = L.axq_linear_f8(w.data.data_ptr(), 256, w.scales.data_ptr(), 0, cpu.data_ptr(), 256, None, None, 0, y.data_ptr(), 256,
                          256, 4, big.data_ptr(), 8192, None)
     assert st == ax.Status.ERR_INVALID
+
+
+def test_overlaps_are_refused(cuda):
+    w = ax.quantize_f8(ax.F8Tensor.empty(256, 256), torch.randn(256, 256, device="cuda"))
+    x = torch.randn(4, 256, device="cuda")
+    both = torch.zeros(5, 256, device="cuda")
+    for first in (0, 1):  # the same rows, and shifted by one
+        with pytest.raises(ax.AxqError, match="must not overlap x"):
+            ax.linear_f8(both[:4], w, out=both[first:first + 4])
+    room = torch.zeros(4 * 256 * 4, dtype=torch.uint8, device="cuda")
+    xq = ax.F8Tensor(room[:1024].view(torch.float8_e4m3fn).view(4, 256), torch.zeros(4, 2, device="cuda"), (4, 256), 1)
+    with pytest.raises(ax.AxqError, match="must not overlap x"):
+        ax.linear_f8(xq, w, out=room.view(torch.float32).view(4, 256))
+    bias = torch.zeros(4 * 256, device="cuda")
+    with pytest.raises(ax.AxqError, match="the bias"):
+        ax.linear_f8(x, w, bias=bias[256:512], out=bias.view(4, 256))
+    src = torch.zeros(64, 64, device="cuda")
+    codes = ax.F8Tensor(src.view(torch.float8_e4m3fn).view(-1)[:64 * 64].view(64, 64), torch.empty(1, 1, device="cuda"), (64, 64))
+    with pytest.raises(ax.AxqError, match="must not overlap"):
+        ax.quantize_f8(codes, src)
+    with pytest.raises(ax.AxqError, match="must not overlap"):
+        ax.dequantize_f8(src, codes)
+    rows = torch.zeros(8, 256, device="cuda")
+    rows[:4] = x
+    assert torch.equal(ax.linear_f8(rows[:4], w, out=rows[4:]), ax.linear_f8(x, w))  # neighbours do not

@@ -287,3 +287,25 @@ def test_refusals(cuda, orc):
     f = ax.F8Tensor.empty(2 * 100, 128)
     with pytest.raises(ax.AxqError, match="multiples of 128"):
         ax.moe_mlp_q(torch.zeros(1, 128, device="cuda"), ids, p, f, f, _q(Weights(orc, "Q4_K", 2, 128, 100, rng)), experts=2)
+
+
+def test_overlaps_and_no_features_are_refused(cuda, orc):
+    rng = np.random.default_rng(3)
+    q = _q(Weights(orc, "Q4_K", 2, 32, 64, rng))
+    d = _q(Weights(orc, "Q4_K", 2, 64, 32, rng))
+    both = torch.zeros(3, 64, device="cuda")
+    ids, p = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, 1, device="cuda")
+    wr = torch.zeros(2, 64, device="cuda")
+    for first in (0, 1):
+        with pytest.raises(ax.AxqError, match="must not overlap"):
+            ax.moe_mlp_q(both[:2], ids, p, q, q, d, experts=2, out=both[first:first + 2])
+        with pytest.raises(ax.AxqError, match="must not overlap"):
+            ax.moe_q(both[:2], wr, q, q, d, 1, out=both[first:first + 2])
+    p = torch.ones(2, 64, device="cuda")
+    with pytest.raises(ax.AxqError, match="must not overlap"):
+        ax.moe_mlp_q(both[:2], torch.zeros(2, 32, dtype=torch.int32, device="cuda"), p.view(-1)[:64].view(2, 32), q, q, d,
+                     experts=2, out=p)
+    none = ax.QTensor(torch.empty(0, dtype=torch.uint8, device="cuda"), (2 * 32, 0), ax.QuantFormat.Q4_K)
+    down = ax.QTensor(torch.empty(0, dtype=torch.uint8, device="cuda"), (0, 32), ax.QuantFormat.Q4_K)
+    with pytest.raises(ax.AxqError, match="hidden must be positive"):
+        ax.moe_q(torch.zeros(2, 0, device="cuda"), torch.zeros(2, 0, device="cuda"), none, none, down, 1)
