@@ -7,7 +7,10 @@
 // infinity makes its block's scale infinite, so the block decodes to NaN.
 //
 // HBM-bound: every element is read once (the block stays in registers between
-// the maximum and the rounding) and one byte written.
+// the maximum and the rounding) and one byte written.  Weights 28672 x 8192 fp32
+// take 234 us, 4.9 TB/s; activations 2500 x 8200 fp16 16 us (issue-bound: the
+// exact division is two FMAs and a product for each element); one row of 4096
+// 2.4 us, a launch.
 #include <algorithm>
 
 #include "axq_common.cuh"

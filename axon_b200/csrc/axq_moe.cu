@@ -3,11 +3,12 @@
 //   y[t]   = sum_j p[t][j] * W_down[e] . (silu(W_gate[e] . x) * (W_up[e] . x)),
 //            e = ids[t][j].
 //
-// HBM-bound on the packed bytes of the experts that some token chose; each is
-// read once per group of up to 8 of its tokens.
+// It has to read the packed bytes of the experts that some token chose; each is
+// read once per group of up to 8 of its tokens.  What bounds it is decoding them.
 //
 //  * moe_route_kernel: a cluster of 8 CTAs per 4 tokens splits the experts, its
-//    first CTA picks the top_k.
+//    first CTA picks the top_k (4 to 6 us: a load's latency, the cluster's
+//    exchange, top_k rounds of warp maxima).
 //  * moe_prep_kernel: the plan (tokens' choices sorted by expert, in groups), and
 //    records of x: per 256 elements one or two fp16 terms (x 2^-e = hi or ~ hi +
 //    lo, 22 bits) in the order of the weights' MMA fragments, and sums for the
@@ -15,13 +16,23 @@
 //  * moe_expert_kernel: a producer warp streams packed rows through a ring of
 //    shared-memory stages (bulk copies); eight consumer warps decode them into
 //    exact fp16 fragments (axq_moe_decode.cuh) and multiply with mma.sync
-//    m16n8k16, whose 8 columns are eight tokens or the two terms of four.  Runs twice: gate
-//    and up (tile 0 and 1 of a unit are 16 rows of each, joined by silu), and
-//    down (32 rows).  mma.sync and not tcgen05: the weights are decoded in
-//    registers, and with at most 8 columns the tensor pipe is idle most of the
-//    time either way.
+//    m16n8k16, whose 8 columns are eight tokens or the two terms of four.  Runs
+//    twice: gate and up (tile 0 and 1 of a unit are 16 rows of each, joined by
+//    silu), and down (32 rows).  A finisher warp joins the consumers' sums of a
+//    round beside the next one.  mma.sync and not tcgen05: the weights are decoded
+//    in registers, and with at most 8 columns the tensor pipe is idle most of the
+//    time either way.  Bound by the decoders' integer and fp16 instructions (3 per
+//    weight of Q4_K, 5.8 of Q6_K) at the half issue rate that 20 warps of 96
+//    registers reach: 304 MB of Q4_K in 104 us (2.9 TB/s), 223 MB of Q6_K in 108,
+//    114 MB of Q3_K in 84, 185 MB of e4m3, which needs few, in 45 (4.1 TB/s).
 //  * moe_combine_kernel: y from the experts' products, in the order of the
 //    token's choices (no atomics on values: results do not depend on timing).
+//    It, the plan and the records take 2 to 5 us each.
+//
+// A form of three kernels for few choices, where every CTA made the plan and the
+// last to finish a part wrote the hidden records and y, was no faster for one token
+// (44.7 us) and slower for four (194 against 180): the counting of parts, with its
+// fences, kept the finisher behind the consumers.
 #include <algorithm>
 
 #include "axq_common.cuh"
@@ -104,8 +115,6 @@ struct RecordArgs {
     uint8_t* rec;
     const int* need;  // rows whose expert id is out of range are skipped; null: none
     int experts;
-    int* clear;       // counters of the kernels behind this one, set to 0
-    int nclear;
 };
 
 // Record `it` (row-major over rows and CGs) by one warp, through its 256 floats.
@@ -136,13 +145,10 @@ __global__ void __launch_bounds__(32 * kPrepWarps) moe_prep_kernel(const T* __re
     pdl_wait();
     pdl_launch_dependents();
     if (plan.ids && blockIdx.x == 0) {
-        moe_make_plan(plan);
+        moe_make_plan<32 * kPrepWarps>(plan);
         return;
     }
-    if (plan.err && !plan.ids && blockIdx.x == 0 && threadIdx.x == 0) *plan.err = 0;
     const int64_t b = blockIdx.x - (plan.ids ? 1 : 0);
-    for (int64_t c = b * (32 * kPrepWarps) + threadIdx.x; c < a.nclear; c += static_cast<int64_t>(gridDim.x) * (32 * kPrepWarps))
-        a.clear[c] = 0;
     record_of(a, x, b * kPrepWarps + warp, buf[warp], lane);
 }
 
@@ -154,15 +160,73 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// The top_k of a token of the cluster, by one warp.  Logits become keys whose order
+// as integers is theirs (NaN 1, chosen ones 0); lane e % 32 holds the best of its own.
+__device__ __forceinline__ void route_token(float* logits, int* ids, float* wt, int token, int lane, int experts, int top_k,
+                                            int slices, int normalize) {
+    uint32_t* keys = reinterpret_cast<uint32_t*>(logits) + token * experts;
+    uint32_t best = 0;
+    int best_e = INT32_MAX;
+    for (int e = lane; e < experts; e += 32) {
+        const float* l = logits + token * experts + e;
+        float v = l[0];
+        for (int sl = 1; sl < slices; ++sl) v += l[sl * kRouteTokens * experts];
+        const uint32_t b = __float_as_uint(v);
+        const uint32_t k = isnan(v) ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+        keys[e] = k;
+        if (k > best) {
+            best = k;
+            best_e = e;
+        }
+    }
+    auto value = [](uint32_t k) {
+        return k == 1u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+    };
+    float mine = 0.0f, sum = 0.0f, mx = 0.0f;
+    int my_id = 0;
+    if (!normalize) {  // the sum over all experts, before the chosen ones are marked
+        mx = value(__reduce_max_sync(0xFFFFFFFFu, best));
+        for (int e = lane; e < experts; e += 32) sum += expf(value(keys[e]) - mx);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    }
+    for (int j = 0; j < top_k; ++j) {
+        const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
+        const int e = __reduce_min_sync(0xFFFFFFFFu, best == m ? best_e : INT32_MAX);  // ties: the lowest index
+        if (j == 0) mx = value(m);
+        const float p = expf(value(m) - mx);
+        if (normalize) sum += p;
+        if (lane == j) {
+            mine = p;
+            my_id = e;
+        }
+        if (lane == (e & 31)) {
+            keys[e] = 0;
+            best = 0;
+            best_e = INT32_MAX;
+            for (int q = lane; q < experts; q += 32)
+                if (keys[q] > best) {
+                    best = keys[q];
+                    best_e = q;
+                }
+        }
+        __syncwarp();
+    }
+    if (lane < top_k) {
+        ids[lane] = my_id;
+        wt[lane] = mine / sum;
+    }
+}
+
 // Logits in fp32 (FMAs over lanes of 128 columns, then a tree over the lanes,
 // then the slices in order); ties go to the lowest index, NaN logits are chosen
 // last.  The cluster's 128 warps take (expert, slice of the columns) each:
 // latency counts here, so few experts are cut into slices.
 template <typename T>
 __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRouteWarps)
-    moe_route_kernel(const T* __restrict__ x, const float* __restrict__ w, int* __restrict__ ids, float* __restrict__ wt,
+    moe_route_kernel(const T* __restrict__ x, const float* __restrict__ w, int* ids, float* wt,
                      int64_t tokens, int experts, int top_k, int64_t hidden, int slices, int normalize, bool vec,
-                     RecordArgs records, int* err) {
+                     RecordArgs records, MoePlan plan) {
     extern __shared__ float logits[];  // [slice][kRouteTokens][experts], of the cluster's first CTA
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -174,9 +238,6 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
         const int b = static_cast<int>(blockIdx.x) - first;
         pdl_wait();
         pdl_launch_dependents();
-        if (b == 0 && threadIdx.x == 0) *err = 0;
-        for (int c = b * (32 * kRouteWarps) + threadIdx.x; c < records.nclear; c += (gridDim.x - first) * (32 * kRouteWarps))
-            records.clear[c] = 0;
         record_of(records, x, static_cast<int64_t>(b) * kRouteWarps + warp, buf[warp], lane);
         return;
     }
@@ -234,61 +295,11 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
     }
     if (!there) cluster_wait();
     cluster_sync_all();
-    if (rank != 0 || warp >= nt) return;
-    // One warp per token.  Logits become keys whose order as integers is theirs
-    // (NaN 1, chosen ones 0); lane e % 32 holds the best of its own.
-    uint32_t* keys = reinterpret_cast<uint32_t*>(logits) + warp * experts;
-    uint32_t best = 0;
-    int best_e = INT32_MAX;
-    for (int e = lane; e < experts; e += 32) {
-        const float* l = logits + warp * experts + e;
-        float v = l[0];
-        for (int sl = 1; sl < slices; ++sl) v += l[sl * kRouteTokens * experts];
-        const uint32_t b = __float_as_uint(v);
-        const uint32_t k = isnan(v) ? 1u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-        keys[e] = k;
-        if (k > best) {
-            best = k;
-            best_e = e;
-        }
-    }
-    auto value = [](uint32_t k) {
-        return k == 1u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
-    };
-    float mine = 0.0f, sum = 0.0f, mx = 0.0f;
-    int my_id = 0;
-    if (!normalize) {  // the sum over all experts, before the chosen ones are marked
-        mx = value(__reduce_max_sync(0xFFFFFFFFu, best));
-        for (int e = lane; e < experts; e += 32) sum += expf(value(keys[e]) - mx);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    }
-    for (int j = 0; j < top_k; ++j) {
-        const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, best);
-        const int e = __reduce_min_sync(0xFFFFFFFFu, best == m ? best_e : INT32_MAX);  // ties: the lowest index
-        if (j == 0) mx = value(m);
-        const float p = expf(value(m) - mx);
-        if (normalize) sum += p;
-        if (lane == j) {
-            mine = p;
-            my_id = e;
-        }
-        if (lane == (e & 31)) {
-            keys[e] = 0;
-            best = 0;
-            best_e = INT32_MAX;
-            for (int q = lane; q < experts; q += 32)
-                if (keys[q] > best) {
-                    best = keys[q];
-                    best_e = q;
-                }
-        }
-        __syncwarp();
-    }
-    if (lane < top_k) {
-        ids[(t0 + warp) * top_k + lane] = my_id;
-        wt[(t0 + warp) * top_k + lane] = mine / sum;
-    }
+    if (rank != 0) return;
+    if (warp < nt) route_token(logits, ids + (t0 + warp) * top_k, wt + (t0 + warp) * top_k, warp, lane, experts, top_k, slices, normalize);
+    if (!plan.ids) return;  // else this is the only cluster with tokens
+    __syncthreads();
+    moe_make_plan<32 * kRouteWarps>(plan);
 }
 
 // ---- experts -------------------------------------------------------------------------
@@ -296,10 +307,18 @@ __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(32 * kRoute
 constexpr int kConsumers = 8;
 constexpr int kMoeThreads = (kConsumers + 2) * 32;  // and the producer and the finisher
 constexpr int kMoeStages = 8;  // most
+// The rounds a CTA has named to its warps and not all of them have done with: one
+// for each stage at most, one being named, three by which the finisher lags.
+constexpr int kMoeNamed = 16;
+static_assert(kMoeStages + 4 < kMoeNamed);
+constexpr int kMoeGroup = 8;  // tokens of a group, at most
 
 struct MoeBars {
     uint64_t full[kMoeStages], empty[kMoeStages];
     uint64_t sums[2], joined[2];  // a round's partial sums are written, and joined
+    uint64_t named[kMoeNamed];    // the q-th round of this CTA is at q % kMoeNamed:
+    int4 round[kMoeNamed];        // expert, tokens, group (-1: no more), first unit
+    int2 entry[kMoeNamed][kMoeGroup];
     int abort;
 };
 
@@ -319,27 +338,10 @@ struct ExpertArgs {
     int64_t rec_row;       // bytes of a record row
     int rec_token;         // a pair's record row is its token's, else its own
     float* out;            // [pair][rows]
-    MoePlan plan;          // ids set: few choices, planned by every CTA
-    // With few choices whoever finishes the last part of something finishes it:
-    // the records of 256 hidden activations (gate and up), or 32 columns of y
-    // (down).  counters count the parts done.
-    int* counters;
-    int h_fmt, h_terms, h_ncg;
-    uint8_t* h_rec;
-    const float* wt;
-    void* y;
-    int y_dtype;
-    int64_t tokens;
+    int* next;             // rounds taken beyond the first of each CTA
+    MoePlan plan;
     int* err;
 };
-
-// The plan as a CTA uses it, from the plan kernel's memory or its own.
-struct PlanView {
-    const int4* groups;
-    const int2* entries;
-    int ngroups;
-};
-
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -519,6 +521,11 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int g, int 
 // half an SM's shared memory, else one after the other.
 template <int F, int NB>
 constexpr int kStageTiles = NB == 1 && (F == F_Q4_K || F == F_Q4_0) ? 2 : 1;
+// Tiles of a unit.  Two hold 16 rows of gate and 16 of up, or 32 rows of down; one
+// 8 and 8, or 16.  The smaller unit shares the SMs better; the larger one lets its
+// tiles share the activations, where they are taken together or stay in registers.
+template <int F, int NB>
+constexpr int kUnitTiles = F == F_F8 ? 2 : kStageTiles<F, NB>;
 // Rows whose packed length is a multiple of 16 start on one.
 template <int F>
 constexpr bool kAlignedRows = F == F_Q4_K || F == F_Q5_K || F == F_F8;
@@ -559,41 +566,42 @@ __device__ __forceinline__ float moe_combined(const float* z, const int* ids, co
 }
 
 // Row (of the expert) of tile `tile` and row r of unit `unit`.
+template <int UT>
 __device__ __forceinline__ int64_t stage_row(const ExpertArgs& a, int unit, int tile, int r) {
-    return a.gate_up ? static_cast<int64_t>(unit) * 16 + r : static_cast<int64_t>(unit) * 32 + 16 * tile + r;
+    return a.gate_up ? static_cast<int64_t>(unit) * (8 * UT) + (UT == 1 ? r & 7 : r)
+                     : static_cast<int64_t>(unit) * (16 * UT) + 16 * tile + r;
 }
 
-// A round: `slots` units of one group, from unit t0.  Rounds are walked in
-// order, so no division is needed after the first.
+// A round: `slots` units of one group, from unit t0.
 struct MoeRound {
-    int grp, t0;
-    __device__ __forceinline__ void next(const ExpertArgs& a) {
-        t0 += a.slots;
-        if (t0 >= a.tiles) {
-            t0 = 0;
-            ++grp;
-        }
-    }
+    int expert, tokens, grp, t0;
+    const int2* entries;
 };
+// The CTA's q-th round; grp < 0: there is none.
+__device__ __forceinline__ MoeRound moe_round(MoeBars& bars, int q, int* err) {
+    const int at = q % kMoeNamed;
+    if (!moe_wait(&bars.named[at], (q / kMoeNamed) & 1, &bars, err)) return MoeRound{0, 0, -1, 0, nullptr};
+    const int4 r = bars.round[at];
+    return MoeRound{r.x, r.y, r.z, r.w, bars.entry[at]};
+}
 
 // Joins the warps' partial sums (rb) of a round and writes its results (one warp).
-template <int kTok>
-__device__ __forceinline__ void moe_results(const ExpertArgs& a, const PlanView& pl, const float* rb, const MoeRound& rd,
-                                            int lane) {
-    const int4 gd = pl.groups[rd.grp];
-    const int rs = a.gate_up ? 4 : 5;  // log2 of a unit's rows
-    const int outputs = gd.z << rs;    // of a unit
+template <int kTok, int UT>
+__device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb, const MoeRound& rd, int lane) {
+    const int rs = (a.gate_up ? 2 : 3) + UT;  // log2 of a unit's rows
+    const int outputs = rd.tokens << rs;         // of a unit
     for (int un = 0; un < a.slots && rd.t0 + un < a.tiles; ++un) {
         for (int o = lane; o < outputs; o += 32) {
             const int rr = o & ((1 << rs) - 1), t = o >> rs;
             const int64_t row = (static_cast<int64_t>(rd.t0 + un) << rs) + rr;
             // the warps' parts are loaded together and added in order
             float part[2][kConsumers];
-            const float* q = rb + (un * a.wps * 2 * kTok + t) * 16 + (a.gate_up ? rr : (rr >> 4) * kTok * 16 + (rr & 15));
+            const float* q = rb + (un * a.wps * UT * kTok + t) * 16 + (rr >> 4) * kTok * 16 + (rr & 15);
+            const int up = UT == 2 ? kTok * 16 : 8;  // from a row of gate to that of up
 #pragma unroll
             for (int w = 0; w < kConsumers; ++w) {
-                part[0][w] = w < a.wps ? q[w * 2 * kTok * 16] : 0.0f;
-                part[1][w] = a.gate_up && w < a.wps ? q[(w * 2 + 1) * kTok * 16] : 0.0f;
+                part[0][w] = w < a.wps ? q[w * UT * kTok * 16] : 0.0f;
+                part[1][w] = a.gate_up && w < a.wps ? q[w * UT * kTok * 16 + up] : 0.0f;
             }
             float v[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -602,55 +610,7 @@ __device__ __forceinline__ void moe_results(const ExpertArgs& a, const PlanView&
                 v[1] += part[1][w];
             }
             const float z = a.gate_up ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
-            if (row < a.rows) a.out[static_cast<int64_t>(pl.entries[gd.y + t].x) * a.rows + row] = z;
-        }
-    }
-}
-
-__device__ __forceinline__ void store_y(const ExpertArgs& a, int64_t at, float v) {
-    if (a.y_dtype == AXQ_DT_F32) static_cast<float*>(a.y)[at] = v;
-    else if (a.y_dtype == AXQ_DT_F16) static_cast<__half*>(a.y)[at] = Elem<__half>::put(v);
-    else static_cast<__nv_bfloat16*>(a.y)[at] = Elem<__nv_bfloat16>::put(v);
-}
-
-// After a round's results, with few choices: counts the units done, and finishes
-// what this round completed (one warp).
-__device__ __forceinline__ void moe_finish(const ExpertArgs& a, const PlanView& pl, const MoeRound& rd, float* buf, int lane) {
-    for (int un = 0; un < a.slots && rd.t0 + un < a.tiles; ++un) {
-        const int unit = rd.t0 + un;
-        __threadfence();  // the results, before the count
-        __syncwarp();
-        int done = 0;
-        if (lane == 0) {
-            const int at = a.gate_up ? rd.grp * a.h_ncg + (unit >> 4) : unit;
-            const int parts = a.gate_up ? min(16, a.tiles - (unit & ~15)) : pl.ngroups;
-            done = atomicAdd(a.counters + at, 1) == parts - 1;
-        }
-        if (!__shfl_sync(0xFFFFFFFFu, done, 0)) continue;
-        __threadfence();  // the count, before the others' results
-        if (a.gate_up) {
-            // the records of the group's 256 hidden activations
-            const int4 gd = pl.groups[rd.grp];
-            const int cg = unit >> 4;
-            for (int t = 0; t < gd.z; ++t) {
-                const int64_t p = pl.entries[gd.y + t].x;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t k = cg * 256 + 32 * j + lane;
-                    buf[32 * j + lane] = k < a.rows ? __ldcg(a.out + p * a.rows + k) : 0.0f;
-                }
-                __syncwarp();
-                write_record(a.h_fmt, a.h_terms, buf, a.h_rec + (p * a.h_ncg + cg) * rec_bytes(a.h_terms), lane);
-                __syncwarp();
-            }
-        } else {
-            const int64_t c = static_cast<int64_t>(unit) * 32 + lane;
-            if (c < a.rows) {
-#pragma unroll 2
-                for (int64_t t = 0; t < a.tokens; ++t)
-                    store_y(a, t * a.rows + c, moe_combined(a.out, a.plan.ids, a.wt, t, c, a.rows, a.plan.top_k, a.plan.experts));
-            }
-            __syncwarp();
+            if (row < a.rows) a.out[static_cast<int64_t>(rd.entries[t].x) * a.rows + row] = z;
         }
     }
 }
@@ -660,7 +620,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
     using C = Cols<T>;
     constexpr int CGB = moe_cg_bytes<F>();
     constexpr int kTok = C::kTokens * NB;
-    constexpr int TL = kStageTiles<F, NB>;
+    constexpr int TL = kStageTiles<F, NB>, UT = kUnitTiles<F, NB>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127);
     float* red = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // the warps' sums of two rounds
@@ -675,30 +635,15 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
             mbar_init(&bars.sums[s], kConsumers);
             mbar_init(&bars.joined[s], 1);
         }
+        for (int s = 0; s < kMoeNamed; ++s) mbar_init(&bars.named[s], 1);
         bars.abort = 0;
         fence_mbar_init();
     }
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ MoeFewPlan few;
-    PlanView pl{a.plan.groups, a.plan.entries, 0};
-    if (a.plan.ids) {
-        moe_few_plan(few, a.plan);
-        pl = PlanView{few.groups, few.entries, few.ngroups};
-        if (pl.ngroups == 0 && !a.gate_up)  // no token chose an expert of this layer
-            for (int64_t o = static_cast<int64_t>(blockIdx.x) * kMoeThreads + threadIdx.x; o < a.tokens * a.rows;
-                 o += static_cast<int64_t>(gridDim.x) * kMoeThreads)
-                store_y(a, o, 0.0f);
-    } else {
-        pl.ngroups = *a.plan.ngroups;
-    }
     const int per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group; all fit 32 bits (checked on the host)
-    const int rounds = pl.ngroups * per;
-    const int lo = static_cast<int>(static_cast<int64_t>(rounds) * blockIdx.x / gridDim.x);
-    const int hi = static_cast<int>(static_cast<int64_t>(rounds) * (blockIdx.x + 1) / gridDim.x);
-    MoeRound rd{lo / per, 0};
-    rd.t0 = (lo - rd.grp * per) * a.slots;
+    const int rounds = *a.plan.ngroups * per;
     const int ksteps = (a.ncg + a.wps - 1) / a.wps;
 
     if (warp == kConsumers) {
@@ -709,20 +654,44 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         int64_t issued = 0;
         constexpr int kMost = TL == 2 ? 4 : 2;  // rows of a stage that a lane copies, at most (four slots)
         const int srows = a.slots * 16 * TL;
-        for (int n = lo; n < hi && ok; ++n, rd.next(a)) {
+        // A CTA's share of the rounds, rounded down, is consecutive (mostly of one group, whose activations stay in L1);
+        // the rest are taken by whoever is free, their numbers asked for a round ahead.  All of them shared out
+        // beforehand left SMs idle (194 against 173 us for four tokens); three quarters beforehand, the rest taken: 180.
+        const int own = max(1, rounds / static_cast<int>(gridDim.x));
+        int n = blockIdx.x * own;
+        for (int q = 0; ok; ++q) {
+            const int at = q % kMoeNamed;
+            if (n >= rounds) {
+                if (lane == 0) {
+                    bars.round[at] = make_int4(0, 0, -1, 0);
+                    mbar_arrive(&bars.named[at]);
+                }
+                break;
+            }
+            int after = n + 1;
+            if (q + 1 >= own && lane == 0) after = static_cast<int>(gridDim.x) * own + atomicAdd(a.next, 1);
+            const int grp = n / per;
+            const int4 gd = a.plan.groups[grp];  // expert, first entry, number of entries
+            const MoeRound rd{gd.x, gd.z, grp, (n - grp * per) * a.slots, nullptr};
+            if (lane < gd.z) bars.entry[at][lane] = a.plan.entries[gd.y + lane];
+            if (lane == 0) bars.round[at] = make_int4(rd.expert, rd.tokens, grp, rd.t0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.named[at]);
             // where this lane's rows of a stage begin (of tile 0, if a stage holds one tile); -1: no such row
-            const int64_t expert = pl.groups[rd.grp].x;
+            const int64_t expert = rd.expert;
             int64_t at0[kMost];
 #pragma unroll
             for (int j = 0; j < kMost; ++j) {
                 const int sr = lane + 32 * j, u = sr / (16 * TL), r = sr & (16 * TL - 1);
-                const int64_t row = stage_row(a, rd.t0 + u, TL == 2 ? r >> 4 : 0, r & 15);
+                const int64_t row = stage_row<UT>(a, rd.t0 + u, TL == 2 ? r >> 4 : 0, r & 15);
                 at0[j] = sr < srows && rd.t0 + u < a.tiles && row < a.rows ? (expert * a.rows + row) * a.rb : -1;
             }
-            for (int step = 0; step < ksteps * (2 / TL); ++step) {
-                const int k = step / (2 / TL), tile = step & 1;  // the tile counts where a stage holds one
+            for (int step = 0; step < ksteps * (UT / TL); ++step) {
+                const int k = step / (UT / TL), tile = step & (UT / TL - 1);
+                // the matrix of row sr of the stage (both are the same for the down product)
+                auto matrix = [&](int sr) { return a.w[UT == 1 ? (sr >> 3) & 1 : TL == 2 ? (sr >> 4) & 1 : tile]; };
                 // tile 1 of the down product is 16 rows on, and may lie past the last row
-                const int64_t skip = TL == 1 && tile && !a.gate_up ? 16 * a.rb : 0;
+                const int64_t skip = tile && !a.gate_up ? 16 * a.rb : 0;
                 const int64_t end = (expert + 1) * a.rows * a.rb;
                 const int64_t off = static_cast<int64_t>(k) * a.wps * CGB;
                 const int64_t seg = min64(static_cast<int64_t>(a.wps) * CGB, a.row_bytes - off);
@@ -741,7 +710,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                     if (to <= a.w_bytes) {
                         tx += len[j] = static_cast<uint32_t>(to - from);
                     } else {  // the rounded end would leave the buffer: bytes one by one
-                        const uint8_t* src = a.w[TL == 2 ? (sr >> 4) & 1 : tile] + at;
+                        const uint8_t* src = matrix(sr) + at;
                         uint8_t* dst = st + sr * a.rs + (at & 15);
                         for (int64_t c = 0; c < seg; ++c) dst[c] = src[c];
                     }
@@ -754,8 +723,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                 for (int j = 0; j < kMost; ++j) {
                     const int sr = lane + 32 * j;
                     if (len[j])
-                        bulk_g2s_hint(st + sr * a.rs,
-                                      a.w[TL == 2 ? (sr >> 4) & 1 : tile] + ((at0[j] + skip + off) & ~int64_t(15)), len[j],
+                        bulk_g2s_hint(st + sr * a.rs, matrix(sr) + ((at0[j] + skip + off) & ~int64_t(15)), len[j],
                                       &bars.full[s], policy);
                 }
                 ++issued;
@@ -764,6 +732,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                     par ^= 1;
                 }
             }
+            n = __shfl_sync(0xFFFFFFFFu, after, 0);
         }
         if (!ok)  // copies still in flight land before the shared memory goes away
             for (int64_t i = max(int64_t(0), issued - a.stages); i < issued; ++i)
@@ -771,16 +740,16 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         return;
     }
 
-    constexpr int kSums = kConsumers * 2 * kTok * 16;  // [warp][tile][token][16 rows]
+    constexpr int kSums = kConsumers * UT * kTok * 16;  // [warp][tile][token][16 rows]
     if (warp > kConsumers) {
         // The finisher joins each round's sums beside the consumers, which go on; it needs no registers that the SM has
         // not left over (18 and 20 warps share its schedulers alike).
-        for (int q = 0; q < hi - lo; ++q, rd.next(a)) {
-            if (!moe_wait(&bars.sums[q & 1], (q >> 1) & 1, &bars, a.err)) break;
-            moe_results<kTok>(a, pl, red + (q & 1) * kSums, rd, lane);
+        for (int q = 0;; ++q) {
+            const MoeRound rd = moe_round(bars, q, a.err);
+            if (rd.grp < 0 || !moe_wait(&bars.sums[q & 1], (q >> 1) & 1, &bars, a.err)) break;
+            moe_results<kTok, UT>(a, red + (q & 1) * kSums, rd, lane);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.joined[q & 1]);
-            if (a.plan.ids) moe_finish(a, pl, rd, red + 2 * kSums, lane);
         }
         return;
     }
@@ -790,31 +759,32 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
     int s = 0;
     uint32_t par = 0;
     bool ok = true;
-    for (int q = 0; q < hi - lo; ++q, rd.next(a)) {
+    for (int q = 0;; ++q) {
+        const MoeRound rd = moe_round(bars, q, a.err);
+        if (rd.grp < 0) break;
         const int unit = rd.t0 + u;
-        const int4 gd = pl.groups[rd.grp];  // expert, first entry, number of entries
         // this lane's B column, and the scales of its sums' columns (columns past the group's end: its first token's)
         const uint8_t *rec0[NB], *scale0[NB][C::kOwn];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const int t = n * C::kTokens + C::token(g);
-            const int2 e = pl.entries[gd.y + (t < gd.z ? t : 0)];
+            const int2 e = rd.entries[t < rd.tokens ? t : 0];
             rec0[n] = a.rec + (a.rec_token ? e.y : e.x) * a.rec_row + C::offset(g, i);
 #pragma unroll
             for (int v = 0; v < C::kOwn; ++v) {
                 const int ts = n * C::kTokens + C::own(i, v);
-                const int2 es = pl.entries[gd.y + (ts < gd.z ? ts : 0)];
+                const int2 es = rd.entries[ts < rd.tokens ? ts : 0];
                 scale0[n][v] = a.rec + (a.rec_token ? es.y : es.x) * a.rec_row + kRecScale<T>;
             }
         }
-        float tot[2][NB][2][C::kOwn];
+        float tot[UT][NB][2][C::kOwn];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < UT; ++t)
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int v = 0; v < C::kOwn; ++v) tot[t][n][0][v] = tot[t][n][1][v] = 0.0f;
-        const int64_t row0 = gd.x * a.rows + stage_row(a, unit, 0, 0);
+        const int64_t row0 = rd.expert * a.rows + stage_row<UT>(a, unit, 0, 0);
         for (int k = 0; k < ksteps; ++k) {
             const int cg = k * a.wps + col;
             const bool mine = cg < a.ncg && unit < a.tiles;
@@ -831,18 +801,18 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
             const uint32_t ph0 = kAlignedRows<F> ? 0u : static_cast<uint32_t>(row0) * static_cast<uint32_t>(a.rb) +
                                                             static_cast<uint32_t>(k * a.wps) * CGB;
             // e4m3: scales of the unit's rows (16 or 32 rows from a multiple of 16, so one block of 128)
-            const int64_t sc0 = F == F_F8 ? min64(row0, (gd.x + 1) * a.rows - 1) / 128 * a.nblk + 2 * cg : 0;
+            const int64_t sc0 = F == F_F8 ? min64(row0, (rd.expert + 1) * a.rows - 1) / 128 * a.nblk + 2 * cg : 0;
             const int blocks = a.nblk - (F == F_F8 ? 2 : 8) * cg;
             ActLines<F, T, NB> x;
 #pragma unroll
-            for (int h = 0; h < 2 / TL; ++h) {
+            for (int h = 0; h < UT / TL; ++h) {
                 if (h == 0 || kAhead<F, NB> < 8)
                     static_for_pairs<kAhead<F, NB>>([&](auto J) { x.template load<decltype(J)::value>(rec); });
                 if (ok) ok = moe_wait(&bars.full[s], par, &bars, a.err);
                 if (ok && mine) {
                     const uint8_t* st = ring + s * a.stage_bytes + u * (16 * TL) * a.rs + col * CGB;
                     const uint8_t* p[TL][2];
-                    const float* wsc[TL];
+                    const float* wsc[TL];  // e4m3, whose units have two tiles
 #pragma unroll
                     for (int t = 0; t < TL; ++t) {
                         const int tile = TL == 2 ? t : h;
@@ -851,8 +821,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                         if constexpr (!kAlignedRows<F>) {
                             // rows start where they do within their 16 bytes in memory
                             const uint32_t ph = ph0 + (g + (a.gate_up ? 0 : 16 * tile)) * static_cast<uint32_t>(a.rb);
-                            p[t][0] += ph & 15u;
-                            p[t][1] += (ph + 8 * static_cast<uint32_t>(a.rb)) & 15u;
+                            p[t][0] += ph & 15u;  // the second row is 8 on, but with 8 and 8 rows the same one of up
+                            p[t][1] += (ph + (UT == 1 && a.gate_up ? 0u : 8 * static_cast<uint32_t>(a.rb))) & 15u;
                         }
                         wsc[t] = F == F_F8 ? a.sc[tile] + sc0 : nullptr;
                     }
@@ -871,12 +841,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         if (ok && q > 1) ok = moe_wait(&bars.joined[q & 1], ((q >> 1) - 1) & 1, &bars, a.err);
         float* rb = red + (q & 1) * kSums;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < UT; ++t)
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int v = 0; v < C::kOwn; ++v) {
-                    float* to = rb + ((warp * 2 + t) * kTok + n * C::kTokens + C::own(i, v)) * 16;
+                    float* to = rb + ((warp * UT + t) * kTok + n * C::kTokens + C::own(i, v)) * 16;
                     to[g] = tot[t][n][0][v];
                     to[g + 8] = tot[t][n][1][v];
                 }
@@ -932,16 +902,17 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     // short rows: several units share a stage, so that every warp has a CG
     a.slots = a.ncg <= 2 ? 4 : a.ncg <= 4 ? 2 : 1;
     a.wps = kConsumers / a.slots;
-    a.tiles = static_cast<int>((a.rows + (a.gate_up ? 15 : 31)) / (a.gate_up ? 16 : 32));
+    const int unit_rows = (a.gate_up ? 8 : 16) * kUnitTiles<F, NB>;
+    a.tiles = static_cast<int>((a.rows + unit_rows - 1) / unit_rows);
     // row stride of a stage: the segment, its phase of up to 15 bytes, the 4 that word loads read past it, rounded
     // to an odd multiple of 16 so that eight rows start in different banks
     const int cgs = std::min(a.wps, a.ncg);
     a.rs = (cgs * CGB + 15 + 4 + 15) / 16 * 16;
     while (a.rs % 128 != 16) a.rs += 16;
     a.stage_bytes = a.slots * 16 * kStageTiles<F, NB> * a.rs;
-    // sums of two rounds, and with few choices 256 hidden activations on their way into a record
-    const int red = 2 * kConsumers * 2 * (8 / T) * NB * 16 * 4 + (a.plan.ids && a.gate_up ? 1024 : 0);
-    // two CTAs per SM, each with up to 3 KB besides (barriers, the plan of few choices, the driver's 1 KB)
+    // sums of two rounds
+    const int red = 2 * kConsumers * kUnitTiles<F, NB> * (8 / T) * NB * 16 * 4;
+    // two CTAs per SM, each with up to 3 KB besides (barriers and rounds, the driver's 1 KB)
     const int budget = 109 * 1024 - 512 - red;
     a.stages = std::min(kMoeStages, budget / a.stage_bytes);
     int per_sm = 2;
@@ -975,18 +946,13 @@ cudaError_t launch_prep(const T* x, const RecordArgs& a, const MoePlan& plan, cu
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-// One warp writes the hidden records of a group and one the columns of y: more
-// tokens are faster with kernels of their own.
-constexpr int64_t kMoeFewTokens = 8;
-
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Tokens of one pass: their choices fit the plan.
 int64_t pass_tokens(int top_k) { return std::max<int64_t>(1, kMoePairs / top_k); }
 
 struct MoeSpace {
-    size_t plan, counters, rec_x, rec_h, h, z, total;
-    int64_t ncounters;
+    size_t plan, rec_x, rec_h, h, z, total;
 };
 
 MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
@@ -999,8 +965,6 @@ MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
         return r;
     };
     w.plan = take(kMoePlanBytes);
-    w.ncounters = kMoeFew * ((ffn + 255) / 256) + (hidden + 31) / 32;
-    w.counters = take(static_cast<size_t>(w.ncounters) * 4);
     w.rec_x = take(static_cast<size_t>(t) * ((hidden + 255) / 256) * kRec<2>);
     w.rec_h = take(static_cast<size_t>(p) * ((ffn + 255) / 256) * kRec<2>);
     w.h = take(static_cast<size_t>(p) * ffn * 4);
@@ -1010,7 +974,7 @@ MoeSpace moe_space(int64_t tokens, int top_k, int64_t hidden, int64_t ffn) {
 }
 
 cudaError_t launch_route(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens, int experts,
-                         int top_k, int64_t hidden, int normalize, const RecordArgs& records, int* err, cudaStream_t s) {
+                         int top_k, int64_t hidden, int normalize, const RecordArgs& records, const MoePlan& plan, cudaStream_t s) {
     return with_dtype(dtype, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         const bool vec = hidden % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
@@ -1023,7 +987,7 @@ cudaError_t launch_route(int dtype, const void* x, const float* w, int* ids, flo
         const size_t smem = static_cast<size_t>(slices) * kRouteTokens * experts * 4;
         cudaError_t e = launch_pdl(moe_route_kernel<T>, dim3(static_cast<unsigned>((clusters + extra) * kRouteCtas)),
                                    dim3(32 * kRouteWarps), smem, s, static_cast<const T*>(x), w, ids, weights, tokens,
-                                   experts, top_k, hidden, slices, normalize, vec, records, err);
+                                   experts, top_k, hidden, slices, normalize, vec, records, plan);
         return e == cudaSuccess ? cudaGetLastError() : e;
     });
 }
@@ -1036,13 +1000,13 @@ size_t moe_workspace_bytes(int64_t tokens, int top_k, int64_t hidden, int64_t ff
 
 cudaError_t moe_route_dispatch(int dtype, const void* x, const float* w, int* ids, float* weights, int64_t tokens,
                                int experts, int top_k, int64_t hidden, int normalize, cudaStream_t s) {
-    return launch_route(dtype, x, w, ids, weights, tokens, experts, top_k, hidden, normalize, RecordArgs{}, nullptr, s);
+    return launch_route(dtype, x, w, ids, weights, tokens, experts, top_k, hidden, normalize, RecordArgs{}, MoePlan{}, s);
 }
 
-// Passes of up to kMoePairs choices.  Few choices (kMoeFew) of few tokens take
-// three kernels: router (if given) and records of x, gate and up with the records
-// of the hidden activations, down with y; more take kernels of their own for the
-// plan, the hidden records and y, whose cost is small beside the experts'.
+// Passes of up to kMoePairs choices.  A pass is five kernels: router, with the
+// records of x and the plan; gate and up; records of the hidden activations; down;
+// y.  Without a router, or with more tokens than one cluster routes, the plan is a
+// kernel too (and with several passes or no router the records are with it).
 cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s) {
     const MoeSpace w = moe_space(m.tokens, m.top_k, m.hidden, m.ffn);
     auto* base = static_cast<uint8_t*>(ws);
@@ -1050,7 +1014,6 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
     const int size = host_dtype_size(m.dtype);
     // 16-bit x is one term; so are the hidden activations of a bf16 result, whose own rounding is 8 times theirs
     const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = m.dtype == AXQ_DT_BF16 ? 1 : 2;
-    const bool few = m.tokens <= kMoeFewTokens && m.tokens * m.top_k <= kMoeFew;
     const bool several = m.tokens > step;  // passes
     if (m.w_router && several) {
         cudaError_t e = moe_route_dispatch(m.dtype, m.x, m.w_router, m.ids, m.weights, m.tokens, m.experts, m.top_k, m.hidden,
@@ -1067,13 +1030,10 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         plan.group = group;
         plan.top_k = m.top_k;
         plan.err = t0 == 0 ? err : nullptr;
-        MoePlan made = plan;  // as the kernels behind the plan see it
-        if (!few) made.ids = nullptr;
         const void* x = static_cast<const uint8_t*>(m.x) + t0 * m.hidden * size;
         void* y = static_cast<uint8_t*>(m.y) + t0 * m.hidden * size;
         float* h = reinterpret_cast<float*>(base + w.h);
         float* z = reinterpret_cast<float*>(base + w.z);
-        int* counters = reinterpret_cast<int*>(base + w.counters);
         RecordArgs rx{};
         rx.fmt = m.fmt;
         rx.terms = terms_x;
@@ -1081,25 +1041,22 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         rx.cols = m.hidden;
         rx.ncg = static_cast<int>((m.hidden + 255) / 256);
         rx.rec = base + w.rec_x;
-        rx.clear = counters;
-        rx.nclear = few ? static_cast<int>(w.ncounters) : 0;
         cudaError_t e;
         const bool routed = m.w_router && !several;  // the router's kernel writes the records too
+        const bool planned = routed && t <= kRouteTokens;  // and makes the plan, if one cluster has all tokens
         if (routed) {
-            e = launch_route(m.dtype, x, m.w_router, m.ids, m.weights, t, m.experts, m.top_k, m.hidden, m.normalize, rx, err, s);
+            e = launch_route(m.dtype, x, m.w_router, m.ids, m.weights, t, m.experts, m.top_k, m.hidden, m.normalize, rx,
+                             planned ? plan : MoePlan{}, s);
             if (e != cudaSuccess) return e;
             rx.rows = 0;
-            plan.err = nullptr;
         }
-        if (!routed || !few) {
-            MoePlan first = plan;
-            if (few) first.ids = nullptr;  // records only
+        if (!planned) {
             e = with_dtype(m.dtype, [&](auto* tag) {
                 using T = std::remove_pointer_t<decltype(tag)>;
-                return launch_prep<T>(static_cast<const T*>(x), rx, first, s);
+                return launch_prep<T>(static_cast<const T*>(x), rx, plan, s);
             });
+            if (e != cudaSuccess) return e;
         }
-        if (e != cudaSuccess) return e;
         ExpertArgs a{};
         a.w[0] = static_cast<const uint8_t*>(m.w_gate);
         a.w[1] = static_cast<const uint8_t*>(m.w_up);
@@ -1113,49 +1070,38 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.rec_row = static_cast<int64_t>(rx.ncg) * rec_bytes(terms_x);
         a.rec_token = 1;
         a.out = h;
-        a.plan = made;
-        a.counters = counters;
-        a.h_fmt = m.fmt_down;
-        a.h_terms = terms_h;
-        a.h_ncg = static_cast<int>((m.ffn + 255) / 256);
-        a.h_rec = base + w.rec_h;
+        a.plan = plan;
+        a.next = plan.taken;
         a.err = err;
         if (e = launch_experts(m.fmt, a, m.hidden, terms_x, group, s); e != cudaSuccess) return e;
-        if (!few) {
-            RecordArgs rh{};
-            rh.fmt = m.fmt_down;
-            rh.terms = terms_h;
-            rh.rows = p;
-            rh.cols = m.ffn;
-            rh.ncg = a.h_ncg;
-            rh.rec = a.h_rec;
-            rh.need = plan.ids;
-            rh.experts = m.experts;
-            made.err = nullptr;
-            if (e = launch_prep<float>(h, rh, made, s); e != cudaSuccess) return e;
-        }
+        RecordArgs rh{};
+        rh.fmt = m.fmt_down;
+        rh.terms = terms_h;
+        rh.rows = p;
+        rh.cols = m.ffn;
+        rh.ncg = static_cast<int>((m.ffn + 255) / 256);
+        rh.rec = base + w.rec_h;
+        rh.need = plan.ids;
+        rh.experts = m.experts;
+        if (e = launch_prep<float>(h, rh, MoePlan{}, s); e != cudaSuccess) return e;
         a.w[0] = a.w[1] = static_cast<const uint8_t*>(m.w_down);
         a.sc[0] = a.sc[1] = m.s_down;
         a.rb = m.ffn;
         a.w_bytes = m.down_bytes;
         a.rows = m.hidden;
         a.gate_up = 0;
-        a.rec = a.h_rec;
-        a.rec_row = static_cast<int64_t>(a.h_ncg) * rec_bytes(terms_h);
+        a.rec = rh.rec;
+        a.rec_row = static_cast<int64_t>(rh.ncg) * rec_bytes(terms_h);
         a.rec_token = 0;
         a.out = z;
-        a.counters = counters + kMoeFew * a.h_ncg;
-        a.wt = m.weights + t0 * m.top_k;
-        a.y = y;
-        a.y_dtype = m.dtype;
-        a.tokens = t;
+        a.next = plan.taken + 1;
         if (e = launch_experts(m.fmt_down, a, m.ffn, terms_h, group, s); e != cudaSuccess) return e;
-        if (few) continue;
+        const float* wt = m.weights + t0 * m.top_k;
         e = with_dtype(m.dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             const int64_t grid = std::min<int64_t>((t * m.hidden + 255) / 256, int64_t(device_sm_count()) * 8);
             cudaError_t r = launch_pdl(moe_combine_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s,
-                                       static_cast<const float*>(z), static_cast<const int*>(plan.ids), a.wt, static_cast<T*>(y), t, m.hidden, m.top_k,
+                                       static_cast<const float*>(z), plan.ids, wt, static_cast<T*>(y), t, m.hidden, m.top_k,
                                        m.experts);
             return r == cudaSuccess ? cudaGetLastError() : r;
         });

@@ -8,91 +8,58 @@
 namespace axq {
 
 constexpr int kMoePairs = 512;     // choices of one pass, at most
-constexpr int kMoeFew = 64;        // choices that each CTA plans for itself, at most
 constexpr int kMoeExperts = 1024;  // experts, at most
 
 struct MoePlan {
-    const int* ids;  // null once the plan is made
-    int npairs, experts, group;
+    const int* ids;  // null: no plan to make
+    int npairs, experts, group, top_k;
     int* ngroups;
+    int* taken;      // counters of the rounds that the two products' CTAs have taken, set to 0
     int4* groups;    // expert, first entry, number of entries
     int2* entries;   // pair and its token, sorted by expert
-    int top_k;
     int* err;        // status word to clear, or null
 };
-
-// The plan of few choices, made by every CTA in its shared memory (no kernel
-// has to come between the choice of experts and their products).
-struct MoeFewPlan {
-    int4 groups[kMoeFew];
-    int2 entries[kMoeFew];
-    int ids[kMoeFew], rank[kMoeFew];
-    int ngroups;
-};
-
-// All threads of the block (at least kMoeFew) call it.
-__device__ __forceinline__ void moe_few_plan(MoeFewPlan& p, const MoePlan& m) {
-    const int tid = threadIdx.x;
-    if (tid < kMoeFew) p.ids[tid] = tid < m.npairs ? m.ids[tid] : -1;
-    __syncthreads();
-    const int mine = tid < kMoeFew ? p.ids[tid] : -1;
-    const bool valid = static_cast<unsigned>(mine) < static_cast<unsigned>(m.experts);
-    int before = 0, rank = 0, total = 0;
-    if (valid) {
-        for (int q = 0; q < m.npairs; ++q) {
-            const int e = p.ids[q];
-            before += (e >= 0 && e < mine) || (e == mine && q < tid) ? 1 : 0;
-            rank += e == mine && q < tid ? 1 : 0;
-            total += e == mine ? 1 : 0;
-        }
-    }
-    if (tid < kMoeFew) p.rank[tid] = valid ? rank % m.group : -1;
-    __syncthreads();
-    int starts = 0;  // groups that begin before this pair, and in all
-    int all = 0;
-    for (int q = 0; q < m.npairs; ++q) {
-        const int e = p.ids[q], s = p.rank[q] == 0 ? 1 : 0;
-        all += s;
-        starts += s && (e < mine || (e == mine && q < tid)) ? 1 : 0;
-    }
-    if (valid) {
-        p.entries[before] = make_int2(tid, tid / m.top_k);
-        if (rank % m.group == 0) p.groups[starts] = make_int4(mine, before, min(m.group, total - rank), 0);
-    }
-    if (tid == 0) p.ngroups = all;
-    __syncthreads();
-}
 
 constexpr size_t kMoePlanBytes = 256 + kMoePairs * 16 + kMoePairs * 8;
 
 inline MoePlan moe_plan_at(uint8_t* p) {
     MoePlan m{};
     m.ngroups = reinterpret_cast<int*>(p);
+    m.taken = m.ngroups + 1;
     m.groups = reinterpret_cast<int4*>(p + 256);
     m.entries = reinterpret_cast<int2*>(p + 256 + kMoePairs * 16);
     return m;
 }
 
-// Makes the plan with one block of 256 threads.  Ids out of range (a padded
+// Makes the plan with one block of kThreads threads.  Ids out of range (a padded
 // token, an expert held elsewhere) appear in no group.
+template <int kThreads>
 __device__ __forceinline__ void moe_make_plan(const MoePlan& m) {
-    __shared__ int ids[kMoePairs];
-    __shared__ int first[kMoeExperts];
-    __shared__ int warp_sum[2][8];
+    constexpr int kOwn = kMoeExperts / kThreads;  // experts of a thread
+    __shared__ int4 ids4[kMoePairs / 4];
+    __shared__ int first[kMoeExperts];  // counts, then first entries
+    __shared__ int warp_sum[2][kThreads / 32];
+    int* ids = reinterpret_cast<int*>(ids4);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid < 2) m.taken[tid] = 0;
     if (tid == 0 && m.err) *m.err = 0;
-    for (int p = tid; p < m.npairs; p += 256) ids[p] = m.ids[p];
-    __syncthreads();
-    // counts of experts 4 tid .. 4 tid + 3, then sums over the experts before
-    int cnt[4] = {0, 0, 0, 0};
-    for (int p = 0; p < m.npairs; ++p) {
-        const int d = ids[p] - 4 * tid;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) cnt[j] += (d == j && ids[p] < m.experts) ? 1 : 0;
+    for (int j = 0; j < kOwn; ++j) first[kOwn * tid + j] = 0;
+    for (int p = tid; p < (m.npairs + 3) / 4 * 4; p += kThreads) {
+        const int e = p < m.npairs ? m.ids[p] : -1;
+        ids[p] = static_cast<unsigned>(e) < static_cast<unsigned>(m.experts) ? e : -1;
     }
+    __syncthreads();
+    for (int p = tid; p < m.npairs; p += kThreads)
+        if (ids[p] >= 0) atomicAdd(&first[ids[p]], 1);
+    __syncthreads();
+    // sums over the experts before those of this thread
+    int cnt[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) cnt[j] = first[kOwn * tid + j];
     int c = 0, g = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kOwn; ++j) {
         c += cnt[j];
         g += (cnt[j] + m.group - 1) / m.group;
     }
@@ -115,22 +82,26 @@ __device__ __forceinline__ void moe_make_plan(const MoePlan& m) {
         cb += warp_sum[0][w];
         gb += warp_sum[1][w];
     }
-    if (tid == 255) *m.ngroups = gb + g;
+    if (tid == kThreads - 1) *m.ngroups = gb + g;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        first[4 * tid + j] = cb;
+    for (int j = 0; j < kOwn; ++j) {
+        first[kOwn * tid + j] = cb;
         for (int k = 0; k * m.group < cnt[j]; ++k)
-            m.groups[gb + k] = make_int4(4 * tid + j, cb + k * m.group, min(m.group, cnt[j] - k * m.group), 0);
+            m.groups[gb + k] = make_int4(kOwn * tid + j, cb + k * m.group, min(m.group, cnt[j] - k * m.group), 0);
         cb += cnt[j];
         gb += (cnt[j] + m.group - 1) / m.group;
     }
     __syncthreads();
     // a pair's place: after the earlier pairs of its expert
-    for (int p = tid; p < m.npairs; p += 256) {
+    for (int p = tid; p < m.npairs; p += kThreads) {
         const int e = ids[p];
-        if (static_cast<unsigned>(e) >= static_cast<unsigned>(m.experts)) continue;
+        if (e < 0) continue;
         int r = first[e];
-        for (int q = 0; q < p; ++q) r += ids[q] == e ? 1 : 0;
+#pragma unroll 4
+        for (int q = 0; q < p; q += 4) {
+            const int4 o = ids4[q / 4];
+            r += (o.x == e) + (o.y == e && q + 1 < p) + (o.z == e && q + 2 < p) + (o.w == e && q + 3 < p);
+        }
         m.entries[r] = make_int2(p, p / m.top_k);
     }
 }

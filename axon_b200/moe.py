@@ -113,7 +113,7 @@ def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: 
           out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None
           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The whole layer: what :func:`moe_route` and then :func:`moe_mlp_q` give, in
-    three kernels for up to 8 tokens with at most 64 choices.  Returns (y, ids, weights)."""
+    fewer kernels.  Returns (y, ids, weights)."""
     dtype = _float_type(x, "x")
     _plain(w_router, "w_router", torch.float32)
     if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:

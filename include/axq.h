@@ -329,8 +329,9 @@ int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const voi
                 const float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
                 int64_t ffn, void* workspace, size_t workspace_bytes, axq_stream_t stream);
 
-/* The whole layer: axq_moe_route into ids and weights, then axq_moe_mlp, in three
- * kernels for up to 8 tokens with at most 64 choices. */
+/* The whole layer: axq_moe_route into ids and weights, then axq_moe_mlp, with the
+ * router's kernel also preparing the activations (and, for up to 4 tokens, the
+ * order of the experts). */
 int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, int fmt_down,
             const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
             int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,
