@@ -7,27 +7,30 @@
 // read once per group of up to 8 of its tokens.  What bounds it is decoding them.
 //
 //  * moe_route_kernel: a cluster of 8 CTAs per 4 tokens splits the experts, its
-//    first CTA picks the top_k (4 to 6 us: a load's latency, the cluster's
-//    exchange, top_k rounds of warp maxima).
-//  * moe_prep_kernel: the plan (tokens' choices sorted by expert, in groups), and
-//    records of x: per 256 elements one or two fp16 terms (x 2^-e = hi or ~ hi +
+//    first CTA picks the top_k (latency: 5 to 8 us, of loads, the cluster's
+//    exchange and top_k rounds of warp maxima) and, if it has all tokens, makes the
+//    plan: the tokens' choices sorted by expert, in groups.  Other clusters write
+//    the records of x: per 256 elements one or two fp16 terms (x 2^-e = hi or ~ hi +
 //    lo, 22 bits) in the order of the weights' MMA fragments, and sums for the
 //    minimums.
+//  * moe_prep_kernel: plan and records where the router's kernel did not make them,
+//    and the records of the hidden activations.
 //  * moe_expert_kernel: a producer warp streams packed rows through a ring of
 //    shared-memory stages (bulk copies); eight consumer warps decode them into
 //    exact fp16 fragments (axq_moe_decode.cuh) and multiply with mma.sync
 //    m16n8k16, whose 8 columns are eight tokens or the two terms of four.  Runs
-//    twice: gate and up (tile 0 and 1 of a unit are 16 rows of each, joined by
-//    silu), and down (32 rows).  A finisher warp joins the consumers' sums of a
-//    round beside the next one.  mma.sync and not tcgen05: the weights are decoded
-//    in registers, and with at most 8 columns the tensor pipe is idle most of the
-//    time either way.  Bound by the decoders' integer and fp16 instructions (3 per
-//    weight of Q4_K, 5.8 of Q6_K) at the half issue rate that 20 warps of 96
-//    registers reach: 304 MB of Q4_K in 104 us (2.9 TB/s), 223 MB of Q6_K in 108,
-//    114 MB of Q3_K in 84, 185 MB of e4m3, which needs few, in 45 (4.1 TB/s).
+//    twice: gate and up (half of a unit's rows each, joined by silu), and down.  A
+//    finisher warp joins the consumers' sums of a round beside the next one.
+//    mma.sync and not tcgen05: the weights are decoded in registers, and with at
+//    most 8 columns the tensor pipe is idle most of the time either way.  Bound by
+//    the decoders' integer and fp16 instructions (3 per weight of Q4_K, 5.7 of
+//    Q6_K, 5 of Q3_K) at 55 to 60 % of the issue rate, which 20 warps of 96
+//    registers reach: 304 MB of Q4_K in 88 us (3.5 TB/s), 222 MB of Q6_K in 88, 114
+//    MB of Q3_K in 72; 185 MB of e4m3, which needs few instructions, in 39 (4.7
+//    TB/s).
 //  * moe_combine_kernel: y from the experts' products, in the order of the
 //    token's choices (no atomics on values: results do not depend on timing).
-//    It, the plan and the records take 2 to 5 us each.
+//    It, the plan and the hidden records take 2 to 5 us each, mostly their start.
 //
 // A form of three kernels for few choices, where every CTA made the plan and the
 // last to finish a part wrote the hidden records and y, was no faster for one token
