@@ -643,10 +643,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         fence_mbar_init();
     }
     __syncthreads();
-    pdl_wait();
-    pdl_launch_dependents();
-    const int per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group; all fit 32 bits (checked on the host)
-    const int rounds = *a.plan.ngroups * per;
+    // The producer of the down product starts before the records of the hidden activations are there: the kernel that
+    // writes them lets this one start only after gate and up have finished, and those began after the plan was made.
+    if (a.gate_up || warp != kConsumers) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     const int ksteps = (a.ncg + a.wps - 1) / a.wps;
 
     if (warp == kConsumers) {
@@ -660,6 +662,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
         // A CTA's share of the rounds, rounded down, is consecutive (mostly of one group, whose activations stay in L1);
         // the rest are taken by whoever is free, their numbers asked for a round ahead.  All of them shared out
         // beforehand left SMs idle (194 against 173 us for four tokens); three quarters beforehand, the rest taken: 180.
+        const int per = (a.tiles + a.slots - 1) / a.slots;  // rounds of a group; all fit 32 bits (checked on the host)
+        const int rounds = __ldcg(a.plan.ngroups) * per;
         const int own = max(1, rounds / static_cast<int>(gridDim.x));
         int n = blockIdx.x * own;
         for (int q = 0; ok; ++q) {
@@ -674,9 +678,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
             int after = n + 1;
             if (q + 1 >= own && lane == 0) after = static_cast<int>(gridDim.x) * own + atomicAdd(a.next, 1);
             const int grp = n / per;
-            const int4 gd = a.plan.groups[grp];  // expert, first entry, number of entries
+            const int4 gd = __ldcg(a.plan.groups + grp);  // expert, first entry, number of entries
             const MoeRound rd{gd.x, gd.z, grp, (n - grp * per) * a.slots, nullptr};
-            if (lane < gd.z) bars.entry[at][lane] = a.plan.entries[gd.y + lane];
+            if (lane < gd.z) bars.entry[at][lane] = __ldcg(a.plan.entries + gd.y + lane);
             if (lane == 0) bars.round[at] = make_int4(rd.expert, rd.tokens, grp, rd.t0);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.named[at]);

@@ -309,3 +309,34 @@ def test_overlaps_and_no_features_are_refused(cuda, orc):
     down = ax.QTensor(torch.empty(0, dtype=torch.uint8, device="cuda"), (0, 32), ax.QuantFormat.Q4_K)
     with pytest.raises(ax.AxqError, match="hidden must be positive"):
         ax.moe_q(torch.zeros(2, 0, device="cuda"), torch.zeros(2, 0, device="cuda"), none, none, down, 1)
+
+
+@pytest.mark.parametrize("T", [2, 24])
+def test_weights_packed_right_before_each_call(cuda, T):
+    """The kernels of a stream start early on one another: calls without a wait between them, on weights that are packed
+    anew in the same memory before each, against the same calls with a wait after every step."""
+    E, K, hidden, ffn = 4, 2, 512, 1024
+    g = torch.Generator(device="cuda").manual_seed(T)
+    src = [[torch.randn(E * r, c, device="cuda", generator=g) * 0.05 for r, c in ((ffn, hidden), (ffn, hidden), (hidden, ffn))]
+           for _ in range(3)]
+    xs = [torch.randn(T, hidden, device="cuda", generator=g) for _ in range(3)]
+    wr = torch.randn(E, hidden, device="cuda", generator=g)
+    w = [ax.F8Tensor.empty(*s.shape) for s in src[0]]
+    x = torch.empty_like(xs[0])
+
+    def call(i, wait):
+        steps = [lambda: x.copy_(xs[i])] + [lambda k=k: ax.quantize_f8(w[k], src[i][k]) for k in range(3)]
+        for s in steps:
+            s()
+            if wait:
+                torch.cuda.synchronize()
+        y = ax.moe_q(x, wr, *w, K)[0]
+        if wait:
+            torch.cuda.synchronize()
+        return y
+
+    want = [call(i, True) for i in range(3)]
+    got = [(i, call(i, False)) for _ in range(20) for i in range(3)]
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i])
