@@ -525,8 +525,9 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int g, int 
 template <int F, int NB>
 constexpr int kStageTiles = NB == 1 && (F == F_Q4_K || F == F_Q4_0) ? 2 : 1;
 // Tiles of a unit.  Two hold 16 rows of gate and 16 of up, or 32 rows of down; one
-// 8 and 8, or 16.  The smaller unit shares the SMs better; the larger one lets its
-// tiles share the activations, where they are taken together or stay in registers.
+// 8 and 8, or 16.  The smaller unit shares the SMs better (Q6_K, four tokens: 173
+// against 180 us for the layer); the larger one lets its tiles share the
+// activations, where they are taken together or stay in registers.
 template <int F, int NB>
 constexpr int kUnitTiles = F == F_F8 ? 2 : kStageTiles<F, NB>;
 // Rows whose packed length is a multiple of 16 start on one.

@@ -340,3 +340,24 @@ def test_weights_packed_right_before_each_call(cuda, T):
     torch.cuda.synchronize()
     for i, y in got:
         assert torch.equal(y, want[i])
+
+
+@pytest.mark.parametrize("T,E,K", [(4, 1000, 32), (1, 1000, 1), (4, 3, 3), (5, 1000, 32), (16, 1024, 32)])
+def test_plan_of_the_router_and_of_its_own_kernel(cuda, T, E, K):
+    """Many experts and choices: the layer, whose plan the router's kernel makes for up to 4 tokens, against its parts."""
+    g = torch.Generator(device="cuda").manual_seed(E)
+    q = []
+    for r, c in ((32, 64), (32, 64), (64, 32)):
+        w = ax.QTensor.empty(E * r, c, ax.QuantFormat.Q8_0)
+        ax.quantize(w, torch.randn(E * r, c, device="cuda", generator=g), ax.QuantFormat.Q8_0)
+        q.append(w)
+    x, wr = torch.randn(T, 64, device="cuda", generator=g), torch.randn(E, 64, device="cuda", generator=g)
+    y, ids, p = ax.moe_q(x, wr, *q, K)
+    ids2, p2 = ax.moe_route(x, wr, K)
+    assert torch.equal(ids, ids2) and torch.equal(p, p2)
+    assert torch.equal(y, ax.moe_mlp_q(x, ids, p, *q, experts=E))
+    # each choice by itself, weighed and added in fp32, within the rounding of K sums
+    for t in range(min(T, 2)):
+        parts = torch.cat([ax.moe_mlp_q(x[t:t + 1], ids[t:t + 1, j:j + 1].contiguous(), p[t:t + 1, j:j + 1].contiguous(), *q,
+                                        experts=E) for j in range(K)]).double()
+        assert ((y[t].double() - parts.sum(0)).abs() <= (K + 1) * 2.0 ** -23 * parts.abs().sum(0)).all()
