@@ -318,8 +318,7 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
  * and ffn multiples of 128); otherwise *_scales are NULL.  x and y are [tokens x
  * hidden] in dtype F32, F16 or BF16.  Products and sums are fp32 (x and the hidden
  * activations enter the tensor cores as fp16: one term for 16-bit x, which it holds,
- * two of 22 bits for fp32 x and for the hidden activations, one of 11 bits for those
- * of a bf16 y); y is rounded once.  Tokens beyond 512 / top_k take several passes
+ * two of 22 bits for fp32 x and for the hidden activations); y is rounded once.  Tokens beyond 512 / top_k take several passes
  * over the experts; tokens, hidden and ffn are at most 2^20.  y
  * overlaps neither x nor ids nor weights.  Calls that share a workspace (256-byte
  * aligned) must be ordered; its status is read by axq_workspace_status. */
