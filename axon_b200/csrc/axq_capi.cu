@@ -81,6 +81,20 @@ constexpr size_t kStatusBytes = 256;  // status words at the front of a workspac
 
 int check_device_ptr(const void* p, const char* what, const char* fn) { return check_ptr(p, what, fn); }
 
+int check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read, const char* fn) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        auto apart = [&](const Span& o) -> int {
+            if (!w->p || !o.p || !overlap(w->p, w->n, o.p, o.n)) return AXQ_OK;
+            return fail(AXQ_ERR_INVALID, std::string(fn) + ": " + w->what + " must not overlap " + o.what);
+        };
+        for (auto o = w + 1; o != written.end(); ++o)
+            if (int r = apart(*o)) return r;
+        for (const Span& o : read)
+            if (int r = apart(o)) return r;
+    }
+    return AXQ_OK;
+}
+
 int validate_matmul_ptrs(int fmt, const void* a_q, const void* b, const void* out, const char* fn) {
     if (!known_fmt(fmt)) return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": unsupported format " + std::to_string(fmt));
     if (int r = check_ptr(a_q, "a_q", fn)) return r;

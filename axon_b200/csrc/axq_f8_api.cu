@@ -1,5 +1,6 @@
 // C entry points of the 8-bit floating point blocks (include/axq.h):
 // argument checks and dispatch.  Nothing here allocates device memory.
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -27,11 +28,15 @@ int64_t nkb_of(int64_t cols) { return (cols + kF8Block - 1) / kF8Block; }
 
 bool float_dtype(int dtype) { return host_dtype_size(dtype) != 0; }
 
-// Codes and scales of a [rows x cols] matrix.
+// Row stride, then codes and scales, of a [rows x cols] matrix.
+int check_ld(int64_t ld, int64_t cols, const char* what, const char* fn) {
+    if (ld >= cols && ld % 16 == 0) return AXQ_OK;
+    return fail(AXQ_ERR_INVALID, std::string(fn) + ": the row stride of " + what + " must be a multiple of 16 of at least " +
+                                     std::to_string(cols) + " (got " + std::to_string(ld) + ")");
+}
+
 int check_codes(const void* codes, int64_t ld, const float* scales, int64_t cols, const char* what, const char* fn) {
-    if (ld < cols || ld % 16)
-        return fail(AXQ_ERR_INVALID, std::string(fn) + ": the row stride of " + what + " must be a multiple of 16 of at least " +
-                                         std::to_string(cols) + " (got " + std::to_string(ld) + ")");
+    if (int r = check_ld(ld, cols, what, fn)) return r;
     if (int r = check_device_ptr(codes, what, fn)) return r;
     if (int r = check_device_ptr(scales, (std::string("the scales of ") + what).c_str(), fn)) return r;
     if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4)
@@ -67,14 +72,16 @@ int axq_quantize_f8(int dtype, const void* src, void* codes, int64_t ld, float* 
     if (!float_dtype(dtype)) return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": unsupported dtype " + std::to_string(dtype));
     if (int r = check_blocks(rows, cols, block_rows, fn)) return r;
     if (rows == 0 || cols == 0) return AXQ_OK;
+    if (int r = check_ld(ld, cols, "codes", fn)) return r;
+    // the zeros behind the last row's codes are written too
+    const int64_t codes_bytes = (rows - 1) * ld + std::min(ld, nkb_of(cols) * kF8Block);
+    if (int r = check_apart({{codes, codes_bytes, "codes"}, {scales, scales_span(rows, cols, block_rows), "the scales"}},
+                            {{src, rows * cols * host_dtype_size(dtype), "src"}}, fn))
+        return r;
     if (int r = check_device_ptr(src, "src", fn)) return r;
     if (reinterpret_cast<uintptr_t>(src) % host_dtype_size(dtype))
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": src is not aligned to its element type");
     if (int r = check_codes(codes, ld, scales, cols, "codes", fn)) return r;
-    const int64_t src_span = rows * cols * host_dtype_size(dtype), scales_bytes = scales_span(rows, cols, block_rows);
-    if (overlap(src, src_span, codes, codes_span(rows, cols, ld)) || overlap(src, src_span, scales, scales_bytes) ||
-        overlap(codes, codes_span(rows, cols, ld), scales, scales_bytes))
-        return fail(AXQ_ERR_INVALID, std::string(fn) + ": src, codes and scales must not overlap");
     return status(f8_pack_dispatch(dtype, src, codes, ld, scales, rows, cols, block_rows, nullptr,
                                    reinterpret_cast<cudaStream_t>(stream)), fn);
 }

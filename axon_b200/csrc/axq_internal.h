@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <utility>
 #include <cuda_runtime.h>
@@ -32,6 +33,17 @@ inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
 }
+
+// A range of memory that a call names (p may be NULL: not given).
+struct Span {
+    const void* p;
+    int64_t n;
+    const char* what;
+};
+
+// AXQ_ERR_INVALID if a range that the call writes shares a byte with any other
+// one.  Looks at the numbers only, so it may run before the pointers are checked.
+int check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read, const char* fn);
 
 cudaError_t pack_dispatch(int fmt, const float* src, void* dst, int64_t rows, int64_t cols, cudaStream_t s);
 cudaError_t dequant_dispatch(int fmt, const void* src, float* dst, int64_t rows, int64_t cols, cudaStream_t s);
