@@ -122,6 +122,21 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
     if (M == 0 || N == 0) return AXQ_OK;
     if (N > (int64_t(1) << 24) || M > (int64_t(1) << 30) || K > (int64_t(1) << 30) || N * nkb_of(K) >= (int64_t(1) << 30))
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": shape too large");
+    const size_t need = axq_linear_f8_workspace_size(x_dtype, K, N);
+    if (!workspace || workspace_bytes < need)
+        return fail(AXQ_ERR_WORKSPACE, std::string(fn) + ": workspace of " + std::to_string(need) + " bytes required");
+    // without features neither w nor x is read
+    if (int r = K ? check_ld(w_ld, K, "w", fn) : AXQ_OK) return r;
+    if (int r = K && packed ? check_ld(x_ld, K, "x", fn) : AXQ_OK) return r;
+    const int64_t x_span = packed ? codes_span(N, K, x_ld) : N * K * host_dtype_size(x_dtype);
+    if (int r = check_apart({{y, N * M * host_dtype_size(y_dtype), "y"}, {workspace, static_cast<int64_t>(need), "the workspace"}},
+                            {{bias, M * 4, "the bias"},
+                             {w_codes, K ? codes_span(M, K, w_ld) : 0, "w"},
+                             {w_scales, scales_span(M, K, kF8Block), "the scales of w"},
+                             {x, K ? x_span : 0, "x"},
+                             {packed ? x_scales : nullptr, scales_span(N, K, 1), "the scales of x"}},
+                            fn))
+        return r;
     if (int r = check_device_ptr(y, "y", fn)) return r;
     if (reinterpret_cast<uintptr_t>(y) % host_dtype_size(y_dtype))
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": y is not aligned to its element type");
@@ -129,22 +144,14 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
         if (int r = check_device_ptr(bias, "bias", fn)) return r;
         if (reinterpret_cast<uintptr_t>(bias) % 4) return fail(AXQ_ERR_INVALID, std::string(fn) + ": bias must be 4-byte aligned");
     }
-    const size_t need = axq_linear_f8_workspace_size(x_dtype, K, N);
-    if (!workspace || workspace_bytes < need)
-        return fail(AXQ_ERR_WORKSPACE, std::string(fn) + ": workspace of " + std::to_string(need) + " bytes required");
     if (int r = check_device_ptr(workspace, "workspace", fn)) return r;
     if (reinterpret_cast<uintptr_t>(workspace) % 256)
         return fail(AXQ_ERR_INVALID, std::string(fn) + ": workspace must be 256-byte aligned");
-    const int64_t y_span = N * M * host_dtype_size(y_dtype);
-    if (overlap(y, y_span, workspace, static_cast<int64_t>(need)) || (bias && overlap(y, y_span, bias, M * 4)))
-        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap the workspace or the bias");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     auto* ws = static_cast<uint8_t*>(workspace);
     int* err = reinterpret_cast<int*>(ws);
     if (K == 0) return status(f8_fill_bias_dispatch(y_dtype, y, bias, M, N, err, s), fn);
     if (int r = check_codes(w_codes, w_ld, w_scales, K, "w", fn)) return r;
-    if (overlap(y, y_span, w_codes, codes_span(M, K, w_ld)) || overlap(y, y_span, w_scales, scales_span(M, K, kF8Block)))
-        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap w");
     F8Linear l{};
     l.w = w_codes;
     l.w_scales = w_scales;
@@ -158,8 +165,6 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
     l.err = err;
     if (packed) {
         if (int r = check_codes(x, x_ld, x_scales, K, "x", fn)) return r;
-        if (overlap(y, y_span, x, codes_span(N, K, x_ld)) || overlap(y, y_span, x_scales, scales_span(N, K, 1)))
-            return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap x");
         l.x = x;
         l.x_scales = x_scales;
         l.x_ld = x_ld;
@@ -169,8 +174,6 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
         if (int r = check_device_ptr(x, "x", fn)) return r;
         if (reinterpret_cast<uintptr_t>(x) % host_dtype_size(x_dtype))
             return fail(AXQ_ERR_INVALID, std::string(fn) + ": x is not aligned to its element type");
-        if (overlap(y, y_span, x, N * K * host_dtype_size(x_dtype)))
-            return fail(AXQ_ERR_INVALID, std::string(fn) + ": y must not overlap x");
         if (f8_gemm_packs(M, K, N)) {
             l.x = x;
             return status(f8_gemm_unpacked_dispatch(l, x_dtype, s), fn);

@@ -283,8 +283,8 @@ int axq_dequantize_f8(const void* codes, int64_t ld, const float* scales, int bl
  * 128 x 128 blocks.  x is [tokens x in_features] in x_dtype: F32, F16 or BF16
  * (row-major, x_ld = in_features, x_scales NULL; packed into 1 x 128 blocks by
  * the call, as axq_quantize_f8 does), or F8 (already packed so, x_ld its row
- * stride).  Sums are fp32; the result is rounded once.  y
- * overlaps no operand.  The workspace holds the status word and the packed x
+ * stride).  Sums are fp32; the result is rounded once.  y and the workspace
+ * overlap neither an operand nor each other.  The workspace holds the status word and the packed x
  * (256-byte aligned; calls that share one must be ordered); a bounded wait that
  * gave up is reported by axq_workspace_status. */
 size_t axq_linear_f8_workspace_size(int x_dtype, int64_t in_features, int64_t tokens);

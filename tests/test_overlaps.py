@@ -23,3 +23,33 @@ def test_quantize_f8_padding():
     assert call(c, c + 124, ld=256) and not call(c, c + 128, ld=256)
     assert call(c, c + 256 + 124, rows=2, ld=256, block_rows=128)
     assert call(c, 3 * AT, src=c + 8) and not call(c, 3 * AT, src=c + 16) and call(c, 3 * AT, src=3 * AT)
+
+
+def test_linear_f8():
+    """Neither y nor the workspace may share memory with an operand or with the other."""
+    L = ax.lib()
+    names = ("w", "ws", "x", "xs", "bias", "y", "work")
+    M, K, N = 256, 256, 4
+
+    def call(x_type, **at):
+        p = {n: (i + 1) * 16 * AT for i, n in enumerate(names)}
+        p.update(at)
+        packed = x_type == 3
+        return _refused(L.axq_linear_f8(p["w"], K, p["ws"], x_type, p["x"], K, p["xs"] if packed else None, p["bias"], 0, p["y"],
+                                        M, K, N, p["work"], 1 << 20, None))
+
+    at = {n: (i + 1) * 16 * AT for i, n in enumerate(names)}
+    size = {"w": M * K, "ws": 4 * 4, "xs": N * 2 * 4, "bias": 4 * M}
+    for x_type, x_size in ((0, 4 * N * K), (2, 2 * N * K), (3, N * K)):
+        assert not call(x_type)
+        work = L.axq_linear_f8_workspace_size(x_type, K, N)
+        for n, nbytes in {**size, "x": x_size, "work": work}.items():
+            if n == "xs" and x_type != 3:
+                continue
+            assert call(x_type, y=at[n] + nbytes - 4) and call(x_type, y=at[n] - 4 * N * M + 4), (x_type, n)
+            assert not call(x_type, y=at[n] + nbytes) and not call(x_type, y=at[n] - 4 * N * M), (x_type, n)
+            if n != "work":
+                assert call(x_type, work=at[n] + nbytes - 1) and call(x_type, work=at[n] - work + 1), (x_type, n)
+                assert not call(x_type, work=at[n] + nbytes) and not call(x_type, work=at[n] - work), (x_type, n)
+    # operands that are only read may be the same memory
+    assert not call(3, x=at["w"], xs=at["ws"], bias=at["ws"])
