@@ -70,6 +70,11 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
     if (top_k > experts) return fail(AXQ_ERR_INVALID, std::string(fn) + ": top_k is larger than the number of experts");
     if (tokens == 0) return AXQ_OK;
     if (hidden == 0) return fail(AXQ_ERR_INVALID, std::string(fn) + ": hidden must be positive");
+    // a token's choices are written while other blocks still read x and the router
+    const int64_t choices = tokens * top_k * 4;
+    if (int r = check_apart({{ids, choices, "ids"}, {weights, choices, "weights"}},
+                            {{x, tokens * hidden * host_dtype_size(dtype), "x"}, {w_router, experts * hidden * 4, "w_router"}}, fn))
+        return r;
     if (int r = check_aligned(x, "x", host_dtype_size(dtype), fn)) return r;
     if (int r = check_aligned(w_router, "w_router", 4, fn)) return r;
     if (int r = check_aligned(ids, "ids", 4, fn)) return r;

@@ -304,7 +304,8 @@ int axq_linear_f8(const void* w_codes, int64_t w_ld, const float* w_scales, int 
  * softmax(x . W_router^T), largest first, ties to the lowest index (NaN logits
  * last): x [tokens x hidden] in dtype F32, F16 or BF16, w_router [experts x hidden]
  * fp32, both row-major.  normalize != 0: a token's weights are divided by their
- * sum.  Logits and softmax are fp32. */
+ * sum.  Logits and softmax are fp32.  ids and weights overlap
+ * neither each other nor x or w_router. */
 int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids, float* weights, int64_t tokens,
                   int64_t experts, int64_t top_k, int64_t hidden, int normalize, axq_stream_t stream);
 

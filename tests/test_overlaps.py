@@ -53,3 +53,23 @@ def test_linear_f8():
                 assert not call(x_type, work=at[n] + nbytes) and not call(x_type, work=at[n] - work), (x_type, n)
     # operands that are only read may be the same memory
     assert not call(3, x=at["w"], xs=at["ws"], bias=at["ws"])
+
+
+def test_moe_route():
+    L = ax.lib()
+    T, E, K, H = 5, 8, 2, 96
+    at = {n: (i + 1) * AT for i, n in enumerate(("x", "router", "ids", "p"))}
+
+    def call(dtype=0, **kw):
+        p = {**at, **kw}
+        return _refused(L.axq_moe_route(dtype, p["x"], p["router"], p["ids"], p["p"], T, E, K, H, 1, None))
+
+    out = 4 * T * K
+    assert not call()
+    for dtype, size in ((0, 4), (1, 2)):
+        for n, nbytes in (("x", size * T * H), ("router", 4 * E * H)):
+            for o in ("ids", "p"):
+                assert call(dtype, **{o: at[n] + nbytes - 4}) and call(dtype, **{o: at[n] - out + 4})
+                assert not call(dtype, **{o: at[n] + nbytes}) and not call(dtype, **{o: at[n] - out})
+    assert call(ids=at["p"] + out - 4) and not call(ids=at["p"] + out)
+    assert not call(x=at["router"])
