@@ -104,16 +104,38 @@ static int moe_call(const char* fn, int fmt, const void* w_gate, const float* ga
     if (tokens == 0 || hidden == 0) return AXQ_OK;
     if ((fmt == AXQ_F8_E4M3 || fmt_down == AXQ_F8_E4M3) && (hidden % kF8Block || ffn % kF8Block))
         return fail(AXQ_ERR_UNSUPPORTED, std::string(fn) + ": e4m3 experts need hidden and ffn to be multiples of 128");
+    // without hidden features (ffn 0) neither the experts' weights nor the workspace are looked at
+    const size_t need = ffn ? axq_moe_workspace_size(tokens, top_k, hidden, ffn) : 0;
+    if (ffn && (!workspace || workspace_bytes < need))
+        return fail(AXQ_ERR_WORKSPACE, std::string(fn) + ": workspace of " + std::to_string(need) + " bytes required");
+    const int64_t gate_bytes = ffn ? packed_bytes(fmt, experts * ffn, hidden) : 0;
+    const int64_t down_bytes = ffn ? packed_bytes(fmt_down, experts * hidden, ffn) : 0;
+    if (gate_bytes < 0 || down_bytes < 0) return fail(AXQ_ERR_INVALID, std::string(fn) + ": shape too large");
+    const int64_t row = hidden * host_dtype_size(dtype), choices = tokens * top_k * 4;
+    const int64_t scales = experts * (ffn / kF8Block) * (hidden / kF8Block) * 4;  // of an e4m3 matrix
+    // ids and weights are written where there is a router, else read
+    if (int r = check_apart({{y, tokens * row, "y"},
+                             {workspace, static_cast<int64_t>(need), "the workspace"},
+                             {w_router ? ids : nullptr, choices, "ids"},
+                             {w_router ? weights : nullptr, choices, "weights"}},
+                            {{x, tokens * row, "x"},
+                             {w_router, experts * hidden * 4, "w_router"},
+                             {w_router ? nullptr : ids, choices, "ids"},
+                             {w_router ? nullptr : weights, choices, "weights"},
+                             {w_gate, gate_bytes, "w_gate"},
+                             {w_up, gate_bytes, "w_up"},
+                             {w_down, down_bytes, "w_down"},
+                             {gate_scales, scales, "the scales of w_gate"},
+                             {up_scales, scales, "the scales of w_up"},
+                             {down_scales, scales, "the scales of w_down"}},
+                            fn))
+        return r;
     if (int r = check_aligned(y, "y", host_dtype_size(dtype), fn)) return r;
     if (int r = check_aligned(x, "x", host_dtype_size(dtype), fn)) return r;
     if (int r = check_aligned(ids, "ids", 4, fn)) return r;
     if (int r = check_aligned(weights, "weights", 4, fn)) return r;
     if (w_router)
         if (int r = check_aligned(w_router, "w_router", 4, fn)) return r;
-    const int64_t y_span = tokens * hidden * host_dtype_size(dtype), choices = tokens * top_k * 4;
-    if (overlap(y, y_span, x, y_span) || overlap(y, y_span, ids, choices) || overlap(y, y_span, weights, choices) ||
-        (w_router && overlap(ids, choices, weights, choices)))
-        return fail(AXQ_ERR_INVALID, std::string(fn) + ": y, x, ids and weights must not overlap");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (ffn == 0) {
         if (w_router) {
@@ -126,9 +148,6 @@ static int moe_call(const char* fn, int fmt, const void* w_gate, const float* ga
     if (int r = check_weights(fmt, w_gate, gate_scales, "w_gate", fn)) return r;
     if (int r = check_weights(fmt, w_up, up_scales, "w_up", fn)) return r;
     if (int r = check_weights(fmt_down, w_down, down_scales, "w_down", fn)) return r;
-    const size_t need = axq_moe_workspace_size(tokens, top_k, hidden, ffn);
-    if (!workspace || workspace_bytes < need)
-        return fail(AXQ_ERR_WORKSPACE, std::string(fn) + ": workspace of " + std::to_string(need) + " bytes required");
     if (int r = check_aligned(workspace, "workspace", 256, fn)) return r;
     MoeMlp m{};
     m.fmt = fmt;
@@ -139,9 +158,8 @@ static int moe_call(const char* fn, int fmt, const void* w_gate, const float* ga
     m.s_gate = gate_scales;
     m.s_up = up_scales;
     m.s_down = down_scales;
-    m.gate_bytes = packed_bytes(fmt, experts * ffn, hidden);
-    m.down_bytes = packed_bytes(fmt_down, experts * hidden, ffn);
-    if (m.gate_bytes < 0 || m.down_bytes < 0) return fail(AXQ_ERR_INVALID, std::string(fn) + ": shape too large");
+    m.gate_bytes = gate_bytes;
+    m.down_bytes = down_bytes;
     m.dtype = dtype;
     m.x = x;
     m.w_router = w_router;

@@ -320,8 +320,8 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
  * hidden] in dtype F32, F16 or BF16.  Products and sums are fp32 (x and the hidden
  * activations enter the tensor cores as fp16: one term for 16-bit x, which it holds,
  * two of 22 bits for fp32 x and for the hidden activations); y is rounded once.  Tokens beyond 512 / top_k take several passes
- * over the experts; tokens, hidden and ffn are at most 2^20.  y
- * overlaps neither x nor ids nor weights.  Calls that share a workspace (256-byte
+ * over the experts; tokens, hidden and ffn are at most 2^20.  y and
+ * the workspace overlap neither an operand nor each other.  Calls that share a workspace (256-byte
  * aligned) must be ordered; its status is read by axq_workspace_status. */
 size_t axq_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t ffn);
 int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales,
@@ -331,7 +331,7 @@ int axq_moe_mlp(int fmt, const void* w_gate, const float* gate_scales, const voi
 
 /* The whole layer: axq_moe_route into ids and weights, then axq_moe_mlp, with the
  * router's kernel also preparing the activations (and, for up to 4 tokens, the
- * order of the experts). */
+ * order of the experts).  ids and weights, which it writes, overlap nothing else. */
 int axq_moe(int fmt, const void* w_gate, const float* gate_scales, const void* w_up, const float* up_scales, int fmt_down,
             const void* w_down, const float* down_scales, int dtype, const void* x, const float* w_router, int normalize,
             int32_t* ids, float* weights, void* y, int64_t tokens, int64_t experts, int64_t top_k, int64_t hidden,

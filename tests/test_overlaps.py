@@ -73,3 +73,43 @@ def test_moe_route():
                 assert not call(dtype, **{o: at[n] + nbytes}) and not call(dtype, **{o: at[n] - out})
     assert call(ids=at["p"] + out - 4) and not call(ids=at["p"] + out)
     assert not call(x=at["router"])
+
+
+def _apart(call, at, sizes, written):
+    """Every range in `written` against every other: refused at the last and the first shared byte, else not."""
+    assert not call()
+    for o in written:
+        for n, nbytes in sizes.items():
+            if n != o:
+                assert call(**{o: at[n] + nbytes - 4}) and call(**{o: at[n] - sizes[o] + 4}), (o, n)
+                assert not call(**{o: at[n] + nbytes}) and not call(**{o: at[n] - sizes[o]}), (o, n)
+
+
+def test_moe_layer():
+    L = ax.lib()
+    T, E, K, H, F = 5, 8, 2, 256, 128
+    for fmt, gate, down in ((5, E * F * 144, E * H * 144), (64, E * F * H, E * H * F)):
+        f8 = fmt == 64
+        sizes = {"gate": gate, "up": gate, "down": down, "x": 4 * T * H, "router": 4 * E * H, "ids": 4 * T * K, "p": 4 * T * K,
+                 "y": 4 * T * H, "work": L.axq_moe_workspace_size(T, K, H, F)}
+        if f8:
+            sizes.update({n + "_s": 4 * E * (F // 128) * (H // 128) for n in ("gate", "up", "down")})
+        at = {n: (i + 1) * 64 * AT for i, n in enumerate(sizes)}
+
+        def weights(p):
+            return [v for n in ("gate", "up", "down") for v in ([fmt] if n != "up" else []) + [p[n], p.get(n + "_s")]]
+
+        def layer(**kw):
+            p = {**at, **kw}
+            return _refused(L.axq_moe(*weights(p), 0, p["x"], p["router"], 1, p["ids"], p["p"], p["y"], T, E, K, H, F, p["work"],
+                                      1 << 40, None))
+
+        def mlp(**kw):
+            p = {**at, **kw}
+            return _refused(L.axq_moe_mlp(*weights(p), 0, p["x"], p["ids"], p["p"], p["y"], T, E, K, H, F, p["work"], 1 << 40,
+                                          None))
+
+        _apart(layer, at, sizes, ("y", "work", "ids", "p"))
+        del sizes["router"]
+        _apart(mlp, at, sizes, ("y", "work"))
+        assert not mlp(up=at["gate"]) and not mlp(ids=at["x"])  # only read
