@@ -6,6 +6,10 @@ block (activations).  The reference (ruwwww/Axon) has no floating-point blocks.
 
 Scratch and outputs come from torch's caching allocator for the call's stream,
 one allocation per call: nothing is shared between streams or captured graphs.
+A call that is given a :class:`Workspace` takes its scratch there instead; calls
+that share one must be ordered, and its ``status`` says whether a kernel gave up
+a bounded wait (the call itself only enqueues work; without a workspace of the
+caller's there is nowhere to read that from).
 """
 from __future__ import annotations
 
@@ -16,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._capi import DType, F8_BLOCK, AxqError, Status, check, lib
-from .ops import _req_cuda
+from .ops import Workspace, _aligned_ptr, _req_cuda
 
 # element types as C ABI ids (plain ints: these run on every call)
 FLOAT_TYPES = {torch.float32: int(DType.F32), torch.float16: int(DType.F16), torch.bfloat16: int(DType.BF16)}
@@ -69,12 +73,13 @@ def _on(device: torch.device, stream: Optional[torch.cuda.Stream]):
     return both
 
 
-def _scratch(nbytes: int, like: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
-    """(tensor on `like`'s device, 256-byte aligned address, bytes from there)."""
-    buf = like.new_empty(nbytes + 256, dtype=torch.uint8)
-    p = buf.data_ptr()
-    off = -p % 256
-    return buf, p + off, nbytes + 256 - off
+def _scratch(nbytes: int, like: torch.Tensor, workspace: Optional[Workspace]):
+    """(tensor on `like`'s device, 256-byte aligned address, bytes from there); nothing for 0 bytes, so that a workspace
+    whose status no kernel would set is not made."""
+    if not nbytes:
+        return None, None, 0
+    buf = like.new_empty(nbytes + 256, dtype=torch.uint8) if workspace is None else workspace.get(nbytes + 256, like.device)
+    return (buf, *_aligned_ptr(buf))
 
 
 @dataclass
@@ -154,12 +159,13 @@ def dequantize_f8(dst: torch.Tensor, src: F8Tensor, stream: Optional[torch.cuda.
 
 
 def linear_f8(x, w: F8Tensor, out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
-              stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+              stream: Optional[torch.cuda.Stream] = None, workspace: Optional[Workspace] = None) -> torch.Tensor:
     """Linear on e4m3 blocks: y[N, M] = x[N, K] . W[M, K]^T (+ bias[M], fp32).
 
     ``w`` is packed in 128 x 128 blocks.  ``x`` is fp32, fp16 or bf16 (packed in
     1 x 128 blocks by the call) or an :class:`F8Tensor` with ``block_rows`` 1.
-    The result has ``out``'s type, else x's (fp32 for a packed x); sums are fp32."""
+    The result has ``out``'s type, else x's (fp32 for a packed x); sums are fp32.
+    ``workspace``: scratch of the caller's, whose ``status`` may be asked for."""
     w._check("w")
     if w.block_rows != F8_BLOCK:
         raise _invalid("linear_f8: w must be packed in 128 x 128 blocks")
@@ -188,7 +194,7 @@ def linear_f8(x, w: F8Tensor, out: Optional[torch.Tensor] = None, bias: Optional
     on = _on(device, stream)
     if on is not None:
         with on:
-            return linear_f8(x, w, out, bias)
+            return linear_f8(x, w, out, bias, workspace=workspace)
     if out is None:
         out = xd.new_empty((N, M), dtype=y_type)
         out_type = FLOAT_TYPES[y_type]
@@ -197,7 +203,7 @@ def linear_f8(x, w: F8Tensor, out: Optional[torch.Tensor] = None, bias: Optional
         if out.shape != (N, M):
             raise _invalid(f"linear_f8: out must be [{N} x {M}]")
     L = lib()
-    buf, wp, wbytes = _scratch(L.axq_linear_f8_workspace_size(x_type, K, N), xd)
+    buf, wp, wbytes = _scratch(L.axq_linear_f8_workspace_size(x_type, K, N) if M and N else 0, xd, workspace)
     check(L.axq_linear_f8(w.data.data_ptr(), w.data.shape[1], w.scales.data_ptr(), x_type, xd.data_ptr(), x_ld, x_scales,
                           bias_ptr, out_type, out.data_ptr(), M, K, N, wp, wbytes, _raw_stream(device.index)))
     del buf

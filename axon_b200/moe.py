@@ -14,7 +14,7 @@ import torch
 
 from ._capi import BLOCK_BYTES, F8_BLOCK, F8_E4M3, check, lib
 from .f8 import F8Tensor, _float_type, _invalid, _on, _plain, _raw_stream, _same_device, _scratch
-from .ops import QTensor, _packed_bytes
+from .ops import QTensor, Workspace, _packed_bytes
 
 
 def _weights(w, rows: int, cols: int, name: str):
@@ -81,13 +81,14 @@ def _out(x: torch.Tensor, out: Optional[torch.Tensor], dtype: int) -> torch.Tens
 
 
 def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate, w_up, w_down, experts: int,
-              out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None,
+              workspace: Optional[Workspace] = None) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * W_down[e] . (silu(W_gate[e] . x[t]) * (W_up[e] . x[t])), e = ids[t, j].
 
     x [N, hidden] in fp32, fp16 or bf16; ids int32 [N, top_k] (an id outside
     0 .. experts - 1 adds nothing); w_gate and w_up [experts * ffn, hidden] in one
     format, w_down [experts * hidden, ffn].  Products and sums are fp32, y has x's
-    type."""
+    type.  ``workspace``: scratch of the caller's, whose ``status`` may be asked for."""
     dtype = _float_type(x, "x")
     _plain(ids, "ids", torch.int32)
     _plain(weights, "weights", torch.float32)
@@ -99,10 +100,10 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
     on = _on(device, stream)
     if on is not None:
         with on:
-            return moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, experts, out)
+            return moe_mlp_q(x, ids, weights, w_gate, w_up, w_down, experts, out, workspace=workspace)
     out = _out(x, out, dtype)
     L = lib()
-    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn), x)
+    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn) if n and hidden and ffn else 0, x, workspace)
     check(L.axq_moe_mlp(*w, dtype, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), out.data_ptr(), n, experts, top_k, hidden,
                         ffn, wp, wbytes, _raw_stream(device.index)))
     del buf
@@ -110,10 +111,10 @@ def moe_mlp_q(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w_gate,
 
 
 def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: int, normalize: bool = True,
-          out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None
-          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+          out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None,
+          workspace: Optional[Workspace] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The whole layer: what :func:`moe_route` and then :func:`moe_mlp_q` give, in
-    fewer kernels.  Returns (y, ids, weights)."""
+    fewer kernels.  Returns (y, ids, weights).  ``workspace`` as there."""
     dtype = _float_type(x, "x")
     _plain(w_router, "w_router", torch.float32)
     if x.dim() != 2 or w_router.dim() != 2 or x.shape[1] != w_router.shape[1]:
@@ -124,12 +125,12 @@ def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: 
     on = _on(device, stream)
     if on is not None:
         with on:
-            return moe_q(x, w_router, w_gate, w_up, w_down, top_k, normalize, out)
+            return moe_q(x, w_router, w_gate, w_up, w_down, top_k, normalize, out, workspace=workspace)
     out = _out(x, out, dtype)
     ids = x.new_empty((n, top_k), dtype=torch.int32)
     weights = x.new_empty((n, top_k), dtype=torch.float32)
     L = lib()
-    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn), x)
+    buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn) if n and hidden and ffn else 0, x, workspace)
     check(L.axq_moe(*w, dtype, x.data_ptr(), w_router.data_ptr(), 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
                     out.data_ptr(), n, experts, top_k, hidden, ffn, wp, wbytes, _raw_stream(device.index)))
     del buf

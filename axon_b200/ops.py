@@ -26,6 +26,7 @@ from ._capi import (
     check,
     lib,
     quantized_size_2d,
+    workspace_status,
 )
 
 
@@ -148,6 +149,15 @@ class Workspace:
             buf = torch.empty(max(nbytes, 256) + 256, dtype=torch.uint8, device=f"cuda:{idx}")
             self._bufs[idx] = buf
         return buf
+
+    def status(self, stream: Optional[torch.cuda.Stream] = None) -> None:
+        """Wait for ``stream`` (else for each device's current one) and raise
+        (``Status.ERR_TIMEOUT``) if a kernel of the last call that used this
+        workspace gave up a bounded wait: its results are not valid then."""
+        for idx, buf in self._bufs.items():
+            if stream is None or stream.device_index == idx:
+                with torch.cuda.device(idx):
+                    workspace_status(_aligned_ptr(buf)[0], _stream_handle(stream, buf.device))
 
 
 _default_ws = Workspace()
