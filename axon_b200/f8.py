@@ -67,6 +67,8 @@ def _on(device: torch.device, stream: Optional[torch.cuda.Stream]):
     belongs to its stream)."""
     if stream is None:
         return None if device.index == _current_device() else torch.cuda.device(device)
+    if stream.device_index != device.index:
+        raise _invalid(f"stream is on cuda:{stream.device_index}, not on {device}")
     both = contextlib.ExitStack()
     both.enter_context(torch.cuda.device(device))
     both.enter_context(torch.cuda.stream(stream))
