@@ -34,6 +34,16 @@ def _weights(w, rows: int, cols: int, name: str):
     return int(w.fmt), w.data, None
 
 
+def _choices(x: torch.Tensor, experts: int, top_k: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(ids, weights) of x's tokens, to be written."""
+    if top_k < 1:
+        raise _invalid(f"top_k must be positive (got {top_k})")
+    if top_k > experts:
+        raise _invalid(f"top_k is larger than the number of experts ({top_k} of {experts})")
+    shape = (x.shape[0], top_k)
+    return x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
+
+
 def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bool = True,
               stream: Optional[torch.cuda.Stream] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(ids int32 [N, top_k], weights fp32 [N, top_k]) of the top_k largest of
@@ -51,10 +61,8 @@ def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bo
     if on is not None:
         with on:
             return moe_route(x, w_router, top_k, normalize)
-    n = x.shape[0]
-    ids = x.new_empty((n, top_k), dtype=torch.int32)
-    weights = x.new_empty((n, top_k), dtype=torch.float32)
-    check(lib().axq_moe_route(dtype, x.data_ptr(), w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), n,
+    ids, weights = _choices(x, w_router.shape[0], top_k)
+    check(lib().axq_moe_route(dtype, x.data_ptr(), w_router.data_ptr(), ids.data_ptr(), weights.data_ptr(), x.shape[0],
                               w_router.shape[0], top_k, x.shape[1], 1 if normalize else 0, _raw_stream(device.index)))
     return ids, weights
 
@@ -127,8 +135,7 @@ def moe_q(x: torch.Tensor, w_router: torch.Tensor, w_gate, w_up, w_down, top_k: 
         with on:
             return moe_q(x, w_router, w_gate, w_up, w_down, top_k, normalize, out, workspace=workspace)
     out = _out(x, out, dtype)
-    ids = x.new_empty((n, top_k), dtype=torch.int32)
-    weights = x.new_empty((n, top_k), dtype=torch.float32)
+    ids, weights = _choices(x, experts, top_k)
     L = lib()
     buf, wp, wbytes = _scratch(L.axq_moe_workspace_size(n, top_k, hidden, ffn) if n and hidden and ffn else 0, x, workspace)
     check(L.axq_moe(*w, dtype, x.data_ptr(), w_router.data_ptr(), 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
