@@ -26,8 +26,8 @@ def _weights(w, rows: int, cols: int, name: str):
         if w.block_rows != F8_BLOCK or w.data.shape[1] != cols:
             raise _invalid(f"{name}: e4m3 experts are packed in 128 x 128 blocks, their rows without padding")
         return F8_E4M3, w.data, w.scales.data_ptr()
-    if not isinstance(w, QTensor) or w.fmt not in BLOCK_BYTES:
-        raise _invalid(f"{name} must be a QTensor or an F8Tensor")
+    if w.fmt not in BLOCK_BYTES:
+        raise _invalid(f"{name} must be in a block format (got {w.fmt})")
     _plain(w.data, name, torch.uint8)
     if w.data.numel() < _packed_bytes(rows, cols, w.fmt):
         raise _invalid(f"{name} is smaller than its shape")
@@ -69,6 +69,9 @@ def moe_route(x: torch.Tensor, w_router: torch.Tensor, top_k: int, normalize: bo
 
 def _experts(w_gate, w_up, w_down, experts: int, hidden: int):
     """(ffn, their arguments of the C entry points, their tensors)."""
+    for w, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
+        if not isinstance(w, (QTensor, F8Tensor)):
+            raise _invalid(f"{name} must be a QTensor or an F8Tensor")
     if experts < 1 or w_gate.shape[0] % experts:
         raise _invalid("w_gate must have experts * ffn rows")
     ffn = w_gate.shape[0] // experts

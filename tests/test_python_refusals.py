@@ -27,3 +27,19 @@ def test_number_of_choices():
             moe._choices(x, 4, k)
     ids, weights = moe._choices(x, 4, 4)
     assert ids.shape == weights.shape == (3, 4) and ids.dtype == torch.int32 and weights.dtype == torch.float32
+
+
+def test_kinds_of_weights():
+    from axon_b200 import moe
+
+    q = ax.QTensor.empty(8, 32, ax.QuantFormat.Q8_0, device="cpu")
+    d = ax.QTensor.empty(2 * 32, 4, ax.QuantFormat.Q8_0, device="cpu")
+    for bad in (None, [1], torch.zeros(8, 32)):
+        for at, name in enumerate(("w_gate", "w_up", "w_down")):
+            w = [q, q, d]
+            w[at] = bad
+            with pytest.raises(ax.AxqError, match=f"{name} must be a QTensor or an F8Tensor"):
+                moe._experts(*w, 2, 32)
+    none = ax.QTensor(q.data, (8, 32), ax.QuantFormat.NONE)
+    with pytest.raises(ax.AxqError, match="block format"):
+        moe._experts(none, q, d, 2, 32)
