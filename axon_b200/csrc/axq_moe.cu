@@ -439,18 +439,31 @@ struct ActLines {
     }
 };
 
+// Pairs of MMAs whose sums follow one another in the tensor core before fp32
+// registers take them.  Its additions truncate, always toward zero, so a long chain
+// loses bits: fp32 layers of 256-element formats were 1 to 2.4e-6 off with all 16 or
+// (Q6_K) 32 MMAs of a CG in one chain, up to 1.3e-6 with half of it, 0.8 with a
+// quarter, 0.64 with an eighth, where fp32 alone gives 0.2 to 1.6.  EX, for results in
+// fp32: four MMAs (Q4_K / Q6_K, 4 tokens: 173 -> 183 us; Q3_K / Q5_K, 33 tokens, whose
+// two blocks of columns leave few registers: 143 -> 166); results of 16 bits show none
+// of it.
+template <int F, bool EX>
+constexpr int kChain = !EX ? 8 : F == F_Q6_K ? 1 : 2;
+
 // One CG of TL tiles (rows g and g + 8 of tile t at p[t][0], p[t][1]) times NB
 // blocks of eight columns: tot[t][n][r][u] += row r's product with this lane's
 // u-th token of block n (see Cols).
 // Tiles taken together share the loads of the activations, whose first kAhead
 // lines are in `x`.
-template <int F, int T, int NB, int TL>
+template <int F, int T, int NB, bool EX, int TL>
 __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int g, int i, const uint8_t* const (&rec)[NB],
                                        ActLines<F, T, NB>& x, const float (&xs)[NB][Cols<T>::kOwn], int blocks,
                                        const float* const* wsc, float (*tot)[NB][2][Cols<T>::kOwn]) {
     using C = Cols<T>;
+    constexpr int kPairs = kChain<F, EX>;
     MoeRow<F> r[TL][2];
     float acc[TL][NB][4];
+    [[maybe_unused]] float part[TL][NB][4];  // the chain of MMAs at work
 #pragma unroll
     for (int t = 0; t < TL; ++t) {
         r[t][0].load(p[t][0], i);
@@ -467,7 +480,19 @@ __device__ __forceinline__ void moe_cg(const uint8_t* const (*p)[2], int g, int 
         for (int n = 0; n < NB; ++n) b[n] = x.b[n][MP % (D + 1)];
 #pragma unroll
         for (int t = 0; t < TL; ++t) {
-            moe_pair<F, MP, NB>(r[t], b, acc[t]);
+            if constexpr (kPairs < 8) {
+                if constexpr (MP % kPairs == 0)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) part[t][n][0] = part[t][n][1] = part[t][n][2] = part[t][n][3] = 0.0f;
+                moe_pair<F, MP, NB>(r[t], b, part[t]);
+                if constexpr (MP % kPairs == kPairs - 1)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[t][n][k] += part[t][n][k];
+            } else {
+                moe_pair<F, MP, NB>(r[t], b, acc[t]);
+            }
             if constexpr (F == F_Q8_0 || F == F_Q4_0 || (F == F_F8 && MP % 4 == 3)) {
                 // a block is done: its scales in fp32 (blocks past the row's end hold other rows' bytes)
                 constexpr int B = F == F_F8 ? MP / 4 : MP;
@@ -619,7 +644,7 @@ __device__ __forceinline__ void moe_results(const ExpertArgs& a, const float* rb
     }
 }
 
-template <int F, int T, int NB>
+template <int F, int T, int NB, bool EX>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid_constant__ ExpertArgs a) {
     using C = Cols<T>;
     constexpr int CGB = moe_cg_bytes<F>();
@@ -834,7 +859,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_expert_kernel(const __grid
                         }
                         wsc[t] = F == F_F8 ? a.sc[tile] + sc0 : nullptr;
                     }
-                    moe_cg<F, T, NB, TL>(p, g, i, rec, x, xs, blocks, wsc, tot + (TL == 2 ? 0 : h));
+                    moe_cg<F, T, NB, EX, TL>(p, g, i, rec, x, xs, blocks, wsc, tot + (TL == 2 ? 0 : h));
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.empty[s]);
@@ -894,7 +919,7 @@ cudaError_t with_moe_fmt(int fmt, Fn&& f) {
     }
 }
 
-template <int F, int T, int NB>
+template <int F, int T, int NB, bool EX>
 cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     constexpr int CGB = moe_cg_bytes<F>();
     a.ncg = static_cast<int>((cols + 255) / 256);
@@ -931,19 +956,21 @@ cudaError_t launch_expert(ExpertArgs a, int64_t cols, cudaStream_t s) {
     if (a.stages < 2) return cudaErrorInvalidConfiguration;
     const int smem = a.stages * a.stage_bytes + red + 128;
     static std::atomic<int> cfg[64];
-    if (cudaError_t e = ensure_dyn_smem(moe_expert_kernel<F, T, NB>, smem, cfg); e != cudaSuccess) return e;
-    cudaError_t e = launch_pdl(moe_expert_kernel<F, T, NB>, dim3(static_cast<unsigned>(device_sm_count() * per_sm)),
+    if (cudaError_t e = ensure_dyn_smem(moe_expert_kernel<F, T, NB, EX>, smem, cfg); e != cudaSuccess) return e;
+    cudaError_t e = launch_pdl(moe_expert_kernel<F, T, NB, EX>, dim3(static_cast<unsigned>(device_sm_count() * per_sm)),
                                dim3(kMoeThreads), smem, s, a);
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 // One term: eight columns are up to 8 tokens.  Two terms: a block of columns is 4
 // tokens, and groups of up to 8 take two blocks.
-cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int terms, int group, cudaStream_t s) {
+cudaError_t launch_experts(int fmt, const ExpertArgs& a, int64_t cols, int terms, int group, bool exact, cudaStream_t s) {
     return with_moe_fmt(fmt, [&](auto f) {
         constexpr int F = decltype(f)::value;
-        return terms == 1 ? launch_expert<F, 1, 1>(a, cols, s)
-               : group == 4 ? launch_expert<F, 2, 1>(a, cols, s) : launch_expert<F, 2, 2>(a, cols, s);
+        constexpr bool kLong = Order<F>::SUMS > 0;  // the other formats' sums leave the tensor core after a block
+        if (terms == 1) return launch_expert<F, 1, 1, false>(a, cols, s);
+        if (kLong && exact) return group == 4 ? launch_expert<F, 2, 1, kLong>(a, cols, s) : launch_expert<F, 2, 2, kLong>(a, cols, s);
+        return group == 4 ? launch_expert<F, 2, 1, false>(a, cols, s) : launch_expert<F, 2, 2, false>(a, cols, s);
     });
 }
 
@@ -1022,6 +1049,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
     const int size = host_dtype_size(m.dtype);
     // 16-bit x is one term; fp32 x and the hidden activations, which are fp32 whatever the result's type, are two
     const int terms_x = m.dtype == AXQ_DT_F32 ? 2 : 1, terms_h = 2;
+    const bool exact = m.dtype == AXQ_DT_F32;
     const bool several = m.tokens > step;  // passes
     if (m.w_router && several) {
         cudaError_t e = moe_route_dispatch(m.dtype, m.x, m.w_router, m.ids, m.weights, m.tokens, m.experts, m.top_k, m.hidden,
@@ -1084,7 +1112,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.plan = plan;
         a.next = plan.taken;
         a.err = err;
-        if (e = launch_experts(m.fmt, a, m.hidden, terms_x, group, s); e != cudaSuccess) return e;
+        if (e = launch_experts(m.fmt, a, m.hidden, terms_x, group, exact, s); e != cudaSuccess) return e;
         RecordArgs rh{};
         rh.fmt = m.fmt_down;
         rh.terms = terms_h;
@@ -1106,7 +1134,7 @@ cudaError_t moe_mlp_dispatch(const MoeMlp& m, void* ws, int* err, cudaStream_t s
         a.rec_token = 0;
         a.out = z;
         a.next = plan.taken + 1;
-        if (e = launch_experts(m.fmt_down, a, m.ffn, terms_h, group, s); e != cudaSuccess) return e;
+        if (e = launch_experts(m.fmt_down, a, m.ffn, terms_h, group, exact, s); e != cudaSuccess) return e;
         const float* wt = m.weights + t0 * m.top_k;
         e = with_dtype(m.dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;

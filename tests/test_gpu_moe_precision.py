@@ -44,3 +44,26 @@ def test_bf16_result_is_rounded_once(cuda, orc, fmt):
     err = np.abs(got.double().cpu().numpy() - y)
     bound = tol + _half_step_bf16(np.abs(y) + tol)
     assert np.isfinite(err).all() and (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("fmt", ["Q2_K", "Q3_K", "Q4_K", "Q5_K", "Q6_K"])
+@pytest.mark.parametrize("T", [4, 24])
+def test_fp32_sums(cuda, orc, fmt, T):
+    """An fp32 layer as a whole (2-norms): the sums are fp32 in earnest, as a plain computation's.
+
+    An addition of the tensor core may truncate, by up to 2^-23 of the running sum and always toward zero.  Over four in a
+    row, the running sum growing as the square root, that is up to 3.1 * 2^-23 of the chain's sum and half of it on
+    average.  A chain covers 64 elements (32 of Q6_K); chains have signs and errors of their own, which add as squares, so
+    the sum of all is off by 1.5 * 2^-23 of itself.  Sums of codes are up to twice the size of what is left once their
+    offset is taken off, and three products follow one another: 2 * sqrt(3) * 1.5 * 2^-23 = 6.2e-7; with fp32's own
+    roundings beside that, less than 2^-20 (9.5e-7).  Sixteen or 32 additions in a row were off by 1.4 to 3.9e-6."""
+    rng = np.random.default_rng(50 + T)
+    E, K, hidden, ffn = 4, 2, 1024, 512
+    gate, up = (Weights(orc, fmt, E, ffn, hidden, rng) for _ in range(2))
+    down = Weights(orc, fmt, E, hidden, ffn, rng)
+    x = (rng.standard_normal((T, hidden)) / np.sqrt(hidden)).astype(np.float32)
+    ids = np.stack([rng.permutation(E)[:K] for _ in range(T)]).astype(np.int32)
+    p = rng.random((T, K)).astype(np.float32)
+    got = ax.moe_mlp_q(*(torch.from_numpy(v).cuda() for v in (x, ids, p)), _q(gate), _q(up), _q(down), experts=E)
+    y, _ = layer(x.astype(np.float64), ids, p, gate, up, down, 0.0)
+    assert np.linalg.norm(got.double().cpu().numpy() - y) <= 2.0 ** -20 * np.linalg.norm(y)
