@@ -8,9 +8,10 @@
 //
 // HBM-bound: every element is read once (the block stays in registers between
 // the maximum and the rounding) and one byte written.  Weights 28672 x 8192 fp32
-// take 234 us, 4.9 TB/s; activations 2500 x 8200 fp16 16 us (issue-bound: the
-// exact division is two FMAs and a product for each element); one row of 4096
-// 2.4 us, a launch.
+// take 234 us, 4.9 TB/s; activations 2500 x 8200 fp16 16 us, issue-bound: 18
+// instructions for an element, 3.5 of them the exact division and the conversion
+// to e4m3, the others conversions of the source, maxima, shuffles and addresses;
+// one row of 4096 2.4 us, a launch.
 #include <algorithm>
 
 #include "axq_common.cuh"

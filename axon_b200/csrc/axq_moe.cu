@@ -25,9 +25,12 @@
 //    most 8 columns the tensor pipe is idle most of the time either way.  Bound by
 //    the decoders' integer and fp16 instructions (3 per weight of Q4_K, 5.7 of
 //    Q6_K, 5 of Q3_K) at 55 to 60 % of the issue rate, which 20 warps of 96
-//    registers reach: 304 MB of Q4_K in 88 us (3.5 TB/s), 222 MB of Q6_K in 88, 114
-//    MB of Q3_K in 72; 185 MB of e4m3, which needs few instructions, in 39 (4.7
-//    TB/s).
+//    registers reach: 304 MB of Q4_K in 95 us (3.2 TB/s), 222 MB of Q6_K in 94 (fp32
+//    results; 88 and 88 without the joins of kChain, before which the other figures
+//    for four tokens in this file were taken), 114 MB of Q3_K in 72; 185 MB of e4m3,
+//    which needs few instructions, in 39 (4.7 TB/s).  At 96 registers most kernels
+//    spill a little, most of all Q6_K with two terms and two blocks of columns (168
+//    bytes stored, 208 loaded; the limit of 96 is what two CTAs an SM leave).
 //  * moe_combine_kernel: y from the experts' products, in the order of the
 //    token's choices (no atomics on values: results do not depend on timing).
 //    It, the plan and the hidden records take 2 to 5 us each, mostly their start.
@@ -54,8 +57,10 @@ namespace {
 // Record of one row and CG with T terms: eight lines (one for each pair of MMAs:
 // [term][lane part][16 bytes]), the sums as two terms [2][lane part][8 bytes],
 // the scale.
-// One term holds fp16 and bf16 activations exactly (down to 2^-33 of the largest
-// of the 256), two hold fp32 ones to 22 bits.
+// The largest of the 256 is scaled to 2^8 .. 2^9 and fp16's smallest step is 2^-24, so
+// every element is held to within 2^-33 of the largest.  Above that one term holds
+// 16-bit activations: exactly down to 2^-25 (bf16) or 2^-22 (fp16) of the largest; two
+// hold fp32 ones to 22 bits.
 template <int T> constexpr int kRecSums = 512 * T;
 template <int T> constexpr int kRecScale = kRecSums<T> + 64;
 template <int T> constexpr int kRec = (kRecScale<T> + 4 + 63) / 64 * 64;

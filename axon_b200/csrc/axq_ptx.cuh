@@ -1,7 +1,7 @@
 // Thin inline-PTX wrappers for sm_100a: mbarriers, 1-D bulk async copies
 // (TMA engine, no tensor map), and bounded waits.
 //
-// No cluster multicast is used anywhere in this library.
+// No load with cluster multicast is used anywhere in this library.
 #pragma once
 
 #include <cstdint>

@@ -1,6 +1,7 @@
 // tcgen05 (5th-generation tensor core) helpers for sm_100a: TMEM
 // allocation, shared-memory matrix descriptors, f16 MMA issue/commit and
-// TMEM loads.  Inline PTX only; no cluster multicast.
+// TMEM loads, tensor-map copies.  Inline PTX only; no load with cluster
+// multicast (a CTA pair's commit signals both CTAs by that name: an arrival).
 #pragma once
 
 #include <cstdint>

@@ -283,7 +283,9 @@ int axq_dequantize_f8(const void* codes, int64_t ld, const float* scales, int bl
  * 128 x 128 blocks.  x is [tokens x in_features] in x_dtype: F32, F16 or BF16
  * (row-major, x_ld = in_features, x_scales NULL; packed into 1 x 128 blocks by
  * the call, as axq_quantize_f8 does), or F8 (already packed so, x_ld its row
- * stride).  Sums are fp32; the result is rounded once.  y and the workspace
+ * stride).  Sums are fp32 (a block's two scales are multiplied first, in fp32:
+ * pairs whose product leaves its normal range, 2^-126 .. 2^128, lose bits or
+ * overflow); the result is rounded once.  y and the workspace
  * overlap neither an operand nor each other.  The workspace holds the status word and the packed x
  * (256-byte aligned; calls that share one must be ordered); a bounded wait that
  * gave up is reported by axq_workspace_status. */
@@ -318,8 +320,9 @@ int axq_moe_route(int dtype, const void* x, const float* w_router, int32_t* ids,
  * the rows are codes without padding and *_scales their 128 x 128 scales (hidden
  * and ffn multiples of 128); otherwise *_scales are NULL.  x and y are [tokens x
  * hidden] in dtype F32, F16 or BF16.  Products and sums are fp32 (x and the hidden
- * activations enter the tensor cores as fp16: one term for 16-bit x, which it holds,
- * two of 22 bits for fp32 x and for the hidden activations); y is rounded once.  Tokens beyond 512 / top_k take several passes
+ * activations enter the tensor cores as fp16: one term for 16-bit x, two of 22 bits
+ * for fp32 x and for the hidden activations, each element of 256 neighbours to within
+ * 2^-33 of the largest of them); y is rounded once.  Tokens beyond 512 / top_k take several passes
  * over the experts; tokens, hidden and ffn are at most 2^20.  y and
  * the workspace overlap neither an operand nor each other.  Calls that share a workspace (256-byte
  * aligned) must be ordered; its status is read by axq_workspace_status. */
